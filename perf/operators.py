@@ -105,6 +105,11 @@ def _gen(seed):
     return g
 
 
+def _pow2(p):
+    """2^p in float32, p whole and in -127..127: from the bits, exactly."""
+    return torch.where(p < -126, 2.0 ** -127, ((p + 127).clamp_min(1) << 23).view(torch.float32))
+
+
 def _mx_codes(v):
     """float32 ``(..., K)`` -> (E2M1 codes int32 ``(..., K)``, scale bytes int32
     ``(..., K / 32)``): the scale is the largest magnitude's power of two over
@@ -114,7 +119,7 @@ def _mx_codes(v):
     top = v.abs().amax(-1, keepdim=True)
     field = (top.view(torch.int32) >> 23) & 255       # floor(log2) + 127
     e = (field - 2).clamp_min(0)
-    q = torch.ldexp(v, 127 - e)
+    q = v * _pow2(127 - e)
     a = q.abs()
     code = ((a > 0.25).int() + (a >= 0.75).int() + (a > 1.25).int() + (a >= 1.75).int()
             + (a > 2.5).int() + (a >= 3.5).int() + (a > 5).int())
@@ -127,10 +132,9 @@ def _mx_codes(v):
 def _mx_values(code, e):
     """What codes and scale bytes stand for, in float32."""
     m = code & 7
-    a = torch.where(m < 2, m * 0.5, torch.ldexp(1 + 0.5 * (m & 1), (m >> 1) - 1))
+    a = torch.where(m < 2, m * 0.5, (1 + 0.5 * (m & 1)) * _pow2((m >> 1) - 1))
     a = torch.where(code > 7, -a, a)
-    s = torch.ldexp(torch.ones_like(e, dtype=torch.float32), e - 127)
-    s = torch.where(e == 255, math.nan, s)
+    s = torch.where(e == 255, math.nan, _pow2(e.clamp_max(254) - 127))
     return (a.reshape(*e.shape, 32) * s.unsqueeze(-1)).reshape(a.shape)
 
 
@@ -274,12 +278,16 @@ def work(case):
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
+def _pow2_64(p):
+    return ((p.long() + 1023) << 52).view(torch.float64)
+
+
 def _deq64(w, s):
     """The values of packed codes, by table, in float64 (finite scales)."""
     b = w.view(torch.int32).view(torch.uint8).long()
     table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), dtype=torch.float64, device=b.device)
     v = torch.stack([table[b % 16], table[b // 16]], dim=-1).reshape(*s.shape, 32)
-    return (v * torch.pow(2.0, s.double() - 127).unsqueeze(-1)).reshape(*s.shape[:-1], -1)
+    return (v * _pow2_64(s.long() - 127).unsqueeze(-1)).reshape(*s.shape[:-1], -1)
 
 
 def _round64(v):
@@ -287,14 +295,14 @@ def _round64(v):
     q = v.double().reshape(*v.shape[:-1], -1, 32)
     top = q.abs().amax(-1, keepdim=True)
     # frexp: top = f 2^p with f in [1/2, 1), so floor(log2(top)) = p - 1
-    p = torch.where(top == 0, -126.0, (torch.frexp(top).exponent - 3).double().clamp_min(-127))
-    a = q.abs() / torch.pow(2.0, p)
+    p = _pow2_64(torch.where(top == 0, -126, (torch.frexp(top).exponent - 3).clamp_min(-127)))
+    a = q.abs() / p
     grid = torch.tensor(_E2M1, dtype=torch.float64, device=q.device)
     mid = (grid[1:] + grid[:-1]) / 2
     i = torch.searchsorted(mid, a.contiguous())           # midpoints below a
     tie = (i < 7) & (a == mid[i.clamp_max(6)]) & (i % 2 == 1)
     i = i + tie
-    return (torch.copysign(grid[i], q) * torch.pow(2.0, p)).reshape(v.shape)
+    return (torch.copysign(grid[i], q) * p).reshape(v.shape)
 
 
 def exact(case, seed):
