@@ -431,6 +431,60 @@ int mq_moe_route(const float* logits, int32_t* idx, float* weights, int64_t rows
                  int64_t top_k, const void* x, const void* sgw, void* sgate, int64_t H, int dtype,
                  void* hip_stream);
 
+/*
+ * MXFP4 (OCP Microscaling formats v1.0; MLX's mode="mxfp4"): groups of 32
+ * values along K share a power of two, 2^(e - 127) with e one byte (255: NaN);
+ * a value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6, sign in bit 3) times it.
+ *   w       uint32 [N, K/8]   code j of word i = element 8 i + j at bit 4 j
+ *   scales  uint8 [N, K/32]   no biases
+ *   deq     T(code * 2^(e - 127)), rounded to nearest even
+ * K is a multiple of 32; w, scales, x and quantize's and dequantize's other
+ * arrays are 16-byte aligned.  Kernels read scales in whole 4-byte words: up to
+ * three bytes after an array that does not end on one.  No counterpart in the
+ * reference's kernels; its layers pass `mode` through to stock MLX
+ * (mlxturbo/kernels/dispatch.py:317-327).
+ *
+ * mq_mxfp4_quantize: w [N, K] of any of the three dtypes.  Per group, with max
+ * the largest magnitude: e = max(floor(log2(max)) - 2, -127) + 127, codes
+ * rounded to nearest, ties to even, saturating at 6; a group that holds a NaN or
+ * an infinity has e = 255 and zero codes.
+ * mq_mxfp4_dequantize: out [N, K] of any of the three dtypes.
+ */
+int mq_mxfp4_quantize(const void* w, uint32_t* wq, uint8_t* scales, int64_t N, int64_t K,
+                      int dtype, void* hip_stream);
+int mq_mxfp4_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, int64_t N,
+                        int64_t K, int dtype, void* hip_stream);
+
+/*
+ * out[M, N] = x[M, K] . deq(w)^T, summed in float and rounded once, dtype
+ * bfloat16 or float16 (deq in that type).  A row's result does not depend on M
+ * up to 64 rows.  MQ_EUNSUPPORTED: float32, or K beyond what a workgroup's
+ * tables hold (some 10^5); the caller dequantizes there.
+ */
+int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
+                    int64_t N, int64_t K, int dtype, void* hip_stream);
+
+/*
+ * mq_mxfp4_matmul with x quantized too: out = deq(q(x)) . deq(w)^T with q as
+ * mq_mxfp4_quantize, both operands entering the MFMAs as codes and scales (mx.qqmm,
+ * mode="mxfp4").
+ */
+int mq_mxfp4_qqmm(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
+                  int64_t N, int64_t K, int dtype, void* hip_stream);
+
+/*
+ * out[p, M, N] = x[lhs[p], M, K] . deq(w[rhs[p]])^T for p < P: mq_gather_qmm on
+ * an MXFP4 bank (w [E, N, K/8], scales [E, N, K/32]), with its index rules;
+ * pairs whose expert or x batch does not exist get zeros.  M <= 16, and E <=
+ * 2048 where a workspace is needed, else MQ_EUNSUPPORTED.  workspace holds
+ * mq_mxfp4_gather_qmm_workspace_size(P, M) bytes, 16-byte aligned.
+ */
+size_t mq_mxfp4_gather_qmm_workspace_size(int64_t P, int64_t M);
+int mq_mxfp4_gather_qmm(const void* x, const uint32_t* w, const uint8_t* scales,
+                        const int32_t* lhs_indices, const int32_t* rhs_indices, void* out,
+                        int64_t P, int64_t B, int64_t M, int64_t N, int64_t K, int64_t E,
+                        int dtype, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

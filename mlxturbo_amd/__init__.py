@@ -7,6 +7,7 @@ hand-written HIP kernels behind a C ABI (``include/mlxturbo_amd.h``):
 * :func:`gather_qmm`       - MoE expert gather
 * :func:`dequantize`       - bit-exact MLX affine dequantization (every width)
 * :func:`quantize`         - MLX affine quantization (``mx.quantize``)
+* :func:`qqmm`             - both operands quantized (MXFP4, ``mx.qqmm``)
 * :func:`gather_glu`       - fused MoE gate+up+SiLU at decode widths
 * :func:`moe_combine`      - MoE unsort + router weight + top-k sum epilogue
   (optionally merging the shared expert)
@@ -14,6 +15,9 @@ hand-written HIP kernels behind a C ABI (``include/mlxturbo_amd.h``):
   (one kernel at decode widths)
 * :func:`moe_route`        - MoE top-k routing with softmax weights and the
   shared-expert gate
+
+``mode="mxfp4"`` of quantize, dequantize, quantized_matmul and gather_qmm is the
+block-scaled 4-bit floating point format (:mod:`mlxturbo_amd.mx`).
 
 Module level (:mod:`mlxturbo_amd.nn`, :mod:`mlxturbo_amd.dispatch`): torch
 ``QuantizedLinear`` / ``QuantizedSwitchLinear`` / ``SwitchGLU`` on MLX-format
@@ -25,7 +29,7 @@ layers to another width (dequantize + quantize on the GPU).
 
 from . import checkpoint, dispatch, nn, rebit
 from .ops import (dequantize, gather_glu, gather_qmm, gather_qmm_combine, launch_count,
-                  moe_combine, moe_route, quantize, quantized_matmul, row_identity,
+                  moe_combine, moe_route, qqmm, quantize, quantized_matmul, row_identity,
                   set_row_identity)
 
 __version__ = "0.2.0"
@@ -33,5 +37,5 @@ __version__ = "0.2.0"
 __all__ = ["checkpoint", "rebit", "dequantize", "dispatch", "gather_glu", "gather_qmm",
            "gather_qmm_combine", "launch_count",
            "moe_combine", "moe_route",
-           "nn", "quantize", "quantized_matmul", "row_identity", "set_row_identity",
+           "nn", "qqmm", "quantize", "quantized_matmul", "row_identity", "set_row_identity",
            "__version__"]

@@ -48,6 +48,12 @@ EXPORTED = (
     "mq_moe_combine",
     "mq_moe_combine_shared",
     "mq_moe_route",
+    "mq_mxfp4_quantize",
+    "mq_mxfp4_dequantize",
+    "mq_mxfp4_matmul",
+    "mq_mxfp4_qqmm",
+    "mq_mxfp4_gather_qmm_workspace_size",
+    "mq_mxfp4_gather_qmm",
 )
 
 _lock = threading.Lock()
@@ -125,6 +131,18 @@ def _bind(lib: ctypes.CDLL) -> None:
                                           _i64, _i64, _i64, _i64, _int, _int, _int, _vp]
     lib.mq_moe_combine.restype = _int
     lib.mq_moe_combine.argtypes = [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]
+    lib.mq_mxfp4_quantize.restype = _int
+    lib.mq_mxfp4_quantize.argtypes = [_vp, _vp, _vp, _i64, _i64, _int, _vp]
+    lib.mq_mxfp4_dequantize.restype = _int
+    lib.mq_mxfp4_dequantize.argtypes = [_vp, _vp, _vp, _i64, _i64, _int, _vp]
+    lib.mq_mxfp4_matmul.restype = _int
+    lib.mq_mxfp4_matmul.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp]
+    lib.mq_mxfp4_qqmm.restype = _int
+    lib.mq_mxfp4_qqmm.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp]
+    lib.mq_mxfp4_gather_qmm_workspace_size.restype = _sz
+    lib.mq_mxfp4_gather_qmm_workspace_size.argtypes = [_i64, _i64]
+    lib.mq_mxfp4_gather_qmm.restype = _int
+    lib.mq_mxfp4_gather_qmm.argtypes = [_vp] * 6 + [_i64] * 6 + [_int, _vp, _sz, _vp]
 
 
 def lib() -> ctypes.CDLL:

@@ -58,6 +58,8 @@ UNITS = [("abi.hip", []), ("formats.hip", []), ("prep.hip", []), ("route.hip", [
     ("quad.hip", [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_BITS={bits}", "-mllvm",
                   "-amdgpu-mfma-vgpr-form"])
     for dt in (0, 1) for bits in (4, 8)
+] + [("mx_formats.hip", [])] + [
+    ("mx_skinny.hip", [f"-DMQ_INST_DT={dt}"]) for dt in (0, 1)
 ]
 
 _NOISE = ("packed-fp32-ops", "warning generated", "warnings generated")

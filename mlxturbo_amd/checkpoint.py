@@ -16,6 +16,8 @@ for a module left unquantized) -- how mixed-bit checkpoints record e.g. an
 rebit.py re-quantizes such classes in place).  A module with no entry whose
 tensor shapes disagree with the default bit width has its width inferred
 from the shapes (``weight_cols * 32 / (scales_cols * group_size)``).
+``"mode": "mxfp4"`` layers have uint8 ``scales`` and no ``biases``; an override
+in another width without a mode of its own is affine.
 
 Tensors are memory-mapped from the shards and copied to the device once;
 nothing is converted or repacked.
@@ -82,13 +84,18 @@ def quant_params(config: dict, prefix: str, weight_cols: int,
     override = q.get(prefix)
     if override is False:
         return None
-    gs = int(q.get("group_size", 64))
-    bits = int(q.get("bits", 4))
     mode = q.get("mode", "affine")
+    gs = int(q.get("group_size", 32 if mode == "mxfp4" else 64))
+    bits = int(q.get("bits", 4))
     if isinstance(override, dict):
+        own = override.get("mode")
+        if own is None and mode == "mxfp4" and (override.get("group_size", gs),
+                                                override.get("bits", bits)) != (gs, bits):
+            own = "affine"
+        if own is not None and own != mode:
+            mode, gs, bits = own, 32 if own == "mxfp4" else 64, 4
         gs = int(override.get("group_size", gs))
         bits = int(override.get("bits", bits))
-        mode = override.get("mode", mode)
     elif weight_cols * 32 != scales_cols * gs * bits:
         # no entry: infer the width from the shapes (mixed-bit checkpoints)
         num = weight_cols * 32

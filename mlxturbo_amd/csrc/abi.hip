@@ -11,6 +11,7 @@
 #include "combine.cuh"
 #include "dequant.cuh"
 #include "launch.h"
+#include "mx_launch.h"
 
 namespace {
 
@@ -141,6 +142,46 @@ int moe_combine_checked(const void* y, int64_t y_rows, const int32_t* inv, const
                                   reinterpret_cast<hipStream_t>(hip_stream), sgate, shared);
   if (rc) return fail(rc, "%s: no kernel for this configuration", what);
   return check_launch(what);
+}
+
+// ---- MXFP4 -------------------------------------------------------------------
+
+// Arguments every MXFP4 call shares; what: the packed words and their scales.
+int check_mx(const void* w, const void* scales, int64_t N, int64_t K, int dtype) {
+  if (!w || !scales) return fail(MQ_EINVAL, "w and scales must be non-null");
+  if (N < 0 || K <= 0) return fail(MQ_EINVAL, "invalid sizes N=%lld K=%lld", (long long)N, (long long)K);
+  if (K % mq::kMxGroup)
+    return fail(MQ_EINVAL, "K=%lld is not a multiple of the group of %d", (long long)K, mq::kMxGroup);
+  if (N > INT32_MAX || K > INT32_MAX) return fail(MQ_EINVAL, "dimension exceeds int32 range");
+  if (dtype != MQ_BFLOAT16 && dtype != MQ_FLOAT16 && dtype != MQ_FLOAT32)
+    return fail(MQ_EINVAL, "unknown dtype code %d", dtype);
+  if (!aligned16(w) || !aligned16(scales))
+    return fail(MQ_EINVAL, "w and scales must be 16-byte aligned");
+  return MQ_OK;
+}
+
+// The same of a product: x and out of a 16-bit type.
+int check_mx_product(const void* x, const void* w, const void* scales, const void* out, int64_t M,
+                     int64_t N, int64_t K, int dtype) {
+  const int rc = check_mx(w, scales, N, K, dtype);
+  if (rc) return rc;
+  if (!x || !out) return fail(MQ_EINVAL, "x and out must be non-null");
+  if (M < 0 || M > INT32_MAX) return fail(MQ_EINVAL, "invalid M=%lld", (long long)M);
+  if (dtype == MQ_FLOAT32)
+    return fail(MQ_EUNSUPPORTED, "float32 activations are not implemented on this path");
+  if (!aligned16(x)) return fail(MQ_EINVAL, "x must be 16-byte aligned");
+  if ((uintptr_t)out % 2) return fail(MQ_EINVAL, "out must be 2-byte aligned");
+  return MQ_OK;
+}
+
+// Counts nl launches, or turns a launcher's status or a launch error into one.
+int mx_done(int rc, int nl, const char* what) {
+  if (rc) return fail(rc, "%s: %s", what, rc > 0 ? hipGetErrorString((hipError_t)rc)
+                                                 : "no kernel for this configuration");
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail((int)e, "%s: launch failed: %s", what, hipGetErrorString(e));
+  g_launches.fetch_add((uint64_t)nl, std::memory_order_relaxed);
+  return MQ_OK;
 }
 
 }  // namespace
@@ -727,6 +768,92 @@ int mq_moe_route(const float* logits, int32_t* idx, float* weights, int64_t rows
                                 sg ? dtype : MQ_BFLOAT16, reinterpret_cast<hipStream_t>(hip_stream));
   if (rc) return fail(rc, "moe_route: no kernel for this configuration");
   return check_launch("moe_route");
+}
+
+int mq_mxfp4_quantize(const void* w, uint32_t* wq, uint8_t* scales, int64_t N, int64_t K,
+                      int dtype, void* hip_stream) {
+  const int rc = check_mx(wq, scales, N, K, dtype);
+  if (rc) return rc;
+  if (!w || !aligned16(w)) return fail(MQ_EINVAL, "w must be non-null and 16-byte aligned");
+  if (N == 0) return MQ_OK;
+  return mx_done(mq::launch_mx_quantize(w, wq, scales, N, K, dtype,
+                                        reinterpret_cast<hipStream_t>(hip_stream)),
+                 1, "mxfp4 quantize");
+}
+
+int mq_mxfp4_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, int64_t N,
+                        int64_t K, int dtype, void* hip_stream) {
+  const int rc = check_mx(wq, scales, N, K, dtype);
+  if (rc) return rc;
+  if (!out || !aligned16(out)) return fail(MQ_EINVAL, "out must be non-null and 16-byte aligned");
+  if (N == 0) return MQ_OK;
+  return mx_done(mq::launch_mx_dequantize(wq, scales, out, N, K, dtype,
+                                          reinterpret_cast<hipStream_t>(hip_stream)),
+                 1, "mxfp4 dequantize");
+}
+
+int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
+                    int64_t N, int64_t K, int dtype, void* hip_stream) {
+  int rc = check_mx_product(x, w, scales, out, M, N, K, dtype);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return MQ_OK;
+  hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+  int nl = 0;
+  rc = dtype == MQ_BFLOAT16
+           ? mq::MxSkinnyLaunch<mq::kBF16, false>::run(x, w, scales, out, M, N, K, st, &nl)
+           : mq::MxSkinnyLaunch<mq::kF16, false>::run(x, w, scales, out, M, N, K, st, &nl);
+  return mx_done(rc, nl, "mxfp4 quantized_matmul");
+}
+
+int mq_mxfp4_qqmm(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
+                  int64_t N, int64_t K, int dtype, void* hip_stream) {
+  int rc = check_mx_product(x, w, scales, out, M, N, K, dtype);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return MQ_OK;
+  hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+  int nl = 0;
+  rc = dtype == MQ_BFLOAT16
+           ? mq::MxSkinnyLaunch<mq::kBF16, true>::run(x, w, scales, out, M, N, K, st, &nl)
+           : mq::MxSkinnyLaunch<mq::kF16, true>::run(x, w, scales, out, M, N, K, st, &nl);
+  return mx_done(rc, nl, "mxfp4 qqmm");
+}
+
+size_t mq_mxfp4_gather_qmm_workspace_size(int64_t P, int64_t M) {
+  return mq::gather_workspace_bytes(P, M);
+}
+
+int mq_mxfp4_gather_qmm(const void* x, const uint32_t* w, const uint8_t* scales,
+                        const int32_t* lhs_indices, const int32_t* rhs_indices, void* out,
+                        int64_t P, int64_t B, int64_t M, int64_t N, int64_t K, int64_t E,
+                        int dtype, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  int rc = check_mx_product(x, w, scales, out, M, N, K, dtype);
+  if (rc) return rc;
+  if (!rhs_indices) return fail(MQ_EINVAL, "rhs_indices must be non-null");
+  if (P < 0 || E <= 0 || B < 0)
+    return fail(MQ_EINVAL, "invalid sizes P=%lld E=%lld B=%lld", (long long)P, (long long)E,
+                (long long)B);
+  if (!lhs_indices && P > 0 && (B <= 0 || P % B))
+    return fail(MQ_EINVAL,
+                "lhs_indices=NULL requires B to divide P (pair p reads x batch p / (P / B); "
+                "B=%lld P=%lld)",
+                (long long)B, (long long)P);
+  if (P > INT32_MAX || B > INT32_MAX || E > INT32_MAX || M > 16)
+    return fail(MQ_EUNSUPPORTED, "gather_qmm supports M <= 16 rows per pair");
+  if (P == 0 || M == 0 || N == 0) return MQ_OK;
+  const size_t need = mq::gather_workspace_bytes(P, M);
+  if (need && (workspace_bytes < need || !workspace || !aligned16(workspace)))
+    return fail(MQ_EINVAL, "workspace of %zu bytes, 16-byte aligned, needed", need);
+  if (need && E > mq::kGatherPrepMaxE)
+    return fail(MQ_EUNSUPPORTED, "more than %d pairs need E <= %d", mq::kGatherFusedMaxP,
+                mq::kGatherPrepMaxE);
+  hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+  int nl = 0;
+  rc = dtype == MQ_BFLOAT16
+           ? mq::MxGatherLaunch<mq::kBF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P, B,
+                                                M, N, K, E, workspace, st, &nl)
+           : mq::MxGatherLaunch<mq::kF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P, B,
+                                               M, N, K, E, workspace, st, &nl);
+  return mx_done(rc, nl, "mxfp4 gather_qmm");
 }
 
 }  // extern "C"

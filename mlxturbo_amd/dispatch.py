@@ -35,7 +35,7 @@ from typing import Any, Optional
 import torch
 
 from . import ops
-from .nn import QuantizedLinear
+from .nn import QQLinear, QuantizedLinear
 
 STOCK = "stock"
 SKINNY = "skinny"
@@ -146,10 +146,11 @@ def dispatch_scope():
 def enable(model: Any, *, active: bool = True):
     """Swap every :class:`QuantizedLinear` below ``model`` to the dispatched
     class in place (``__class__`` only; identity and buffers are kept).
-    Idempotent; ``active=False`` routes only inside :func:`dispatch_scope`."""
+    Idempotent; ``active=False`` routes only inside :func:`dispatch_scope`.
+    A :class:`~mlxturbo_amd.nn.QQLinear` has another product and is left alone."""
     for _, module in model.named_modules():
-        if isinstance(module, QuantizedLinear) and not isinstance(module,
-                                                                  DispatchedQuantizedLinear):
+        if isinstance(module, QuantizedLinear) and not isinstance(
+                module, (DispatchedQuantizedLinear, QQLinear)):
             module.__class__ = DispatchedQuantizedLinear
         if isinstance(module, DispatchedQuantizedLinear):
             module._mq_dispatch_always = active

@@ -12,6 +12,10 @@ Torch counterparts of the layers the reference routes through its kernels:
   qwen4_exp.py:1795-1802), including the ``_gather_sort`` path that sorts
   pairs by expert and passes ``sorted_indices=True`` (fused.py:2402-2418).
 
+With ``mode="mxfp4"`` the same layers hold block-scaled 4-bit weights (uint8
+``scales``, no ``biases``, groups of 32); :class:`QQLinear` (``mlx.nn.QQLinear``)
+brings its activations into that format as well.
+
 Every forward runs the HIP kernels; there is no CPU path.
 """
 
@@ -25,13 +29,16 @@ from . import ops
 
 
 def _check_quantized(weight: torch.Tensor, scales: torch.Tensor,
-                     biases: Optional[torch.Tensor], group_size: int, bits: int) -> int:
+                     biases: Optional[torch.Tensor], group_size: int, bits: int,
+                     mode: str = "affine") -> int:
     if weight.dtype != torch.uint32 and weight.dtype != torch.int32:
         raise ValueError(f"weight must hold packed uint32 words, got {weight.dtype}")
     k = weight.shape[-1] * 32 // bits
     if scales.shape[-1] * group_size != k:
         raise ValueError(
             f"scales last dim {scales.shape[-1]} x group_size {group_size} != K={k}")
+    if mode == "mxfp4" and biases is not None:
+        raise ValueError("mxfp4 weights have no biases")
     if biases is not None and biases.shape != scales.shape:
         raise ValueError("biases must have the shape of scales")
     return k
@@ -47,9 +54,11 @@ class QuantizedLinear(torch.nn.Module):
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor,
                  biases: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None,
-                 group_size: int = 64, bits: int = 4, mode: str = "affine"):
+                 group_size: Optional[int] = None, bits: Optional[int] = None,
+                 mode: str = "affine"):
         super().__init__()
-        self.input_dims = _check_quantized(weight, scales, biases, group_size, bits)
+        group_size, bits = ops._format(group_size, bits, mode)
+        self.input_dims = _check_quantized(weight, scales, biases, group_size, bits, mode)
         self.output_dims = weight.shape[0]
         self.group_size = group_size
         self.bits = bits
@@ -96,12 +105,15 @@ class QuantizedLinear(torch.nn.Module):
 
     @classmethod
     def from_linear(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
-                    group_size: int = 64, bits: int = 4) -> "QuantizedLinear":
+                    group_size: Optional[int] = None, bits: Optional[int] = None,
+                    mode: str = "affine") -> "QuantizedLinear":
         """Quantize a float weight ``[N, K]`` (``mlx.nn.QuantizedLinear.
         from_linear``): ``mx.quantize`` on the GPU; scales and biases keep
-        the weight's dtype."""
-        wq, s, b = ops.quantize(weight, group_size=group_size, bits=bits)
-        return cls(wq, s, b, bias=bias, group_size=group_size, bits=bits)
+        the weight's dtype (mxfp4: scales are bytes, no biases)."""
+        group_size, bits = ops._format(group_size, bits, mode)
+        wq, s, *b = ops.quantize(weight, group_size=group_size, bits=bits, mode=mode)
+        return cls(wq, s, b[0] if b else None, bias=bias, group_size=group_size, bits=bits,
+                   mode=mode)
 
     def dequantized_weight(self) -> torch.Tensor:
         """The layer's weight as ``mx.dequantize`` gives it, ``[N, K]``."""
@@ -111,6 +123,32 @@ class QuantizedLinear(torch.nn.Module):
     def extra_repr(self) -> str:
         return (f"input_dims={self.input_dims}, output_dims={self.output_dims}, "
                 f"group_size={self.group_size}, bits={self.bits}, mode={self.mode!r}")
+
+
+class QQLinear(QuantizedLinear):
+    """``mlx.nn.QQLinear`` in mode mxfp4: a quantized layer whose activations
+    are quantized too, ``qqmm(x, weight, scales)`` plus ``bias``."""
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor,
+                 biases: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                 group_size: Optional[int] = None, bits: Optional[int] = None,
+                 mode: str = "mxfp4"):
+        if mode != "mxfp4":
+            raise NotImplementedError(f"mode={mode!r}: QQLinear is mxfp4 on this path")
+        super().__init__(weight, scales, biases, bias, group_size, bits, mode)
+
+    def quantized_forward(self, x: torch.Tensor) -> torch.Tensor:
+        out = ops.qqmm(x, self.weight, self.scales, self.group_size, self.bits, self.mode)
+        return out if self.bias is None else out + self.bias
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.quantized_forward(x)
+
+    @classmethod
+    def from_linear(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                    group_size: Optional[int] = None, bits: Optional[int] = None,
+                    mode: str = "mxfp4") -> "QQLinear":
+        return super().from_linear(weight, bias, group_size, bits, mode)
 
 
 class QuantizedSwitchLinear(torch.nn.Module):
@@ -123,11 +161,13 @@ class QuantizedSwitchLinear(torch.nn.Module):
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor,
                  biases: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None,
-                 group_size: int = 64, bits: int = 4, mode: str = "affine"):
+                 group_size: Optional[int] = None, bits: Optional[int] = None,
+                 mode: str = "affine"):
         super().__init__()
         if weight.ndim != 3:
             raise ValueError("an expert bank weight is [E, N, K*bits/32]")
-        self.input_dims = _check_quantized(weight, scales, biases, group_size, bits)
+        group_size, bits = ops._format(group_size, bits, mode)
+        self.input_dims = _check_quantized(weight, scales, biases, group_size, bits, mode)
         self.num_experts, self.output_dims = weight.shape[0], weight.shape[1]
         self.group_size = group_size
         self.bits = bits
@@ -223,7 +263,8 @@ class SwitchGLU(torch.nn.Module):
 
     def _fused(self, pairs: int) -> bool:
         g, u = self.gate_proj, self.up_proj
-        return (self.fuse_gate_up and pairs < ops._GLU_FUSED_MAX_ROWS and g.bias is None
+        return (self.fuse_gate_up and g.mode == "affine"
+                and pairs < ops._GLU_FUSED_MAX_ROWS and g.bias is None
                 and u.bias is None and g.weight.shape == u.weight.shape
                 and (g.group_size, g.bits, g.mode) == (u.group_size, u.bits, u.mode))
 
@@ -277,7 +318,10 @@ class SwitchGLU(torch.nn.Module):
         if pre is not None:
             return pre.reshape(*lead, *pre.shape[1:]) if scores is None else \
                 pre.reshape(*lead, pre.shape[-1])
-        do_sort = idx.numel() >= self.SORT_THRESHOLD
+        # the mxfp4 gathers group unsorted pairs at every width
+        do_sort = (idx.numel() >= self.SORT_THRESHOLD
+                   and not all(m.mode == "mxfp4"
+                               for m in (self.gate_proj, self.up_proj, self.down_proj)))
         if do_sort:
             flat = idx.reshape(-1)
             order = torch.argsort(flat, stable=True)
@@ -311,4 +355,4 @@ class SwitchGLU(torch.nn.Module):
         return y
 
 
-__all__ = ["QuantizedLinear", "QuantizedSwitchLinear", "SwitchGLU"]
+__all__ = ["QQLinear", "QuantizedLinear", "QuantizedSwitchLinear", "SwitchGLU"]

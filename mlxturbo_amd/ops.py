@@ -16,8 +16,14 @@ MLX 0.32's operators as the reference calls them:
 * ``moe_combine`` - MoE unsort + router weight + top-k sum
   (kernels/moe_combine.py:160-195)
 
+* ``qqmm`` - mx.qqmm: activations and weights both quantized
+
+``mode="mxfp4"`` (:mod:`mlxturbo_amd.mx`): block-scaled 4-bit floating point
+codes, without biases, in quantize, dequantize, quantized_matmul, gather_qmm and
+qqmm; the fused mixture-of-experts operators compose those.
+
 Errors and coverage: genuinely invalid arguments raise ``ValueError`` as MLX
-does; non-affine modes raise ``NotImplementedError``.  Every affine
+does; modes other than affine and mxfp4 raise ``NotImplementedError``.  Every affine
 configuration returns a result, as the reference's wrappers do by falling
 back to ``mx.quantized_matmul`` (fast_qmm.py:356-362): the kernels take 4/8
 bits with bf16/fp16 activations in the scales' dtype, and the rest (other
@@ -80,6 +86,17 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _format(group_size: Optional[int], bits: Optional[int], mode: str):
+    """``(group_size, bits)`` with the mode's own where they are not given:
+    affine groups of 64 in 4 bits; mxfp4 is groups of 32 in 4 bits only."""
+    if mode == "mxfp4":
+        if group_size not in (None, _mx.GROUP_SIZE) or bits not in (None, _mx.BITS):
+            raise ValueError(f"mode='mxfp4' is groups of {_mx.GROUP_SIZE} in {_mx.BITS} bits, "
+                             f"got group_size={group_size}, bits={bits}")
+        return _mx.GROUP_SIZE, _mx.BITS
+    return 64 if group_size is None else group_size, 4 if bits is None else bits
+
+
 def _check_mode(mode: str, biases) -> None:
     if mode != "affine":
         raise NotImplementedError(
@@ -126,13 +143,18 @@ def _dtype_code(x_dtype: torch.dtype, s_dtype: torch.dtype) -> int:
     return _DTYPE_CODE[x_dtype]
 
 
-def quantize(w: torch.Tensor, group_size: int = 64, bits: int = 4, mode: str = "affine"):
+def quantize(w: torch.Tensor, group_size: Optional[int] = None, bits: Optional[int] = None,
+             mode: str = "affine"):
     """``mx.quantize(w, group_size, bits, mode="affine")``: returns
     ``(w_q, scales, biases)`` with ``w_q`` uint32 ``[..., K*bits/32]`` and
     scales/biases ``[..., K/group_size]`` in ``w``'s dtype, as the reference
     calls it when it requantizes a layer (mlxturbo/rebit.py:119) or builds
     test weights (kernels/moe_verify_gather.py:887).  One HIP kernel; the
-    per-group arithmetic is the C ABI's ``mq_quantize``."""
+    per-group arithmetic is the C ABI's ``mq_quantize``.  ``mode="mxfp4"``
+    returns ``(w_q, scales)``, the scales uint8 exponents (mq_mxfp4_quantize)."""
+    group_size, bits = _format(group_size, bits, mode)
+    if mode == "mxfp4":
+        return _mx.quantize(w)
     if mode != "affine":
         raise NotImplementedError(f"mode={mode!r}: only affine quantization is on this path")
     dev = _require_gpu(w)
@@ -186,10 +208,18 @@ def _requantize(w, scales, biases, from_group_size: int, from_bits: int, group_s
 
 
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: Optional[torch.Tensor] = None,
-               group_size: int = 64, bits: int = 4, mode: str = "affine") -> torch.Tensor:
+               group_size: Optional[int] = None, bits: Optional[int] = None,
+               mode: str = "affine", dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``mx.dequantize``: ``T(float(s)*q + float(b))`` bit-exact, dtype of
-    ``scales``, for every MLX width (2, 3, 4, 5, 6, 8 bits)."""
+    ``scales``, for every MLX width (2, 3, 4, 5, 6, 8 bits).  ``mode="mxfp4"``:
+    ``T(code * 2**(e - 127))`` in ``dtype`` (default bfloat16)."""
+    group_size, bits = _format(group_size, bits, mode)
+    if mode == "mxfp4":
+        return _mx.dequantize(w, scales, biases, dtype)
     _check_mode(mode, biases)
+    if dtype is not None and dtype != scales.dtype:
+        raise NotImplementedError(f"affine weights dequantize in their scales' dtype "
+                                  f"{scales.dtype}, not {dtype}")
     dev = _require_gpu(w, scales, biases)
     K = _check_quant(w, scales, biases, group_size, bits)
     if scales.dtype not in _DTYPE_CODE:
@@ -236,7 +266,8 @@ def _composed_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases
 
 def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
                      biases: Optional[torch.Tensor] = None, transpose: bool = True,
-                     group_size: int = 64, bits: int = 4, mode: str = "affine") -> torch.Tensor:
+                     group_size: Optional[int] = None, bits: Optional[int] = None,
+                     mode: str = "affine") -> torch.Tensor:
     """``mx.quantized_matmul``: ``x @ dequantize(w).T`` for ``x[..., K]``
     (``transpose=False``: ``x @ dequantize(w)`` with ``w`` quantized along N).
 
@@ -244,8 +275,12 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     (as mlxturbo/kernels/dispatch.py:332-382 does around its kernels).
     4- and 8-bit codes with bf16/fp16 activations in the scales' dtype run on
     the matmul kernels; every other MLX configuration runs as the library's
-    dequantize plus one GPU GEMM (:func:`_composed_qmm`).
+    dequantize plus one GPU GEMM (:func:`_composed_qmm`).  ``mode="mxfp4"``
+    (uint8 scales, no biases) takes the same x and gives x's dtype.
     """
+    group_size, bits = _format(group_size, bits, mode)
+    if mode == "mxfp4":
+        return _mx.quantized_matmul(x, w, scales, biases, transpose)
     _check_mode(mode, biases)
     dev = _require_gpu(x, w, scales, biases)
     if w.ndim != 2:
@@ -278,6 +313,20 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
                                     ws.numel() if ws is not None else 0, _stream_ptr(out))
     _lib.check(rc, "quantized_matmul")
     return out
+
+
+def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
+         group_size: Optional[int] = None, bits: Optional[int] = None,
+         mode: str = "mxfp4") -> torch.Tensor:
+    """``mx.qqmm``: ``x`` is quantized along its last axis in the weight's
+    format and multiplied there, ``dequantize(quantize(x)) @ dequantize(w).T``
+    with float sums, rounded once to x's dtype.  ``w`` ``[N, K/8]`` and
+    ``scales`` ``[N, K/32]`` are :func:`quantize`'s.  Both operands enter the
+    MFMAs as codes with their scales; the mode is mxfp4."""
+    _format(group_size, bits, mode)
+    if mode != "mxfp4":
+        raise NotImplementedError(f"mode={mode!r}: qqmm is mxfp4 on this path")
+    return _mx.qqmm(x, w, scales)
 
 
 class PreparedWeights:
@@ -450,6 +499,29 @@ def _as_index(t, dev) -> torch.Tensor:
     return t.to(device=dev)
 
 
+def _gather_pairs(dev, bx: tuple, bw: tuple, lhs_indices, rhs_indices):
+    """A gather's index pairs: ``(shape, P, lhs, rhs)``, the broadcast shape of
+    the indices over x's batch dims ``bx`` and w's ``bw``, its size, and both
+    flattened over it as int32 (lhs None where the kernels' own rule gives it;
+    both None when there is no pair)."""
+    lhs = None if lhs_indices is None else _as_index(lhs_indices, dev)
+    rhs = (torch.arange(math.prod(bw), device=dev, dtype=torch.int32).reshape(bw)
+           if rhs_indices is None else _as_index(rhs_indices, dev))
+    lshape = bx if lhs is None else tuple(lhs.shape)
+    try:
+        shape = tuple(torch.broadcast_shapes(lshape, rhs.shape))
+    except RuntimeError as exc:
+        raise ValueError(f"lhs_indices {lshape} and rhs_indices "
+                         f"{tuple(rhs.shape)} do not broadcast") from exc
+    P = math.prod(shape)
+    if P == 0:
+        return shape, P, None, None
+    lhs_f = (_default_lhs(dev, bx, shape) if lhs is None
+             else lhs.expand(shape).reshape(-1).to(torch.int32).contiguous())
+    rhs_f = rhs.expand(shape).reshape(-1).to(torch.int32).contiguous()
+    return shape, P, lhs_f, rhs_f
+
+
 def _gather_prep(x, banks, lhs_indices, rhs_indices, transpose, group_size, bits, mode,
                  alloc=True):
     """Validation and flattening shared by gather_qmm and gather_glu; ``banks``
@@ -482,22 +554,10 @@ def _gather_prep(x, banks, lhs_indices, rhs_indices, transpose, group_size, bits
     bw = tuple(w0.shape[:-2])
     B = math.prod(bx)
     E = math.prod(bw)
-    lhs = None if lhs_indices is None else _as_index(lhs_indices, dev)
-    rhs = (torch.arange(E, device=dev, dtype=torch.int32).reshape(bw) if rhs_indices is None
-           else _as_index(rhs_indices, dev))
-    lshape = bx if lhs is None else tuple(lhs.shape)
-    try:
-        shape = torch.broadcast_shapes(lshape, rhs.shape)
-    except RuntimeError as exc:
-        raise ValueError(f"lhs_indices {lshape} and rhs_indices "
-                         f"{tuple(rhs.shape)} do not broadcast") from exc
-    P = math.prod(shape)
+    shape, P, lhs_f, rhs_f = _gather_pairs(dev, bx, bw, lhs_indices, rhs_indices)
     out = torch.empty((*shape, M, N), dtype=out_dtype, device=dev) if alloc else None
     if P == 0 or M == 0 or N == 0:
         return out, None
-    lhs_f = (_default_lhs(dev, bx, tuple(shape)) if lhs is None
-             else lhs.expand(shape).reshape(-1).to(torch.int32).contiguous())
-    rhs_f = rhs.expand(shape).reshape(-1).to(torch.int32).contiguous()
     flat = []
     for w, s, b in banks:
         flat += [_aligned(w.reshape(E, *w.shape[-2:])),
@@ -592,8 +652,9 @@ def _tables_launch(a, out, tables: GatherTables, group_size, bits) -> bool:
 
 
 def gather_swiglu(x: torch.Tensor, gate, up, rhs_indices: torch.Tensor,
-                  tables: GatherTables, transpose: bool = True, group_size: int = 64,
-                  bits: int = 4, mode: str = "affine") -> torch.Tensor:
+                  tables: Optional[GatherTables], transpose: bool = True,
+                  group_size: Optional[int] = None, bits: Optional[int] = None,
+                  mode: str = "affine") -> torch.Tensor:
     """A prefill MoE layer's gate and up projections and its activation:
     ``swiglu(gather_qmm(x, *gate, rhs_indices=rhs_indices, tables=tables),
     gather_qmm(x, *up, ...))``, bit for bit, in one launch over the layer's
@@ -603,7 +664,12 @@ def gather_swiglu(x: torch.Tensor, gate, up, rhs_indices: torch.Tensor,
     ``(w, scales, biases)`` banks of one shape; x reaches pair p through
     batch ``p / top_k`` (no lhs table), as the tables were built.  The
     reference runs the gate and up grouped GEMMs over its shared tables and
-    then the activation (fused.py:3294-3302)."""
+    then the activation (fused.py:3294-3302).  ``mode="mxfp4"`` runs the three
+    calls."""
+    group_size, bits = _format(group_size, bits, mode)
+    if mode == "mxfp4":
+        kw = dict(rhs_indices=rhs_indices, transpose=transpose, mode=mode)
+        return swiglu(gather_qmm(x, *gate, **kw), gather_qmm(x, *up, **kw))
     out, a = _gather_prep(x, [tuple(gate), tuple(up)], None, rhs_indices, transpose, group_size,
                           bits, mode)
     if a is None:
@@ -659,8 +725,8 @@ def _gather_rows(a, out, group_size, bits, sorted_indices) -> torch.Tensor:
     lhs1 = (lhs[:, None] * M + rows[None, :]).reshape(-1).contiguous()
     rhs1 = a["rhs"][:, None].expand(P, M).reshape(-1).contiguous()
     o = out.reshape(P * M, 1, N)
-    _gather_launch(a["x"].reshape(B * M, 1, K), a["flat"], lhs1, rhs1, o, P * M, B * M, 1, N, K,
-                   a["E"], group_size, bits, sorted_indices)
+    a.get("launch", _gather_launch)(a["x"].reshape(B * M, 1, K), a["flat"], lhs1, rhs1, o, P * M,
+                                    B * M, 1, N, K, a["E"], group_size, bits, sorted_indices)
     return out
 
 
@@ -677,8 +743,9 @@ def _gather_slices(a, out, group_size, bits, sorted_indices) -> torch.Tensor:
         r = torch.where(inside, rhs - e0, torch.full_like(rhs, -1))
         part = torch.empty_like(out) if res is not None else out
         flat = [t[e0:e1] for t in a["flat"]]
-        _gather_launch(a["x"], flat, a["lhs"], r, part.reshape(P, a["M"], a["N"]), P, a["B"],
-                       a["M"], a["N"], a["K"], e1 - e0, group_size, bits, sorted_indices)
+        a.get("launch", _gather_launch)(a["x"], flat, a["lhs"], r, part.reshape(P, a["M"], a["N"]),
+                                        P, a["B"], a["M"], a["N"], a["K"], e1 - e0, group_size,
+                                        bits, sorted_indices)
         if res is None:
             res = part
         else:
@@ -686,13 +753,12 @@ def _gather_slices(a, out, group_size, bits, sorted_indices) -> torch.Tensor:
     return res
 
 
-def _gather_composed(a, out, bank, group_size, bits) -> torch.Tensor:
+def _gather_composed(a, out, deq_of) -> torch.Tensor:
     """Formats and dtypes without a gather kernel: each distinct expert's
-    weights dequantized by this library (bit-exact) in the promoted dtype
+    weights dequantized by this library (bit-exact; ``deq_of(e)``) in the promoted dtype
     and applied to its pairs with one GPU GEMM; pairs with an out-of-range
     index get zero rows, as in the kernels.  (The expert list is read on the
     host, so this path synchronises the stream.)"""
-    w, s, b = bank
     P, B, M, N, K, E = a["P"], a["B"], a["M"], a["N"], a["K"], a["E"]
     dt = a["dtype"]
     res = out.reshape(P, M, N)
@@ -706,7 +772,7 @@ def _gather_composed(a, out, bank, group_size, bits) -> torch.Tensor:
         if e < 0:
             continue
         sel = (rhs_h == e).nonzero().reshape(-1).to(a["dev"])
-        deq = dequantize(w[e], s[e].to(dt), b[e].to(dt), group_size, bits)
+        deq = deq_of(e)
         xe = xs[lhs[sel]]                                     # (n_e, M, K)
         ye = (torch.nn.functional.linear(xe, deq) if a["transpose"]
               else torch.matmul(xe, deq))
@@ -716,7 +782,8 @@ def _gather_composed(a, out, bank, group_size, bits) -> torch.Tensor:
 
 def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
                biases: Optional[torch.Tensor] = None, lhs_indices=None, rhs_indices=None,
-               transpose: bool = True, group_size: int = 64, bits: int = 4,
+               transpose: bool = True, group_size: Optional[int] = None,
+               bits: Optional[int] = None,
                mode: str = "affine", sorted_indices: bool = False,
                tables: Optional["GatherTables"] = None) -> torch.Tensor:
     """``mx.gather_qmm``: per index pair, ``x[lhs] @ dequantize(w[rhs]).T``.
@@ -732,8 +799,13 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     ``tables`` (:func:`gather_tables` of the same routing) skips building the
     segment tables where the call runs the thin grouped kernel (a MoE
     layer's gathers over one routing share one build); the result is the
-    same bit for bit.
+    same bit for bit.  ``mode="mxfp4"`` (uint8 scales, no biases) groups its
+    pairs itself and takes no tables.
     """
+    group_size, bits = _format(group_size, bits, mode)
+    if mode == "mxfp4":
+        return _mx.gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose,
+                              sorted_indices)
     out, a = _gather_prep(x, [(w, scales, biases)], lhs_indices, rhs_indices, transpose,
                           group_size, bits, mode)
     if a is None:
@@ -742,7 +814,9 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
                                                                         group_size, bits):
         return out
     if a["route"] == "composed":
-        return _gather_composed(a, out, a["flat"][:3], group_size, bits)
+        bank, dt = a["flat"][:3], a["dtype"]
+        return _gather_composed(a, out, lambda e: dequantize(
+            bank[0][e], bank[1][e].to(dt), bank[2][e].to(dt), group_size, bits))
     if a["route"] == "rows":
         return _gather_rows(a, out, group_size, bits, sorted_indices)
     if a["route"] == "slices":
@@ -756,8 +830,8 @@ def gather_glu(x: torch.Tensor, gate_w: torch.Tensor, gate_scales: torch.Tensor,
                gate_biases: Optional[torch.Tensor], up_w: torch.Tensor,
                up_scales: torch.Tensor, up_biases: Optional[torch.Tensor],
                lhs_indices=None, rhs_indices=None, transpose: bool = True,
-               group_size: int = 64, bits: int = 4, mode: str = "affine",
-               sorted_indices: bool = False) -> torch.Tensor:
+               group_size: Optional[int] = None, bits: Optional[int] = None,
+               mode: str = "affine", sorted_indices: bool = False) -> torch.Tensor:
     """Fused MoE gate+up+SiLU: ``silu(g) * u`` with ``g``, ``u`` the
     :func:`gather_qmm` products of the gate and up banks (same indices and
     broadcasting), summed in float and rounded once -- the reference's
@@ -769,11 +843,15 @@ def gather_glu(x: torch.Tensor, gate_w: torch.Tensor, gate_scales: torch.Tensor,
     result is composed from two :func:`gather_qmm` calls and a float
     SiLU-multiply of their rounded outputs, as the reference keeps its stock
     path outside decode widths (fused.py:2476-2479)."""
-    out, a = _gather_prep(x, [(gate_w, gate_scales, gate_biases), (up_w, up_scales, up_biases)],
-                          lhs_indices, rhs_indices, transpose, group_size, bits, mode)
-    if a is None:
-        return out
-    if a["route"] != "kernel" or a["P"] * a["M"] >= _GLU_FUSED_MAX_ROWS:
+    group_size, bits = _format(group_size, bits, mode)
+    a = None
+    if mode != "mxfp4":
+        out, a = _gather_prep(x, [(gate_w, gate_scales, gate_biases),
+                                  (up_w, up_scales, up_biases)],
+                              lhs_indices, rhs_indices, transpose, group_size, bits, mode)
+        if a is None:
+            return out
+    if a is None or a["route"] != "kernel" or a["P"] * a["M"] >= _GLU_FUSED_MAX_ROWS:
         kw = dict(lhs_indices=lhs_indices, rhs_indices=rhs_indices, transpose=transpose,
                   group_size=group_size, bits=bits, mode=mode, sorted_indices=sorted_indices)
         g = gather_qmm(x, gate_w, gate_scales, gate_biases, **kw)
@@ -802,8 +880,9 @@ _EUNSUPPORTED = -2
 
 def gather_qmm_combine(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
                        biases: Optional[torch.Tensor], rhs_indices: torch.Tensor,
-                       weights: torch.Tensor, transpose: bool = True, group_size: int = 64,
-                       bits: int = 4, mode: str = "affine", sgate: Optional[torch.Tensor] = None,
+                       weights: torch.Tensor, transpose: bool = True,
+                       group_size: Optional[int] = None, bits: Optional[int] = None,
+                       mode: str = "affine", sgate: Optional[torch.Tensor] = None,
                        shared: Optional[torch.Tensor] = None) -> torch.Tensor:
     """MoE down projection and combine: ``x`` holds one row per (token,
     expert) pair (``(T, top_k, 1, K)`` or anything of ``T * top_k * K``
@@ -818,6 +897,7 @@ def gather_qmm_combine(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     down kernel and then the combine (kernels/moe_decode_fused.py:378-397,
     kernels/moe_combine.py:160-195); otherwise, and for configurations that
     kernel does not take, the two calls run (faster there)."""
+    group_size, bits = _format(group_size, bits, mode)
     dev = _require_gpu(x, w, scales, biases, rhs_indices, weights, sgate, shared)
     if rhs_indices.ndim < 1 or rhs_indices.shape[-1] < 1:
         raise ValueError("rhs_indices must be (..., top_k)")
@@ -838,7 +918,7 @@ def gather_qmm_combine(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
         return moe_combine(y.reshape(T * top_k, y.shape[-1]), None, weights, T, top_k, sgate,
                            shared)
 
-    if T == 0 or T * top_k > _FOLD_MAX_P:
+    if T == 0 or T * top_k > _FOLD_MAX_P or mode == "mxfp4":
         return composed()
     _, a = _gather_prep(xs, [(w, scales, biases)], None, idx, transpose, group_size, bits, mode,
                         alloc=False)
@@ -1067,7 +1147,8 @@ def _block_fused(x, logits, top_k, gate, up, down, sgw, shared, group_size, bits
 
 
 def moe_layer(x: torch.Tensor, rhs_indices: torch.Tensor, weights: torch.Tensor, gate, up,
-              down, group_size: int = 64, bits: int = 4, mode: str = "affine") -> torch.Tensor:
+              down, group_size: Optional[int] = None, bits: Optional[int] = None,
+              mode: str = "affine") -> torch.Tensor:
     """A decode MoE layer after its routing (the reference's fused decode
     route, kernels/moe_decode_fused.py:331-397 with the combine of
     kernels/moe_combine.py:160-195): ``gather_glu(x, gate, up, rhs_indices)``
@@ -1212,3 +1293,7 @@ __all__: Sequence[str] = ("quantize", "dequantize", "quantized_matmul", "quantiz
                           "PreparedWeights", "gather_qmm", "gather_glu", "moe_combine",
                           "gather_tables", "GatherTables", "swiglu", "moe_block",
                           "launch_count", "set_row_identity", "row_identity")
+
+
+# after the helpers that it uses
+from . import mx as _mx  # noqa: E402

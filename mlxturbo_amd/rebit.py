@@ -40,15 +40,17 @@ CLASS_PATTERNS: Dict[str, Tuple[str, ...]] = {
 }
 
 
-def requantize(layer, bits: int, group_size: int = 64) -> QuantizedLinear:
+def requantize(layer, bits: int, group_size: int = 64,
+               mode: str = "affine") -> QuantizedLinear:
     """A new :class:`QuantizedLinear` holding ``layer``'s weight at ``bits`` /
     ``group_size``: a quantized layer is dequantized first (double
     quantization, as rebit.py:96-120 does); a ``torch.nn.Linear`` or any
-    module with a float ``weight`` is quantized directly.  ``bias`` is kept."""
+    module with a float ``weight`` is quantized directly.  ``bias`` is kept.
+    ``mode="mxfp4"`` takes ``bits=4, group_size=32``."""
     if isinstance(layer, QuantizedLinear):
         # both steps in one pass over the codes where the kernel takes them
         # (5120 x 17408, 8 to 4 bits: 47.6 us against 96.0 for the two)
-        if (layer.mode == "affine" and layer.weight.is_cuda
+        if (layer.mode == mode == "affine" and layer.weight.is_cuda
                 and type(layer).dequantized_weight is QuantizedLinear.dequantized_weight):
             q = ops._requantize(layer.weight, layer.scales, layer.biases, layer.group_size,
                                 layer.bits, group_size, bits)
@@ -63,14 +65,15 @@ def requantize(layer, bits: int, group_size: int = 64) -> QuantizedLinear:
         raise ValueError(f"in_dims={w.shape[-1]} is not a multiple of group_size={group_size}")
     bias = getattr(layer, "bias", None)
     new = QuantizedLinear.from_linear(w, bias=None if bias is None else bias.detach(),
-                                      group_size=group_size, bits=bits)
+                                      group_size=group_size, bits=bits, mode=mode)
     del w
     return new
 
 
-def parse(spec: str) -> Dict[str, Tuple[int, int]]:
-    """``"gdn=4,hc=4:32"`` -> ``{"gdn": (4, 64), "hc": (4, 32)}``."""
-    out: Dict[str, Tuple[int, int]] = {}
+def parse(spec: str) -> Dict[str, tuple]:
+    """``"gdn=4,hc=4:32"`` -> ``{"gdn": (4, 64), "hc": (4, 32)}``; ``"attn=mxfp4"``
+    -> ``{"attn": (4, 32, "mxfp4")}``."""
+    out: Dict[str, tuple] = {}
     for part in spec.split(","):
         part = part.strip()
         if not part:
@@ -79,6 +82,11 @@ def parse(spec: str) -> Dict[str, Tuple[int, int]]:
         bits, _, gs = rhs.partition(":")
         if cls not in CLASSES:
             raise ValueError(f"unknown class {cls!r} (known: {CLASSES})")
+        if bits == "mxfp4":
+            if gs:
+                raise ValueError(f"{part!r}: mxfp4 has groups of 32 only")
+            out[cls] = (4, 32, "mxfp4")
+            continue
         out[cls] = (int(bits), int(gs) if gs else 64)
     return out
 
@@ -100,20 +108,23 @@ def _targets(model: torch.nn.Module, patterns: Iterable[str]):
 def apply(model: torch.nn.Module, spec: str, patterns: Optional[Dict[str, Iterable[str]]] = None,
           verbose: bool = False) -> Dict[str, int]:
     """Re-quantize every layer of each class in ``spec`` in place; layers
-    already at the requested width and group size are left alone.  Returns
+    already at the requested width, group size and mode are left alone.  Returns
     the number of layers replaced per class."""
     table = CLASS_PATTERNS if patterns is None else patterns
     counts: Dict[str, int] = {}
-    for cls, (bits, gs) in parse(spec).items():
+    for cls, (bits, gs, *rest) in parse(spec).items():
+        mode = rest[0] if rest else "affine"
         n = 0
         for parent, attr, lin in list(_targets(model, table.get(cls, ()))):
-            if isinstance(lin, QuantizedLinear) and lin.bits == bits and lin.group_size == gs:
+            if (isinstance(lin, QuantizedLinear) and lin.bits == bits and lin.group_size == gs
+                    and lin.mode == mode):
                 continue
-            setattr(parent, attr, requantize(lin, bits, gs))
+            setattr(parent, attr, requantize(lin, bits, gs, mode))
             n += 1
         counts[cls] = n
         if verbose:
-            print(f"  rebit {cls}: {n} layers to {bits}bit/gs{gs}", flush=True)
+            print(f"  rebit {cls}: {n} layers to {bits}bit/gs{gs}"
+                  + (f" {mode}" if rest else ""), flush=True)
     return counts
 
 
