@@ -50,7 +50,9 @@ EXPORTED = (
     "mq_moe_route",
     "mq_mxfp4_quantize",
     "mq_mxfp4_dequantize",
+    "mq_mxfp4_matmul_workspace_size",
     "mq_mxfp4_matmul",
+    "mq_mxfp4_qqmm_workspace_size",
     "mq_mxfp4_qqmm",
     "mq_mxfp4_gather_qmm_workspace_size",
     "mq_mxfp4_gather_qmm",
@@ -135,10 +137,12 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mq_mxfp4_quantize.argtypes = [_vp, _vp, _vp, _i64, _i64, _int, _vp]
     lib.mq_mxfp4_dequantize.restype = _int
     lib.mq_mxfp4_dequantize.argtypes = [_vp, _vp, _vp, _i64, _i64, _int, _vp]
-    lib.mq_mxfp4_matmul.restype = _int
-    lib.mq_mxfp4_matmul.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp]
-    lib.mq_mxfp4_qqmm.restype = _int
-    lib.mq_mxfp4_qqmm.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp]
+    for name in ("mq_mxfp4_matmul", "mq_mxfp4_qqmm"):
+        size, call = getattr(lib, name + "_workspace_size"), getattr(lib, name)
+        size.restype = _sz
+        size.argtypes = [_i64] * 3
+        call.restype = _int
+        call.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp, _sz, _vp]
     lib.mq_mxfp4_gather_qmm_workspace_size.restype = _sz
     lib.mq_mxfp4_gather_qmm_workspace_size.argtypes = [_i64, _i64]
     lib.mq_mxfp4_gather_qmm.restype = _int

@@ -60,6 +60,9 @@ UNITS = [("abi.hip", []), ("formats.hip", []), ("prep.hip", []), ("route.hip", [
     for dt in (0, 1) for bits in (4, 8)
 ] + [("mx_formats.hip", [])] + [
     ("mx_skinny.hip", [f"-DMQ_INST_DT={dt}"]) for dt in (0, 1)
+] + [
+    ("mx_wide.hip", [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_QQ={qq}", "-fno-slp-vectorize"])
+    for dt in (0, 1) for qq in (0, 1)
 ]
 
 _NOISE = ("packed-fp32-ops", "warning generated", "warnings generated")

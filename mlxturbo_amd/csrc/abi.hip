@@ -174,6 +174,33 @@ int check_mx_product(const void* x, const void* w, const void* scales, const voi
   return MQ_OK;
 }
 
+int mx_done(int rc, int nl, const char* what);
+
+template <bool QQ>
+int mx_product(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
+               int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes,
+               void* hip_stream, const char* what) {
+  int rc = check_mx_product(x, w, scales, out, M, N, K, dtype);
+  if (rc) return rc;
+  if (workspace && !aligned16(workspace)) return fail(MQ_EINVAL, "workspace must be 16-byte aligned");
+  if (M == 0 || N == 0) return MQ_OK;
+  hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+  const size_t room = workspace ? workspace_bytes : 0;
+  int nl = 0;
+  rc = mq::kStatusUnsupported;
+  if (mq::mx_wide_route(M, N, K))
+    rc = dtype == MQ_BFLOAT16
+             ? mq::MxWideLaunch<mq::kBF16, QQ>::run(x, w, scales, out, M, N, K, workspace, room,
+                                                    st, &nl)
+             : mq::MxWideLaunch<mq::kF16, QQ>::run(x, w, scales, out, M, N, K, workspace, room,
+                                                   st, &nl);
+  if (rc == mq::kStatusUnsupported)
+    rc = dtype == MQ_BFLOAT16
+             ? mq::MxSkinnyLaunch<mq::kBF16, QQ>::run(x, w, scales, out, M, N, K, st, &nl)
+             : mq::MxSkinnyLaunch<mq::kF16, QQ>::run(x, w, scales, out, M, N, K, st, &nl);
+  return mx_done(rc, nl, what);
+}
+
 // Counts nl launches, or turns a launcher's status or a launch error into one.
 int mx_done(int rc, int nl, const char* what) {
   if (rc) return fail(rc, "%s: %s", what, rc > 0 ? hipGetErrorString((hipError_t)rc)
@@ -792,30 +819,28 @@ int mq_mxfp4_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, in
                  1, "mxfp4 dequantize");
 }
 
+size_t mq_mxfp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return mq::mx_workspace_bytes(M, N, K, false, mq::device_cu_count());
+}
+
+size_t mq_mxfp4_qqmm_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return mq::mx_workspace_bytes(M, N, K, true, mq::device_cu_count());
+}
+
 int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
-                    int64_t N, int64_t K, int dtype, void* hip_stream) {
-  int rc = check_mx_product(x, w, scales, out, M, N, K, dtype);
-  if (rc) return rc;
-  if (M == 0 || N == 0) return MQ_OK;
-  hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
-  int nl = 0;
-  rc = dtype == MQ_BFLOAT16
-           ? mq::MxSkinnyLaunch<mq::kBF16, false>::run(x, w, scales, out, M, N, K, st, &nl)
-           : mq::MxSkinnyLaunch<mq::kF16, false>::run(x, w, scales, out, M, N, K, st, &nl);
-  return mx_done(rc, nl, "mxfp4 quantized_matmul");
+                    int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes,
+                    void* hip_stream) {
+  return mx_product<false>(x, w, scales, out, M, N, K, dtype, workspace, workspace_bytes,
+                           hip_stream, "mxfp4 quantized_matmul");
 }
 
 int mq_mxfp4_qqmm(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
-                  int64_t N, int64_t K, int dtype, void* hip_stream) {
-  int rc = check_mx_product(x, w, scales, out, M, N, K, dtype);
-  if (rc) return rc;
-  if (M == 0 || N == 0) return MQ_OK;
-  hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
-  int nl = 0;
-  rc = dtype == MQ_BFLOAT16
-           ? mq::MxSkinnyLaunch<mq::kBF16, true>::run(x, w, scales, out, M, N, K, st, &nl)
-           : mq::MxSkinnyLaunch<mq::kF16, true>::run(x, w, scales, out, M, N, K, st, &nl);
-  return mx_done(rc, nl, "mxfp4 qqmm");
+                  int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes,
+                  void* hip_stream) {
+  return mx_product<true>(x, w, scales, out, M, N, K, dtype, workspace, workspace_bytes,
+                          hip_stream, "mxfp4 qqmm");
 }
 
 size_t mq_mxfp4_gather_qmm_workspace_size(int64_t P, int64_t M) {

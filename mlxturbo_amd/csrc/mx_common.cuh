@@ -76,6 +76,13 @@ __device__ __forceinline__ uint32_t mx_max2(uint32_t a, uint32_t b) {
   return bitcast<uint32_t>(__builtin_elementwise_max(bitcast<u16x2>(a), bitcast<u16x2>(b)));
 }
 
+// Largest of the four lanes of a quad, in each of them.
+__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
+  // quad_perm [1,0,3,2], then [2,3,0,1]
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));
+}
+
 // Scales of an expert or tile as a byte range: [first, first + bytes) of an
 // array whose base is 16-byte aligned, as a descriptor from the 16-byte
 // boundary before it to the end of the 4-byte word that holds its last byte,

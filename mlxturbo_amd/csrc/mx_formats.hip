@@ -18,12 +18,6 @@ namespace {
 constexpr int kMxThreads = 256;
 constexpr int kMxUnits = 4;
 
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  // quad_perm [1,0,3,2], then [2,3,0,1]
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));
-  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));
-}
-
 // units: N * K / 8, a multiple of 4, so a group's four threads are all there
 // or none is.
 template <int DT>
@@ -56,7 +50,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(const void* __r
       for (int j = 0; j < 4; ++j) top = mx_max2(top, v[i][0][j] & 0x7fff7fffu);
       top = max(top & 0xffffu, top >> 16);
     }
-    const uint32_t e = mx_scale_byte<DT>(quad_max(top));
+    const uint32_t e = mx_scale_byte<DT>(mx_quad_max(top));
     const float s = mx_scale(e);
     uint32_t c;
     if constexpr (DT == kF32) {

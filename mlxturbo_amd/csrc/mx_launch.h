@@ -22,6 +22,83 @@ struct MxSkinnyLaunch {
                  int64_t N, int64_t K, hipStream_t st, int* nlaunch);
 };
 
+// The same on the MFMA tile (mx_wide.cuh); ws of ws_bytes holds
+// mx_wide_workspace_bytes of the plan, or of the plan without K splits.
+template <int DT, bool QQ>
+struct MxWideLaunch {
+  static int run(const void* x, const uint32_t* w, const uint8_t* s, void* out, int64_t M,
+                 int64_t N, int64_t K, void* ws, size_t ws_bytes, hipStream_t st, int* nlaunch);
+};
+
+// ---- the wide tile's plan ----------------------------------------------------
+
+constexpr int kMxStepBytes = 256;               // of an x row per step (mx_tile.cuh)
+
+// Bytes of x packed for the 4-bit tile: codes of whole steps, then scales.
+inline size_t mx_pack_bytes(int64_t M, int64_t K) {
+  return (size_t)(M * ((K + 511) / 512)) * (kMxStepBytes + 16);
+}
+
+// A tile's x rows and weight rows have to fit 31-bit buffer ranges, the grid
+// its limits.
+inline bool mx_wide_fits(int64_t M, int64_t N, int64_t K) {
+  return K < ((int64_t)1 << 21) && (M + 63) / 64 * ((N + 255) / 256) < INT32_MAX - 8 &&
+         M * ((K + 511) / 512) < ((int64_t)1 << 31) && M * N < ((int64_t)1 << 40);
+}
+
+// Tile height and K split of least modelled cost: rounds of a tile per CU (two
+// 64-row tiles of T side by side on a CU take as long as in turn) of c0 + t us
+// per step each; K splits sum into float planes that a second kernel adds.  t measured at
+// K=5120 N=17408 (M = 64 .. 2048, one tile per CU and many rounds):
+// T 64/128/192 rows 1.0, 1.6, 2.25 us per 128 codes; QQ 2.6, 3.3,
+// 3.6 per 512.
+struct MxWidePlan {
+  int bm = 192, splits = 1;
+  double cost_us = 0.0;
+};
+
+inline MxWidePlan mx_wide_plan(int64_t M, int64_t N, int64_t K, bool qq, int cus,
+                               int max_splits = 16) {
+  const int bms[3] = {192, 128, 64};
+  const double us[2][3] = {{2.25, 1.6, 1.0}, {3.6, 3.3, 2.6}};
+  const int64_t nk = qq ? (K + 511) / 512 : (K + 127) / 128, cols = (N + 255) / 256;
+  MxWidePlan best;
+  for (int sp = 1; sp <= max_splits; ++sp) {
+    const int64_t steps = (nk + sp - 1) / sp;
+    if (sp > 1 && steps < 4) break;
+    for (int i = 0; i < 3; ++i) {
+      const int64_t tiles = cols * ((M + bms[i] - 1) / bms[i]) * sp;
+      const double round = 4.0 + us[qq][i] * (double)steps;
+      double cost = (double)((tiles + cus - 1) / cus) * round;
+      if (sp > 1) cost += 3.0 + (8.0 * sp + 2.0) * (double)M * (double)N / 5.0e6;
+      if (best.cost_us == 0.0 || cost < best.cost_us) {
+        best.bm = bms[i];
+        best.splits = sp;
+        best.cost_us = cost;
+      }
+    }
+  }
+  return best;
+}
+
+inline size_t mx_wide_workspace_bytes(const MxWidePlan& p, int64_t M, int64_t N, int64_t K,
+                                      bool qq) {
+  const size_t pack = qq ? (mx_pack_bytes(M, K) + 255) & ~(size_t)255 : 0;
+  return pack + (p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)N * sizeof(float) : 0);
+}
+
+// Whether a product runs on the tile: from 65 rows on, where the skinny kernel's
+// workgroups would read the weights again for every 64 rows.
+inline bool mx_wide_route(int64_t M, int64_t N, int64_t K) {
+  return M > 64 && mx_wide_fits(M, N, K);
+}
+
+// Device workspace of mq_mxfp4_matmul / mq_mxfp4_qqmm.
+inline size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, bool qq, int cus) {
+  if (!mx_wide_route(M, N, K)) return 0;
+  return mx_wide_workspace_bytes(mx_wide_plan(M, N, K, qq, cus), M, N, K, qq);
+}
+
 // gather_qmm over P (x batch, expert) pairs on the skinny kernel; ws as
 // gather_workspace_bytes(P, M) says.
 template <int DT>

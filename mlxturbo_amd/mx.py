@@ -111,6 +111,15 @@ def _composed(x, w, scales, transpose: bool) -> torch.Tensor:
     return torch.nn.functional.linear(x, deq) if transpose else torch.matmul(x, deq)
 
 
+def _product(call, size, x, w, s, out, M: int, N: int, K: int) -> int:
+    """One product call with this stream's workspace; its status."""
+    nbytes = int(size(M, N, K)) if M > 64 else 0     # up to 64 rows use none
+    ws = ops._workspace(out.device, nbytes) if nbytes else None
+    return call(x.data_ptr(), w.data_ptr(), s.data_ptr(), out.data_ptr(), M, N, K,
+                ops._DTYPE_CODE[out.dtype], ops._ptr(ws), ws.numel() if ws is not None else 0,
+                ops._stream_ptr(out))
+
+
 def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
     _no_biases(biases)
     dev = ops._require_gpu(x, w, scales)
@@ -135,8 +144,8 @@ def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
     if K == 0:
         return out.zero_()
     x_, w_, s_ = ops._aligned(x), ops._aligned(w), ops._aligned(scales)
-    rc = _lib.lib().mq_mxfp4_matmul(x_.data_ptr(), w_.data_ptr(), s_.data_ptr(), out.data_ptr(),
-                                    M, N, K, ops._DTYPE_CODE[x.dtype], ops._stream_ptr(out))
+    lib = _lib.lib()
+    rc = _product(lib.mq_mxfp4_matmul, lib.mq_mxfp4_matmul_workspace_size, x_, w_, s_, out, M, N, K)
     if rc == ops._EUNSUPPORTED:
         return _composed(x, w, scales, True)
     _lib.check(rc, "quantized_matmul")
@@ -163,9 +172,9 @@ def qqmm(x, w, scales) -> torch.Tensor:
     rc = ops._EUNSUPPORTED
     if x.dtype != torch.float32:
         x_, w_, s_ = ops._aligned(x), ops._aligned(w), ops._aligned(scales)
-        rc = _lib.lib().mq_mxfp4_qqmm(x_.data_ptr(), w_.data_ptr(), s_.data_ptr(),
-                                      out.data_ptr(), M, N, K, ops._DTYPE_CODE[x.dtype],
-                                      ops._stream_ptr(out))
+        lib = _lib.lib()
+        rc = _product(lib.mq_mxfp4_qqmm, lib.mq_mxfp4_qqmm_workspace_size, x_, w_, s_, out, M, N,
+                      K)
     if rc == ops._EUNSUPPORTED:
         return _composed(dequantize(*quantize(x), dtype=x.dtype), w, scales, True)
     _lib.check(rc, "qqmm")

@@ -115,7 +115,8 @@ def test_format_shapes_and_strides():
 SHAPES = [(1, 1, 32), (1, 16, 128), (2, 17, 96), (5, 250, 160), (16, 33, 1056), (17, 64, 512),
           (31, 100, 544), (33, 48, 2080), (64, 30, 256), (65, 257, 320), (130, 515, 1152),
           (1, 12000, 352), (300, 260, 64), (3, 10300, 64), (48, 10250, 96), (7, 40, 17408),
-          (513, 640, 832)]
+          (513, 640, 832), (192, 256, 2048), (200, 300, 17440), (1000, 128, 5152), (70, 70, 32),
+          (2049, 33, 96), (129, 1030, 3584)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -57,7 +57,7 @@ def test_product_argument_validation(lib, entry, kw, code, needle):
                                      a["N"], a["K"], 2, a["dtype"], None, 0, None)
     else:
         f = lib.mq_mxfp4_matmul if entry == "matmul" else lib.mq_mxfp4_qqmm
-        rc = f(a["x"], a["w"], a["s"], a["out"], a["M"], a["N"], a["K"], a["dtype"], None)
+        rc = f(a["x"], a["w"], a["s"], a["out"], a["M"], a["N"], a["K"], a["dtype"], None, 0, None)
     assert rc == code and needle in lib.mq_last_error().decode()
 
 
