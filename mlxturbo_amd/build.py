@@ -63,6 +63,8 @@ UNITS = [("abi.hip", []), ("formats.hip", []), ("prep.hip", []), ("route.hip", [
 ] + [
     ("mx_wide.hip", [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_QQ={qq}", "-fno-slp-vectorize"])
     for dt in (0, 1) for qq in (0, 1)
+] + [
+    ("mx_grouped.hip", [f"-DMQ_INST_DT={dt}", "-fno-slp-vectorize"]) for dt in (0, 1)
 ]
 
 _NOISE = ("packed-fp32-ops", "warning generated", "warnings generated")

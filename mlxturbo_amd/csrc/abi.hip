@@ -873,11 +873,19 @@ int mq_mxfp4_gather_qmm(const void* x, const uint32_t* w, const uint8_t* scales,
                 mq::kGatherPrepMaxE);
   hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
   int nl = 0;
-  rc = dtype == MQ_BFLOAT16
-           ? mq::MxGatherLaunch<mq::kBF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P, B,
-                                                M, N, K, E, workspace, st, &nl)
-           : mq::MxGatherLaunch<mq::kF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P, B,
-                                               M, N, K, E, workspace, st, &nl);
+  rc = mq::kStatusUnsupported;
+  if (need)
+    rc = dtype == MQ_BFLOAT16
+             ? mq::MxGroupedLaunch<mq::kBF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P,
+                                                   B, M, N, K, E, workspace, st, &nl)
+             : mq::MxGroupedLaunch<mq::kF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P,
+                                                  B, M, N, K, E, workspace, st, &nl);
+  if (rc == mq::kStatusUnsupported)
+    rc = dtype == MQ_BFLOAT16
+             ? mq::MxGatherLaunch<mq::kBF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P,
+                                                  B, M, N, K, E, workspace, st, &nl)
+             : mq::MxGatherLaunch<mq::kF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P, B,
+                                                 M, N, K, E, workspace, st, &nl);
   return mx_done(rc, nl, "mxfp4 gather_qmm");
 }
 

@@ -108,4 +108,13 @@ struct MxGatherLaunch {
                  int64_t K, int64_t E, void* ws, hipStream_t st, int* nlaunch);
 };
 
+// The same on the MFMA tile (mx_grouped.cuh), for calls that use a workspace;
+// kStatusUnsupported beyond its address ranges.
+template <int DT>
+struct MxGroupedLaunch {
+  static int run(const void* x, const uint32_t* w, const uint8_t* s, const int32_t* lhs,
+                 const int32_t* rhs, void* out, int64_t P, int64_t B, int64_t M, int64_t N,
+                 int64_t K, int64_t E, void* ws, hipStream_t st, int* nlaunch);
+};
+
 }  // namespace mq
