@@ -458,11 +458,11 @@ int mq_mxfp4_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, in
 /*
  * out[M, N] = x[M, K] . deq(w)^T, summed in float and rounded once, dtype
  * bfloat16 or float16 (deq in that type).  A row's result does not depend on M
- * up to 64 rows.  workspace (16-byte aligned, may be NULL) of
+ * up to 16 rows, or 32 under mq_set_row_identity.  workspace (16-byte aligned, may be NULL) of
  * mq_mxfp4_matmul_workspace_size(M, N, K) bytes lets wide products split K over
  * workgroups; calls sharing one must be ordered.  MQ_EUNSUPPORTED: float32, or
  * sizes beyond the kernels' address ranges (K of 2^21 and more, or of some 10^5
- * at up to 64 rows); the caller dequantizes there.
+ * at up to 16 rows); the caller dequantizes there.
  */
 size_t mq_mxfp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K);
 int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,
@@ -473,7 +473,7 @@ int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, voi
  * mq_mxfp4_matmul with x quantized too: out = deq(q(x)) . deq(w)^T with q as
  * mq_mxfp4_quantize, both operands entering the MFMAs as codes and scales
  * (mx.qqmm, mode="mxfp4").  Without the workspace (x's codes, and K splits) the
- * call runs at any size, slower above 64 rows.
+ * call runs at any size, slower above 16 rows.
  */
 size_t mq_mxfp4_qqmm_workspace_size(int64_t M, int64_t N, int64_t K);
 int mq_mxfp4_qqmm(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,

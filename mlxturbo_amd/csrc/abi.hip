@@ -188,7 +188,7 @@ int mx_product(const void* x, const uint32_t* w, const uint8_t* scales, void* ou
   const size_t room = workspace ? workspace_bytes : 0;
   int nl = 0;
   rc = mq::kStatusUnsupported;
-  if (mq::mx_wide_route(M, N, K))
+  if (mq::mx_wide_route(M, N, K, g_row_identity.load(std::memory_order_relaxed) != 0))
     rc = dtype == MQ_BFLOAT16
              ? mq::MxWideLaunch<mq::kBF16, QQ>::run(x, w, scales, out, M, N, K, workspace, room,
                                                     st, &nl)
@@ -821,12 +821,14 @@ int mq_mxfp4_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, in
 
 size_t mq_mxfp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return mq::mx_workspace_bytes(M, N, K, false, mq::device_cu_count());
+  return mq::mx_workspace_bytes(M, N, K, false, mq::device_cu_count(),
+                                g_row_identity.load(std::memory_order_relaxed) != 0);
 }
 
 size_t mq_mxfp4_qqmm_workspace_size(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return mq::mx_workspace_bytes(M, N, K, true, mq::device_cu_count());
+  return mq::mx_workspace_bytes(M, N, K, true, mq::device_cu_count(),
+                                g_row_identity.load(std::memory_order_relaxed) != 0);
 }
 
 int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, void* out, int64_t M,

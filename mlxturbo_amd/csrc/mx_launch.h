@@ -14,8 +14,8 @@ int launch_mx_quantize(const void* w, uint32_t* wq, uint8_t* scales, int64_t N, 
 int launch_mx_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, int64_t N,
                          int64_t K, int dtype, hipStream_t st);
 
-// out [M, N] = x [M, K] . deq(w)^T on the skinny kernel (mx_skinny.cuh); QQ: x
-// brought into MXFP4 first.  Any M; *nlaunch counts the kernels enqueued.
+// out [M, N] = x [M, K] . deq(w)^T on the skinny kernel (mx_skinny.cuh), 16 rows
+// at a time; QQ: x brought into MXFP4 first.  Any M; *nlaunch counts the kernels enqueued.
 template <int DT, bool QQ>
 struct MxSkinnyLaunch {
   static int run(const void* x, const uint32_t* w, const uint8_t* s, void* out, int64_t M,
@@ -87,15 +87,16 @@ inline size_t mx_wide_workspace_bytes(const MxWidePlan& p, int64_t M, int64_t N,
   return pack + (p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)N * sizeof(float) : 0);
 }
 
-// Whether a product runs on the tile: from 65 rows on, where the skinny kernel's
-// workgroups would read the weights again for every 64 rows.
-inline bool mx_wide_route(int64_t M, int64_t N, int64_t K) {
-  return M > 64 && mx_wide_fits(M, N, K);
+// Whether a product runs on the tile: above 16 rows, where the skinny kernel
+// would read the weights again for every 16; with row identity above 32.
+inline bool mx_wide_route(int64_t M, int64_t N, int64_t K, bool row_identity) {
+  return M > (row_identity ? 32 : 16) && mx_wide_fits(M, N, K);
 }
 
 // Device workspace of mq_mxfp4_matmul / mq_mxfp4_qqmm.
-inline size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, bool qq, int cus) {
-  if (!mx_wide_route(M, N, K)) return 0;
+inline size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, bool qq, int cus,
+                                 bool row_identity) {
+  if (!mx_wide_route(M, N, K, row_identity)) return 0;
   return mx_wide_workspace_bytes(mx_wide_plan(M, N, K, qq, cus), M, N, K, qq);
 }
 

@@ -113,7 +113,7 @@ def _composed(x, w, scales, transpose: bool) -> torch.Tensor:
 
 def _product(call, size, x, w, s, out, M: int, N: int, K: int) -> int:
     """One product call with this stream's workspace; its status."""
-    nbytes = int(size(M, N, K)) if M > 64 else 0     # up to 64 rows use none
+    nbytes = int(size(M, N, K)) if M > 16 else 0     # up to 16 rows use none
     ws = ops._workspace(out.device, nbytes) if nbytes else None
     return call(x.data_ptr(), w.data_ptr(), s.data_ptr(), out.data_ptr(), M, N, K,
                 ops._DTYPE_CODE[out.dtype], ops._ptr(ws), ws.numel() if ws is not None else 0,
