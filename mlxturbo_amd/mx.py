@@ -181,18 +181,18 @@ def qqmm(x, w, scales) -> torch.Tensor:
     return out
 
 
-def _gather_launch(x3, flat, lhs, rhs, out, P, B, M, N, K, E, group_size, bits,
+def _gather_launch(x, flat, lhs, rhs, out, P, B, M, N, K, E, group_size, bits,
                    sorted_indices) -> None:
     """One mq_mxfp4_gather_qmm call on flattened, validated arguments (the
     signature of ops' launch of affine banks)."""
-    x_ = ops._aligned(x3)
+    x_ = ops._aligned(x)
     w_, s_ = (ops._aligned(t) for t in flat)
     lib = _lib.lib()
     nbytes = int(lib.mq_mxfp4_gather_qmm_workspace_size(P, M))
     ws = ops._workspace(out.device, nbytes) if nbytes else None
     rc = lib.mq_mxfp4_gather_qmm(x_.data_ptr(), w_.data_ptr(), s_.data_ptr(), ops._ptr(lhs),
                                  rhs.data_ptr(), out.data_ptr(), P, B, M, N, K, E,
-                                 ops._DTYPE_CODE[x3.dtype], ops._ptr(ws),
+                                 ops._DTYPE_CODE[x.dtype], ops._ptr(ws),
                                  ws.numel() if ws is not None else 0, ops._stream_ptr(out))
     _lib.check(rc, "gather_qmm")
 
@@ -218,16 +218,20 @@ def gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose: bool,
         return out
     if K == 0 or B == 0 or E == 0:
         return out.zero_()
-    bank = [w.reshape(E, *w.shape[-2:]), scales.reshape(E, *scales.shape[-2:])]
+    if w.ndim != 3:
+        w, scales = w.reshape(E, *w.shape[-2:]), scales.reshape(E, *scales.shape[-2:])
+    bank = [w, scales]
+    composed = not transpose or x.dtype == torch.float32
+    if not composed and M <= 16 and (
+            E <= ops._GATHER_PREP_MAX_E
+            or not _lib.lib().mq_mxfp4_gather_qmm_workspace_size(P, M)):
+        _gather_launch(x, bank, lhs, rhs, out, P, B, M, N, K, E, GROUP_SIZE, BITS, sorted_indices)
+        return out
     a = dict(x=x.reshape(B, M, K), flat=bank, lhs=lhs, rhs=rhs, P=P, B=B, M=M, N=N, K=K, E=E,
              dev=dev, transpose=transpose, shape=shape, dtype=x.dtype, launch=_gather_launch)
-    if not transpose or x.dtype == torch.float32:
+    if composed:
         return ops._gather_composed(
-            a, out, lambda e: dequantize(bank[0][e], bank[1][e], dtype=x.dtype))
+            a, out, lambda e: dequantize(w[e], scales[e], dtype=x.dtype))
     if M > 16:
         return ops._gather_rows(a, out, GROUP_SIZE, BITS, sorted_indices)
-    if E > ops._GATHER_PREP_MAX_E and _lib.lib().mq_mxfp4_gather_qmm_workspace_size(P, M):
-        return ops._gather_slices(a, out, GROUP_SIZE, BITS, sorted_indices)
-    _gather_launch(a["x"], bank, lhs, rhs, out, P, B, M, N, K, E, GROUP_SIZE, BITS,
-                   sorted_indices)
-    return out
+    return ops._gather_slices(a, out, GROUP_SIZE, BITS, sorted_indices)

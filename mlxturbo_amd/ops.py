@@ -504,6 +504,17 @@ def _gather_pairs(dev, bx: tuple, bw: tuple, lhs_indices, rhs_indices):
     the indices over x's batch dims ``bx`` and w's ``bw``, its size, and both
     flattened over it as int32 (lhs None where the kernels' own rule gives it;
     both None when there is no pair)."""
+    if (lhs_indices is None and isinstance(rhs_indices, torch.Tensor)
+            and rhs_indices.dtype == torch.int32 and rhs_indices.is_cuda
+            and rhs_indices.get_device() == _dev_index(dev) and rhs_indices.is_contiguous()):
+        # the layers' call, tokens (T, 1) against experts (T, top_k): nothing to
+        # broadcast (torch.broadcast_shapes alone takes as long as a launch)
+        shape = tuple(rhs_indices.shape)
+        full = (1,) * (len(shape) - len(bx)) + bx
+        if (len(full) == len(shape) and _repeat_broadcast(bx, shape)
+                and all(b == s or b == 1 for b, s in zip(full, shape))):
+            P = math.prod(shape)
+            return shape, P, None, rhs_indices.reshape(-1) if P else None
     lhs = None if lhs_indices is None else _as_index(lhs_indices, dev)
     rhs = (torch.arange(math.prod(bw), device=dev, dtype=torch.int32).reshape(bw)
            if rhs_indices is None else _as_index(rhs_indices, dev))
