@@ -46,12 +46,15 @@ inline bool mx_wide_fits(int64_t M, int64_t N, int64_t K) {
          M * ((K + 511) / 512) < ((int64_t)1 << 31) && M * N < ((int64_t)1 << 40);
 }
 
-// Tile height and K split of least modelled cost: rounds of a tile per CU (two
-// 64-row tiles of T side by side on a CU take as long as in turn) of c0 + t us
-// per step each; K splits sum into float planes that a second kernel adds.  t measured at
-// K=5120 N=17408 (M = 64 .. 2048, one tile per CU and many rounds):
-// T 64/128/192 rows 1.0, 1.6, 2.25 us per 128 codes; QQ 2.6, 3.3,
-// 3.6 per 512.
+// Tile height and K split of least modelled cost, fitted to K=5120 N=17408 and
+// K=17408 N=5120 at 24 to 4096 rows, splits 1 to 12:
+//  * a round of a tile per CU takes 5 us and t per step (two 64-row tiles of T
+//    side by side on a CU take as long as in turn); over many rounds power and
+//    the L2 hold every CU to tp per step;
+//  * K splits sum into float planes that a second kernel adds, 3 us and (8 S + 2)
+//    M N bytes at 4.5 TB/s.
+// t, tp of 64 / 128 / 192 rows: T 0.77 / 1.25 / 1.55 and 1.1 / 1.9 / 2.1 us per
+// 128 codes; QQ 2.3 / 2.55 / 2.67 and 3.2 / 4.2 / 4.2 per 512.
 struct MxWidePlan {
   int bm = 192, splits = 1;
   double cost_us = 0.0;
@@ -60,17 +63,21 @@ struct MxWidePlan {
 inline MxWidePlan mx_wide_plan(int64_t M, int64_t N, int64_t K, bool qq, int cus,
                                int max_splits = 16) {
   const int bms[3] = {192, 128, 64};
-  const double us[2][3] = {{2.25, 1.6, 1.0}, {3.6, 3.3, 2.6}};
+  const double us[2][3] = {{1.55, 1.25, 0.77}, {2.67, 2.55, 2.3}};
+  const double held[2][3] = {{2.1, 1.9, 1.1}, {4.2, 4.2, 3.2}};
   const int64_t nk = qq ? (K + 511) / 512 : (K + 127) / 128, cols = (N + 255) / 256;
+  const int64_t unit = qq || K % 512 ? 1 : 4;   // steps that a split takes or leaves
   MxWidePlan best;
   for (int sp = 1; sp <= max_splits; ++sp) {
-    const int64_t steps = (nk + sp - 1) / sp;
-    if (sp > 1 && steps < 4) break;
+    const int64_t steps = (nk / unit + sp - 1) / sp * unit;
+    if (sp > 1 && (steps < 4 || sp > nk / unit)) break;
     for (int i = 0; i < 3; ++i) {
       const int64_t tiles = cols * ((M + bms[i] - 1) / bms[i]) * sp;
-      const double round = 4.0 + us[qq][i] * (double)steps;
+      const double round = 5.0 + us[qq][i] * (double)steps;
       double cost = (double)((tiles + cus - 1) / cus) * round;
-      if (sp > 1) cost += 3.0 + (8.0 * sp + 2.0) * (double)M * (double)N / 5.0e6;
+      const double many = 5.0 + (double)tiles / cus * held[qq][i] * (double)steps;
+      if (many > cost) cost = many;
+      if (sp > 1) cost += 3.0 + (8.0 * sp + 2.0) * (double)M * (double)N / 4.5e6;
       if (best.cost_us == 0.0 || cost < best.cost_us) {
         best.bm = bms[i];
         best.splits = sp;

@@ -32,7 +32,7 @@
 
 namespace mq {
 
-// x rows of codes as the 4-bit products take them (mx_pack.cuh's layout): row m
+// x rows of codes as the 4-bit products take them (mx_wide.cuh's layout): row m
 // at m * steps * 256 bytes, padded with zero codes to whole steps of 512; the
 // scales of row m and step s are 16 bytes at (m * steps + s) * 16, byte 4 c + q
 // that of group 16 s + 4 q + c.
@@ -44,8 +44,9 @@ template <int BM> struct MxTileShape {
 };
 
 // xoff(r): byte offset of tile row r in xr, or 0x80000000 (zeros); QQ: xs holds
-// the rows' scale bytes, row r at soff(r).  TAIL: K is not whole steps (T: of
-// 128; QQ: of 512), or, QQ, the scale bytes are not 16-byte aligned.
+// the rows' scale bytes, row r at soff(r).  TAIL: K is not whole 512s (rows of
+// scale bytes are not 16-byte aligned, and steps may end in the middle).
+// T without TAIL: kt0 and nk in whole rounds of kStages steps.
 // put(i, j, v): v[e] = the sum of tile row 16 i + r and the wave's weight row 16
 // j + 4 c + e.
 template <int DT, bool QQ, int BM, bool TAIL, class XOff, class SOff, class Put>
@@ -58,16 +59,19 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
                                         unsigned char* __restrict__ A2,
                                         unsigned char* __restrict__ A3) {
   constexpr int ST = MxTileShape<BM>::kStages, MB = BM / 16, SLOTS = 4 * MB, DM = BM / 16;
-  constexpr int P = MB <= 6 ? MB - 1 : 6;       // slots a fragment is read ahead
-  constexpr int R = 8;                          // fragment registers
+  // slots a fragment is read ahead, and fragment registers
+  constexpr int P = MB == 1 ? 2 : MB <= 4 ? 3 : 6, R = MB == 1 ? 4 : 8;
+  static_assert(!QQ || MB >= P + 1, "scale bytes are read with the first substep's fragments");
   static_assert(SLOTS % R == 0 && P < R, "a step's slots run through whole rings");
   constexpr int WQ = QQ ? 4 : 1;                // 16-byte weight loads per block and step
-  constexpr int SQ = !QQ ? 1 : TAIL ? 4 : 1;    // scale loads per block and step
+  constexpr int SQ = TAIL ? (QQ ? 4 : 1) : (QQ ? 1 : 0);   // scale loads per block and step
   constexpr int XS = QQ ? 1 : 0;                // scale loads of x per wave and step
   constexpr int NL = DM + XS + 4 * WQ + 4 * SQ;
-  // Steps of weights in registers; QQ leaves no room for a second one beside
-  // the sums of tall tiles.
-  constexpr int WR = QQ && BM >= 192 ? 1 : 2, SR = 2;
+  // Steps of weights and of their scale bytes in registers, as many as the sums
+  // leave room for (T, 64 rows: with two, a step waited for the weights of the
+  // step before it).
+  constexpr int WR = QQ ? (BM >= 192 ? 1 : 2) : BM >= 192 ? 2 : 4, SR = QQ ? 2 : WR;
+  constexpr bool PAIR = WR == 4;
   using T = T16<DT>;
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -79,7 +83,7 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
   for (int j = 0; j < 4; ++j) {
     const int row = 64 * wave + 16 * j + r;
     wo[j] = (uint32_t)(row * G + c) * 16u;
-    so[j] = row < ncols ? skew + (uint32_t)(row * G + (QQ && !TAIL ? 0 : c)) : 0x80000000u;
+    so[j] = row < ncols ? skew + (uint32_t)(row * G + (TAIL ? c : 0)) : 0x80000000u;
   }
   // fragment addresses per stage and substep; the opaque zero keeps a stage's
   // base in the address register, since an offset field reaches 64 KB only
@@ -96,6 +100,25 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
 
   u32x4 W[WR][4][WQ];
   u32x4 S[SR][4];                               // scale bytes: [0], or by substep
+  // T, whole rounds: a round's scale bytes (four per step) in one load per block.
+  // Byte loads for every step brought each row's line to the L1 again, as much
+  // as the weights (N=5120 K=17408, 45 rows, 12 splits: 40 against 32 us).
+  uint32_t cur[4][ST], nxt[4][ST];
+  auto sround = [&](int s, uint32_t (&d)[4][ST]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t o = s < nk ? (uint32_t)(kt0 + s) * 4u : 0x80000000u;
+      if constexpr (ST == 4) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, so[j], o, 0);
+#pragma unroll
+        for (int i = 0; i < ST; ++i) d[j][i] = v[i];
+      } else {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rs, so[j], o, 0);
+#pragma unroll
+        for (int i = 0; i < ST; ++i) d[j][i] = v[i];
+      }
+    }
+  };
   // byte offset of step s in rows of b bytes a step; past the last step, past
   // every range (zeros, no traffic)
   auto at = [&](int s, uint32_t b) { return s < nk ? (uint32_t)(kt0 + s) * b : 0x80000000u; };
@@ -110,7 +133,7 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
       if constexpr (TAIL && !QQ) o = 4 * k + c < G ? o : 0x80000000u;
       W[SW][j][q] = __builtin_amdgcn_raw_buffer_load_b128(rw, o + 64u * q, at(s, 64u * WQ), 0);
     } else if constexpr (v < 4 * WQ + 4 * SQ) {
-      constexpr int j = (v - 4 * WQ) / SQ, q = (v - 4 * WQ) % SQ;
+      constexpr int n = SQ ? SQ : 1, j = (v - 4 * WQ) / n, q = (v - 4 * WQ) % n;
       if constexpr (QQ && !TAIL) {
         S[SS][j] = __builtin_amdgcn_raw_buffer_load_b128(rs, so[j], at(s, 16u), 0);
       } else {
@@ -122,7 +145,7 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
       constexpr int i = v - 4 * WQ - 4 * SQ;
       uint32_t o = dmo[i];
       if constexpr (TAIL && !QQ) {
-        const int p = (lane & 15) ^ (4 * (i & 3) + (lane >> 4));
+        const int p = (lane & 15) ^ (4 * ((wave * DM + i) & 3) + (lane >> 4));
         o = 4 * k + (p >> 2) < G ? o : 0x80000000u;
       }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -146,7 +169,7 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
       // zeros of their own: from one shared zero the compiler made the first
       // MFMA of every sum in the loop read a copy (192 moves and their waits
       // per 384 MFMAs; M=2048 316 against 272 us)
-      asm volatile("" : "+a"(acc[i][j]));
+      if constexpr (BM > 64 || QQ) asm volatile("" : "+a"(acc[i][j]));
     }
   u32x4 A[R];
   u32x4 B[2][4];                                // T operands of a substep
@@ -167,7 +190,10 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
     if constexpr (QQ) {
       if constexpr (e == 0) we[q & 1][j] = TAIL ? S[SS][j][q] : S[SS][j][q] >> (8 * c);
     } else {
-      if constexpr (q == 0 && e == 0) sf[j] = mx_scale(S[SS][j][0]);
+      if constexpr (q == 0 && e == 0) {
+        constexpr int i = decltype(swc)::value % ST;
+        sf[j] = mx_scale(TAIL ? S[SS][j][0] : (cur[j][i] >> (8 * c)) & 255u);
+      }
       B[q & 1][j][e] = mx_pair<DT, e>(W[SW][j][0][q], sf[j]);
     }
   };
@@ -185,10 +211,15 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
   using I3 = std::integral_constant<int, 3>;
 
   // prologue: the weights first (x rows may have to be looked up)
+  if constexpr (!QQ && !TAIL) sround(0, cur);
   constexpr int NW = 4 * WQ + 4 * SQ;
   constexpr int NWB = 4 * WQ;
   static_for<0, NW>([&](auto vc) { load(0, I0{}, vc); });
   static_for<WR == 1 ? NWB : 0, NW>([&](auto vc) { load(1, I1{}, vc); });
+  if constexpr (WR == 4) {
+    static_for<0, NW>([&](auto vc) { load(2, I2{}, vc); });
+    static_for<0, NW>([&](auto vc) { load(3, I3{}, vc); });
+  }
 #pragma unroll
   for (int i = 0; i < DM; ++i) {
     const int row = 4 * (wave * DM + i) + (lane >> 4);
@@ -206,13 +237,16 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
 
   // A step issues, in this order: in its first substep the x of step s + ST - 1;
   // QQ: after each substep its weights of step s + WR; in the last substep,
-  // before the barrier, the scale bytes (T: and the weights) of step s + 2.
+  // before the barrier, the scale bytes (T: and the weights) of step s + SR, or,
+  // PAIR, in every second step's those of the next two steps' successors.
   // Flight: those issued after the x of step s + 1, which the wait before the
   // barrier may leave in flight.
   constexpr int FREE = SLOTS - P;
   constexpr int kLate = (QQ ? 8 + (MB - P < 4 ? MB - P : 4) : 0) + NW - (QQ ? NWB : 0);
   constexpr int kAll = QQ ? 16 + NW - NWB : NW;
-  constexpr int kFlight = ST == 2 ? kLate : 2 * (DM + XS) + 2 * kAll + kLate;
+  // (pairs: 2 NW in every second step, so as many in any two steps)
+  constexpr int kFlight =
+      ST == 2 ? kLate : 2 * (DM + XS) + (PAIR ? 2 * NW : 2 * kAll + kLate);
   using Flight = std::integral_constant<int, (kFlight < 63 ? kFlight : 63)>;
   // one step; u: its stage
   auto step = [&](int s, auto uc) {
@@ -240,6 +274,15 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
           acc[i][j] = T::mfma(B[q & 1][j], A[t % R], acc[i][j]);
         }
       }
+      if constexpr (!QQ && !TAIL) {
+        if constexpr (u == 0 && q == 1 && i == 0) sround(s + ST, nxt);
+        if constexpr (u == ST - 1 && q == 3 && i == 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < ST; ++k) cur[j][k] = nxt[j][k];
+        }
+      }
       // the next substep's operands
       static_for<i * 16 / MB, (i + 1) * 16 / MB>([&](auto xc) {
         if constexpr (q < 3) piece(U{}, std::integral_constant<int, q + 1>{}, xc);
@@ -252,10 +295,17 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
       if constexpr (QQ && q > 0 && i < 4)
         load(s + WR, std::integral_constant<int, u + WR>{},
              std::integral_constant<int, i * WQ + q - 1>{});
-      if constexpr (q == 3 && t < FREE) {
+      if constexpr (PAIR) {
+        // both halves of a line together, in the second step of a pair
+        if constexpr (q == 3 && (u & 1))
+          static_for<i * NW / MB, (i + 1) * NW / MB>([&](auto vc) {
+            load(s + 3, std::integral_constant<int, u + 3>{}, vc);
+            load(s + 4, std::integral_constant<int, u + 4>{}, vc);
+          });
+      } else if constexpr (q == 3 && t < FREE) {
         constexpr int F = QQ ? NWB : 0, n = MB - P;
         static_for<i * (NW - F) / n, (i + 1) * (NW - F) / n>([&](auto vc) {
-          load(s + 2, std::integral_constant<int, u + 2>{},
+          load(s + SR, std::integral_constant<int, u + SR>{},
                std::integral_constant<int, F + decltype(vc)::value>{});
         });
       }

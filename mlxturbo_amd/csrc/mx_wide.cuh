@@ -31,9 +31,9 @@ __global__ __launch_bounds__(256) void mx_pack_kernel(const uint16_t* __restrict
     scales[(row * steps + (g >> 4)) * 16 + 4 * (g & 3) + ((g >> 2) & 3)] = (uint8_t)e;
 }
 
-// A tile per workgroup, placed so that an XCD runs a contiguous range of weight
-// columns over all rows (grouped_tile); blockIdx.y = z sums its share of the
-// steps, into the float plane part[z] where part is given.
+// A tile and a share z of the steps per workgroup, placed so that an XCD runs a
+// contiguous range of weight columns and shares over all rows (grouped_tile);
+// where part is given the sums go to its float plane part[z].
 template <int DT, bool QQ, int BM, bool TAIL>
 __global__ __launch_bounds__(256, BM <= 64 && !QQ ? 2 : 1) void mx_wide_kernel(
     const void* __restrict__ x, const uint8_t* __restrict__ xscales,
@@ -45,13 +45,16 @@ __global__ __launch_bounds__(256, BM <= 64 && !QQ ? 2 : 1) void mx_wide_kernel(
   __shared__ __align__(16) unsigned char A1[kBytes];
   __shared__ __align__(16) unsigned char A2[Sh::kStages > 2 ? kBytes : 16];
   __shared__ __align__(16) unsigned char A3[Sh::kStages > 2 ? kBytes : 16];
-  int col, mt;
-  if (!grouped_tile(blockIdx.x, (N + 255) / 256, (M + BM - 1) / BM, col, mt)) return;
+  int cz, mt;
+  if (!grouped_tile(blockIdx.x, (N + 255) / 256 * splits, (M + BM - 1) / BM, cz, mt)) return;
+  const int col = cz / splits, z = cz - col * splits;
   const int m0 = mt * BM, n0 = col * 256;
   const int mrows = min(BM, M - m0), ncols = min(256, N - n0);
-  const int steps = QQ ? (G + 15) / 16 : (G + 3) / 4, z = blockIdx.y;
-  const int kt0 = (int)((int64_t)steps * z / splits);
-  const int kt1 = (int)((int64_t)steps * (z + 1) / splits);
+  const int steps = QQ ? (G + 15) / 16 : (G + 3) / 4;
+  constexpr int kUnit = QQ || TAIL ? 1 : Sh::kStages;
+  const int nu = steps / kUnit;
+  const int kt0 = kUnit * (int)((int64_t)nu * z / splits);
+  const int kt1 = kUnit * (int)((int64_t)nu * (z + 1) / splits);
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t rowb = QQ ? (uint32_t)steps * 256u : (uint32_t)G * 64u;
@@ -95,14 +98,14 @@ template <int DT, bool QQ, int BM>
 inline int mx_wide_launch_bm(const void* x, const uint8_t* xs, const uint32_t* w,
                              const uint8_t* s, void* out, int64_t M, int64_t N, int64_t K,
                              int splits, float* part, hipStream_t st) {
-  const int64_t G = K / kMxGroup, tiles = (N + 255) / 256 * ((M + BM - 1) / BM);
+  const int64_t G = K / kMxGroup, tiles = (N + 255) / 256 * ((M + BM - 1) / BM) * splits;
   if ((tiles + 7) / 8 * 8 > INT32_MAX) return kStatusUnsupported;
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)splits);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
   auto go = [&](auto tail) {
     hipLaunchKernelGGL((mx_wide_kernel<DT, QQ, BM, decltype(tail)::value>), grid, dim3(256), 0,
                        st, x, xs, w, s, (uint16_t*)out, part, (int)M, (int)N, (int)G, splits);
   };
-  if (G % (QQ ? 16 : 4)) go(std::true_type{});
+  if (G % 16) go(std::true_type{});
   else go(std::false_type{});
   if (splits > 1) {
     const int64_t MN = M * N;
