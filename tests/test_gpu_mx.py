@@ -288,6 +288,25 @@ def test_gather_indices_rows_and_invalid_pairs(P, B, M):
     _check_gather(out, x, v, lhs, srt)
 
 
+@pytest.mark.parametrize("P", [257, 1027, 16383, 16385, 32766, 32769, 70001])
+@pytest.mark.parametrize("E", [3, 700])
+def test_gather_sorts_any_number_of_pairs(P, E):
+    g = _gen(P + E)
+    N, K, B = 20, 64, 37
+    w, s, v = weights(g, E, N, K)
+    x = _randn(g, B, 1, K, dtype=torch.float16)
+    # most pairs on one expert, many experts without any, some out of range
+    rhs = (torch.rand(P, generator=g, device="cuda") ** 4 * (E + 1)).int()
+    rhs[torch.randint(0, P, (P // 9,), generator=g, device="cuda")] = -3
+    lhs = torch.randint(0, B, (P,), generator=g, device="cuda").int()
+    lhs[P - 1], lhs[P // 2] = B, -1
+    out = mq.gather_qmm(x, w, s, lhs_indices=lhs, rhs_indices=rhs, **KW)
+    _check_gather(out, x, v, lhs, rhs)
+    rhs[P - 3:] = E - 1                                      # the last pairs, no lhs
+    out = mq.gather_qmm(x[:1], w, s, rhs_indices=rhs[1:], **KW)   # and 4-byte alignment
+    _check_gather(out, x[:1], v, torch.zeros_like(rhs[1:]), rhs[1:])
+
+
 def test_gather_many_experts_in_slices():
     g = _gen(8)
     E, N, K, P = 2050, 16, 32, 400
