@@ -35,14 +35,14 @@ __device__ __forceinline__ void mx_grouped_tile(const MxGroupedLds<LBM>& lds,
   const auto xr = wide_rsrc(x, (int64_t)B * Mi * G * 64);
   const int64_t row0 = (int64_t)e * N + n0;
   const bool vec = N % 4 == 0 && (uintptr_t)out % 8 == 0;
-  mx_tile<DT, false, BM, TAIL>(
+  mx_tile<DT, BM, TAIL>(
       xr,
       [&](int i) {
         if (i >= rows) return 0x80000000u;      // zeros, no memory access
         const int q = Mi == 1 ? i : i / Mi;
         return (uint32_t)(((int64_t)x_batch(lhs, lds.pair[q], P, B) * Mi + i - q * Mi) * G * 64);
       },
-      xr, [](int) { return 0u; }, w + row0 * G * 4, scales + row0 * G, ncols, G, 0, (G + 3) / 4,
+      w + row0 * G * 4, scales + row0 * G, ncols, G, 0, (G + 3) / 4,
       [&](int i, int j, const f32x4& v) {
         const int m = 16 * i + r, n = 64 * wave + 16 * j + 4 * c;
         if (m >= rows) return;

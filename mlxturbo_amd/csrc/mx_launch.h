@@ -32,7 +32,7 @@ struct MxWideLaunch {
 
 // ---- the wide tile's plan ----------------------------------------------------
 
-constexpr int kMxStepBytes = 256;               // of an x row per step (mx_tile.cuh)
+constexpr int kMxStepBytes = 256;               // of codes of an x row per 512 of K
 
 // Bytes of x packed for the 4-bit tile: codes of whole steps, then scales.
 inline size_t mx_pack_bytes(int64_t M, int64_t K) {
@@ -48,13 +48,13 @@ inline bool mx_wide_fits(int64_t M, int64_t N, int64_t K) {
 
 // Tile height and K split of least modelled cost, fitted to K=5120 N=17408 and
 // K=17408 N=5120 at 24 to 4096 rows, splits 1 to 12:
-//  * a round of a tile per CU takes 5 us and t per step (two 64-row tiles of T
-//    side by side on a CU take as long as in turn); over many rounds power and
-//    the L2 hold every CU to tp per step;
+//  * a round of a tile per CU takes c0 and t per step (two 64-row tiles of T side by
+//    side on a CU take as long as in turn); over many rounds power and the L2 hold
+//    every CU to tp per step;
 //  * K splits sum into float planes that a second kernel adds, 3 us and (8 S + 2)
-//    M N bytes at 4.5 TB/s.
-// t, tp of 64 / 128 / 192 rows: T 0.77 / 1.25 / 1.55 and 1.1 / 1.9 / 2.1 us per
-// 128 codes; QQ 2.3 / 2.55 / 2.67 and 3.2 / 4.2 / 4.2 per 512.
+//    M N bytes at 4.5 (QQ: 7) TB/s.
+// c0, t, tp of 64 / 128 / 192 rows: T 5 us, 0.77 / 1.25 / 1.55 and 1.1 / 1.9 / 2.1 us
+// per 128 codes; QQ 4.5, 1.45 / 1.9 / 2.2 and 1.9 / 2.15 / 3.3 per 512.
 struct MxWidePlan {
   int bm = 192, splits = 1;
   double cost_us = 0.0;
@@ -63,8 +63,9 @@ struct MxWidePlan {
 inline MxWidePlan mx_wide_plan(int64_t M, int64_t N, int64_t K, bool qq, int cus,
                                int max_splits = 16) {
   const int bms[3] = {192, 128, 64};
-  const double us[2][3] = {{1.55, 1.25, 0.77}, {2.67, 2.55, 2.3}};
-  const double held[2][3] = {{2.1, 1.9, 1.1}, {4.2, 4.2, 3.2}};
+  const double us[2][3] = {{1.55, 1.25, 0.77}, {2.2, 1.9, 1.45}};
+  const double held[2][3] = {{2.1, 1.9, 1.1}, {3.3, 2.15, 1.9}};
+  const double c0 = qq ? 4.5 : 5.0, bw = qq ? 7.0e6 : 4.5e6;
   const int64_t nk = qq ? (K + 511) / 512 : (K + 127) / 128, cols = (N + 255) / 256;
   const int64_t unit = qq || K % 512 ? 1 : 4;   // steps that a split takes or leaves
   MxWidePlan best;
@@ -73,11 +74,11 @@ inline MxWidePlan mx_wide_plan(int64_t M, int64_t N, int64_t K, bool qq, int cus
     if (sp > 1 && (steps < 4 || sp > nk / unit)) break;
     for (int i = 0; i < 3; ++i) {
       const int64_t tiles = cols * ((M + bms[i] - 1) / bms[i]) * sp;
-      const double round = 5.0 + us[qq][i] * (double)steps;
+      const double round = c0 + us[qq][i] * (double)steps;
       double cost = (double)((tiles + cus - 1) / cus) * round;
-      const double many = 5.0 + (double)tiles / cus * held[qq][i] * (double)steps;
+      const double many = c0 + (double)tiles / cus * held[qq][i] * (double)steps;
       if (many > cost) cost = many;
-      if (sp > 1) cost += 3.0 + (8.0 * sp + 2.0) * (double)M * (double)N / 4.5e6;
+      if (sp > 1) cost += 3.0 + (8.0 * sp + 2.0) * (double)M * (double)N / bw;
       if (best.cost_us == 0.0 || cost < best.cost_us) {
         best.bm = bms[i];
         best.splits = sp;

@@ -1,17 +1,16 @@
-// The MFMA tile of wide MXFP4 products: BM rows of x times 256 weight rows.
+// The MFMA tile of wide MXFP4 products with x of 16 bits: BM rows of x times 256
+// weight rows.
 //
 // 256 threads = 4 waves, one per SIMD (two workgroups per CU at BM = 64); a
-// wave owns all BM rows and 64 weight rows as four 16-row blocks.  Per step an
-// x row is 256 bytes: 128 values of T, or, QQ, 512 codes; a step is four
-// substeps q, and per substep and 16-row block of x ("slot") a wave runs four
-// MFMAs, one per weight block: 16x16x32 on T values, or 16x16x128 on codes with
-// their scale bytes.  Every MFMA takes 16 cycles, a slot 64, either way.
+// wave owns all BM rows and 64 weight rows as four 16-row blocks.  A step is 128
+// values of K (256 bytes of an x row), four substeps q; per substep and 16-row
+// block of x ("slot") a wave runs four 16x16x32 MFMAs, one per weight block, of 16
+// cycles each.
 //
-//  * Lane (r = lane & 15, c = lane >> 4) of an operand holds row r.  T: 16 bytes
-//    of weights are its group c of the step's four, word q the 8 codes of
-//    substep q, converted by four instructions of two codes into the MFMA's
-//    operand; the x chunk is 4 c + q.  QQ: 16 bytes of weights and of x are
-//    group 4 q + c, straight into the MFMA.
+//  * Lane (r = lane & 15, c = lane >> 4) of an operand holds row r: 16 bytes of
+//    weights are its group c of the step's four, word q the 8 codes of substep q,
+//    converted by four instructions of two codes into the MFMA's operand; the x
+//    chunk is 4 c + q.
 //  * x goes to LDS by the buffer loads' LDS form, ST - 1 steps ahead in ST
 //    stages (whole 256-byte row pieces; chunk p of row r stored at p ^ (r & 15),
 //    so the 16 rows of a fragment read lie in distinct banks); weights and their
@@ -24,34 +23,25 @@
 //  * What is not an MFMA (fragment reads, conversions, loads) is placed between
 //    them slot by slot (sched_barrier): a wave runs alone on its SIMD.
 //
-// Groups past K: zero codes and scale bytes 0 (outside the buffer ranges), x
-// zero (outside its range, or the quantizer's padding).
+// Groups past K: zero codes and scale bytes 0, x zero (outside the buffer ranges).
 #pragma once
 #include "mx_common.cuh"
 #include "mx_launch.h"
 
 namespace mq {
 
-// x rows of codes as the 4-bit products take them (mx_wide.cuh's layout): row m
-// at m * steps * 256 bytes, padded with zero codes to whole steps of 512; the
-// scales of row m and step s are 16 bytes at (m * steps + s) * 16, byte 4 c + q
-// that of group 16 s + 4 q + c.
-
 template <int BM> struct MxTileShape {
   static constexpr int kStages = BM >= 192 ? 2 : 4;
-  static constexpr int kStage = BM * kMxStepBytes;       // bytes of x
-  static constexpr int kScales = 4096;                   // QQ: its scales, after them
+  static constexpr int kStage = BM * 256;                // bytes of x
 };
 
-// xoff(r): byte offset of tile row r in xr, or 0x80000000 (zeros); QQ: xs holds
-// the rows' scale bytes, row r at soff(r).  TAIL: K is not whole 512s (rows of
-// scale bytes are not 16-byte aligned, and steps may end in the middle).
-// T without TAIL: kt0 and nk in whole rounds of kStages steps.
+// xoff(r): byte offset of tile row r in xr, or 0x80000000 (zeros).  TAIL: K is not
+// whole 512s (rows of scale bytes are not 16-byte aligned, and steps may end in the
+// middle).  Without TAIL: kt0 and nk in whole rounds of kStages steps.
 // put(i, j, v): v[e] = the sum of tile row 16 i + r and the wave's weight row 16
 // j + 4 c + e.
-template <int DT, bool QQ, int BM, bool TAIL, class XOff, class SOff, class Put>
+template <int DT, int BM, bool TAIL, class XOff, class Put>
 __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
-                                        __amdgpu_buffer_rsrc_t xs, SOff soff,
                                         const uint32_t* __restrict__ w,
                                         const uint8_t* __restrict__ scales, int ncols, int G,
                                         int kt0, int nk, Put put, unsigned char* __restrict__ A0,
@@ -61,16 +51,13 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
   constexpr int ST = MxTileShape<BM>::kStages, MB = BM / 16, SLOTS = 4 * MB, DM = BM / 16;
   // slots a fragment is read ahead, and fragment registers
   constexpr int P = MB == 1 ? 2 : MB <= 4 ? 3 : 6, R = MB == 1 ? 4 : 8;
-  static_assert(!QQ || MB >= P + 1, "scale bytes are read with the first substep's fragments");
   static_assert(SLOTS % R == 0 && P < R, "a step's slots run through whole rings");
-  constexpr int WQ = QQ ? 4 : 1;                // 16-byte weight loads per block and step
-  constexpr int SQ = TAIL ? (QQ ? 4 : 1) : (QQ ? 1 : 0);   // scale loads per block and step
-  constexpr int XS = QQ ? 1 : 0;                // scale loads of x per wave and step
-  constexpr int NL = DM + XS + 4 * WQ + 4 * SQ;
+  constexpr int SQ = TAIL ? 1 : 0;              // scale loads per block and step
+  constexpr int NW = 4 + 4 * SQ, NL = NW + DM;  // loads of weights, of all, per wave and step
   // Steps of weights and of their scale bytes in registers, as many as the sums
-  // leave room for (T, 64 rows: with two, a step waited for the weights of the
+  // leave room for (64 rows: with two, a step waited for the weights of the
   // step before it).
-  constexpr int WR = QQ ? (BM >= 192 ? 1 : 2) : BM >= 192 ? 2 : 4, SR = QQ ? 2 : WR;
+  constexpr int WR = BM >= 192 ? 2 : 4;
   constexpr bool PAIR = WR == 4;
   using T = T16<DT>;
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, c = lane >> 4;
@@ -95,12 +82,12 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
   };
   uint32_t fo[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) fo[q] = zero + r * 256 + (((QQ ? 4 * q + c : 4 * c + q) ^ r) << 4);
-  uint32_t dmo[DM], dso = 0;
+  for (int q = 0; q < 4; ++q) fo[q] = zero + r * 256 + (((4 * c + q) ^ r) << 4);
+  uint32_t dmo[DM];
 
-  u32x4 W[WR][4][WQ];
-  u32x4 S[SR][4];                               // scale bytes: [0], or by substep
-  // T, whole rounds: a round's scale bytes (four per step) in one load per block.
+  u32x4 W[WR][4];
+  uint32_t S[WR][4];                            // TAIL: scale bytes
+  // Whole rounds: a round's scale bytes (four per step) in one load per block.
   // Byte loads for every step brought each row's line to the L1 again, as much
   // as the weights (N=5120 K=17408, 45 rows, 12 splits: 40 against 32 us).
   uint32_t cur[4][ST], nxt[4][ST];
@@ -124,39 +111,24 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
   auto at = [&](int s, uint32_t b) { return s < nk ? (uint32_t)(kt0 + s) * b : 0x80000000u; };
   // item v of the loads of step s, into stage / ring slot sc
   auto load = [&](int s, auto sc, auto vc) {
-    constexpr int v = decltype(vc)::value;
-    constexpr int SW = decltype(sc)::value % WR, SS = decltype(sc)::value % SR;
+    constexpr int v = decltype(vc)::value, SW = decltype(sc)::value % WR;
     const int k = kt0 + s;
-    if constexpr (v < 4 * WQ) {
-      constexpr int j = v / WQ, q = v % WQ;
-      uint32_t o = wo[j];
-      if constexpr (TAIL && !QQ) o = 4 * k + c < G ? o : 0x80000000u;
-      W[SW][j][q] = __builtin_amdgcn_raw_buffer_load_b128(rw, o + 64u * q, at(s, 64u * WQ), 0);
-    } else if constexpr (v < 4 * WQ + 4 * SQ) {
-      constexpr int n = SQ ? SQ : 1, j = (v - 4 * WQ) / n, q = (v - 4 * WQ) % n;
-      if constexpr (QQ && !TAIL) {
-        S[SS][j] = __builtin_amdgcn_raw_buffer_load_b128(rs, so[j], at(s, 16u), 0);
-      } else {
-        uint32_t o = so[j];
-        if constexpr (TAIL) o = (QQ ? 16 * k + 4 * q : 4 * k) + c < G ? o : 0x80000000u;
-        S[SS][j][q] = __builtin_amdgcn_raw_buffer_load_b8(rs, o + 4u * q, at(s, 4u * WQ), 0);
-      }
-    } else if constexpr (v < NL - XS) {
-      constexpr int i = v - 4 * WQ - 4 * SQ;
+    if constexpr (v < 4) {
+      uint32_t o = wo[v];
+      if constexpr (TAIL) o = 4 * k + c < G ? o : 0x80000000u;
+      W[SW][v] = __builtin_amdgcn_raw_buffer_load_b128(rw, o, at(s, 64u), 0);
+    } else if constexpr (v < NW) {
+      const uint32_t o = 4 * k + c < G ? so[v - 4] : 0x80000000u;
+      S[SW][v - 4] = __builtin_amdgcn_raw_buffer_load_b8(rs, o, at(s, 4u), 0);
+    } else {
+      constexpr int i = v - NW;
       uint32_t o = dmo[i];
-      if constexpr (TAIL && !QQ) {
+      if constexpr (TAIL) {
         const int p = (lane & 15) ^ (4 * ((wave * DM + i) & 3) + (lane >> 4));
         o = 4 * k + (p >> 2) < G ? o : 0x80000000u;
       }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          xr, (lds_void*)(stage(sc) + (wave * DM + i) * 1024), 16, o, at(s, 256u), 0,
-          0);
-    } else {
-      // every wave loads 64 rows, past the tile's zeros (no branch: the compiler
-      // would sink the MFMAs below it)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          xs, (lds_void*)(stage(sc) + BM * 256 + wave * 1024), 16, dso, at(s, 16u), 0,
-          0);
+          xr, (lds_void*)(stage(sc) + (wave * DM + i) * 1024), 16, o, at(s, 256u), 0, 0);
     }
   };
 
@@ -169,33 +141,22 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
       // zeros of their own: from one shared zero the compiler made the first
       // MFMA of every sum in the loop read a copy (192 moves and their waits
       // per 384 MFMAs; M=2048 316 against 272 us)
-      if constexpr (BM > 64 || QQ) asm volatile("" : "+a"(acc[i][j]));
+      if constexpr (BM > 64) asm volatile("" : "+a"(acc[i][j]));
     }
   u32x4 A[R];
-  u32x4 B[2][4];                                // T operands of a substep
-  uint32_t xe[MB], we[2][4];                    // QQ: scale bytes (of four substeps; of one)
+  u32x4 B[2][4];                                // weight operands of a substep
   float sf[4];
   auto frag = [&](auto sc, auto tc) {           // fragment of slot t of stage sc
     constexpr int t = decltype(tc)::value, q = t / MB, i = t % MB;
     A[t % R] = *reinterpret_cast<const u32x4*>(stage(sc) + fo[q] + 4096 * i);
-    if constexpr (QQ && q == 0)
-      xe[i] = *reinterpret_cast<const uint32_t*>(stage(sc) + zero + BM * 256 + 256 * i + 16 * r +
-                                                 4 * c);
   };
-  // piece x of 16 of the operands of substep q from ring slot sw into B / we [q & 1]
+  // piece x of 16 of the operands of substep q from ring slot sw into B[q & 1]
   auto piece = [&](auto swc, auto qc, auto xc) {
-    constexpr int SW = decltype(swc)::value % WR, SS = decltype(swc)::value % SR;
-    constexpr int q = decltype(qc)::value;
+    constexpr int u = decltype(swc)::value, q = decltype(qc)::value;
     constexpr int x = decltype(xc)::value, j = x / 4, e = x % 4;
-    if constexpr (QQ) {
-      if constexpr (e == 0) we[q & 1][j] = TAIL ? S[SS][j][q] : S[SS][j][q] >> (8 * c);
-    } else {
-      if constexpr (q == 0 && e == 0) {
-        constexpr int i = decltype(swc)::value % ST;
-        sf[j] = mx_scale(TAIL ? S[SS][j][0] : (cur[j][i] >> (8 * c)) & 255u);
-      }
-      B[q & 1][j][e] = mx_pair<DT, e>(W[SW][j][0][q], sf[j]);
-    }
+    if constexpr (q == 0 && e == 0)
+      sf[j] = mx_scale(TAIL ? S[u % WR][j] : (cur[j][u % ST] >> (8 * c)) & 255u);
+    B[q & 1][j][e] = mx_pair<DT, e>(W[u % WR][j][q], sf[j]);
   };
   auto barrier = [&](auto vmc) {
     __builtin_amdgcn_sched_barrier(0);
@@ -211,11 +172,9 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
   using I3 = std::integral_constant<int, 3>;
 
   // prologue: the weights first (x rows may have to be looked up)
-  if constexpr (!QQ && !TAIL) sround(0, cur);
-  constexpr int NW = 4 * WQ + 4 * SQ;
-  constexpr int NWB = 4 * WQ;
+  if constexpr (!TAIL) sround(0, cur);
   static_for<0, NW>([&](auto vc) { load(0, I0{}, vc); });
-  static_for<WR == 1 ? NWB : 0, NW>([&](auto vc) { load(1, I1{}, vc); });
+  static_for<0, NW>([&](auto vc) { load(1, I1{}, vc); });
   if constexpr (WR == 4) {
     static_for<0, NW>([&](auto vc) { load(2, I2{}, vc); });
     static_for<0, NW>([&](auto vc) { load(3, I3{}, vc); });
@@ -225,28 +184,22 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
     const int row = 4 * (wave * DM + i) + (lane >> 4);
     dmo[i] = xoff(row) + 16u * (uint32_t)((lane & 15) ^ (row & 15));
   }
-  if constexpr (QQ) dso = 64 * wave + lane < BM ? soff(64 * wave + lane) : 0x80000000u;
   static_for<NW, NL>([&](auto vc) { load(0, I0{}, vc); });
   if constexpr (ST > 2) {
     static_for<NW, NL>([&](auto vc) { load(1, I1{}, vc); });
     static_for<NW, NL>([&](auto vc) { load(2, I2{}, vc); });
   }
-  barrier(std::integral_constant<int, (ST - 2) * (DM + XS)>{});
+  barrier(std::integral_constant<int, (ST - 2) * DM>{});
   static_for<0, P>([&](auto tc) { frag(I0{}, tc); });
   static_for<0, 16>([&](auto xc) { piece(I0{}, I0{}, xc); });
 
-  // A step issues, in this order: in its first substep the x of step s + ST - 1;
-  // QQ: after each substep its weights of step s + WR; in the last substep,
-  // before the barrier, the scale bytes (T: and the weights) of step s + SR, or,
-  // PAIR, in every second step's those of the next two steps' successors.
-  // Flight: those issued after the x of step s + 1, which the wait before the
-  // barrier may leave in flight.
+  // A step issues, in this order: in its first substep the x of step s + ST - 1; in
+  // the last substep, before the barrier, the weights of step s + WR, or, PAIR, in
+  // every second step's those of the next two steps' successors.  Flight: those
+  // issued after the x of step s + 1, which the wait before the barrier may leave in
+  // flight.
   constexpr int FREE = SLOTS - P;
-  constexpr int kLate = (QQ ? 8 + (MB - P < 4 ? MB - P : 4) : 0) + NW - (QQ ? NWB : 0);
-  constexpr int kAll = QQ ? 16 + NW - NWB : NW;
-  // (pairs: 2 NW in every second step, so as many in any two steps)
-  constexpr int kFlight =
-      ST == 2 ? kLate : 2 * (DM + XS) + (PAIR ? 2 * NW : 2 * kAll + kLate);
+  constexpr int kFlight = ST == 2 ? NW : 2 * DM + 2 * NW;
   using Flight = std::integral_constant<int, (kFlight < 63 ? kFlight : 63)>;
   // one step; u: its stage
   auto step = [&](int s, auto uc) {
@@ -260,21 +213,8 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
       if constexpr (t + P < SLOTS) frag(U{}, std::integral_constant<int, t + P>{});
       else frag(N1{}, std::integral_constant<int, t + P - SLOTS>{});
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (QQ) {
-          const i32x8 a = __builtin_shufflevector(bitcast<i32x4>(W[u % WR][j][q]),
-                                                  bitcast<i32x4>(W[u % WR][j][q]), 0, 1, 2, 3, -1,
-                                                  -1, -1, -1);
-          const i32x8 b = __builtin_shufflevector(bitcast<i32x4>(A[t % R]),
-                                                  bitcast<i32x4>(A[t % R]), 0, 1, 2, 3, -1, -1, -1,
-                                                  -1);
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              a, b, acc[i][j], 4, 4, 0, (int)we[q & 1][j], q, (int)xe[i]);
-        } else {
-          acc[i][j] = T::mfma(B[q & 1][j], A[t % R], acc[i][j]);
-        }
-      }
-      if constexpr (!QQ && !TAIL) {
+      for (int j = 0; j < 4; ++j) acc[i][j] = T::mfma(B[q & 1][j], A[t % R], acc[i][j]);
+      if constexpr (!TAIL) {
         if constexpr (u == 0 && q == 1 && i == 0) sround(s + ST, nxt);
         if constexpr (u == ST - 1 && q == 3 && i == 0) {
 #pragma unroll
@@ -292,9 +232,6 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
         static_for<i * (NL - NW) / MB, (i + 1) * (NL - NW) / MB>([&](auto vc) {
           load(s + ST - 1, XN{}, std::integral_constant<int, NW + decltype(vc)::value>{});
         });
-      if constexpr (QQ && q > 0 && i < 4)
-        load(s + WR, std::integral_constant<int, u + WR>{},
-             std::integral_constant<int, i * WQ + q - 1>{});
       if constexpr (PAIR) {
         // both halves of a line together, in the second step of a pair
         if constexpr (q == 3 && (u & 1))
@@ -303,19 +240,13 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
             load(s + 4, std::integral_constant<int, u + 4>{}, vc);
           });
       } else if constexpr (q == 3 && t < FREE) {
-        constexpr int F = QQ ? NWB : 0, n = MB - P;
-        static_for<i * (NW - F) / n, (i + 1) * (NW - F) / n>([&](auto vc) {
-          load(s + SR, std::integral_constant<int, u + SR>{},
-               std::integral_constant<int, F + decltype(vc)::value>{});
+        constexpr int n = MB - P;
+        static_for<i * NW / n, (i + 1) * NW / n>([&](auto vc) {
+          load(s + WR, std::integral_constant<int, u + WR>{}, vc);
         });
       }
       __builtin_amdgcn_sched_barrier(0);
     });
-    if constexpr (QQ)
-      static_for<0, 4>([&](auto jc) {
-        load(s + WR, std::integral_constant<int, u + WR>{},
-             std::integral_constant<int, decltype(jc)::value * WQ + 3>{});
-      });
   };
   // Whole rounds of the stages, in a loop that is left at its end alone (left
   // in its middle, loads into registers may be moved past the exits, and no

@@ -1,12 +1,13 @@
-// Wide MXFP4 products on the tile of mx_tile.cuh: quantized_matmul (T) and qqmm
-// (QQ: x packed into codes by mx_pack_kernel first).
+// Wide MXFP4 products: quantized_matmul (T) on the tile of mx_tile.cuh and qqmm (QQ:
+// x packed into codes by mx_pack_kernel first) on that of mx_code.cuh.
 #pragma once
 #include "dense.cuh"
+#include "mx_code.cuh"
 #include "mx_tile.cuh"
 
 namespace mq {
 
-// x [M, K] -> codes and scales as the 4-bit tile takes them (mx_tile.cuh): a
+// x [M, K] -> codes and scales as the 4-bit tile takes them (mx_code.cuh): a
 // thread takes 8 values, a group's four threads agree on its scale, groups past
 // K are zero.  units = M * steps * 64.
 template <int DT>
@@ -31,22 +32,41 @@ __global__ __launch_bounds__(256) void mx_pack_kernel(const uint16_t* __restrict
     scales[(row * steps + (g >> 4)) * 16 + 4 * (g & 3) + ((g >> 2) & 3)] = (uint8_t)e;
 }
 
-// A tile and a share z of the steps per workgroup, placed so that an XCD runs a
-// contiguous range of weight columns and shares over all rows (grouped_tile);
-// where part is given the sums go to its float plane part[z].
+// Tiles of rows that run side by side: six by five columns of weights move about as
+// few bytes of x as of weights through an XCD's L2 (4096 rows, T, N=17408 K=5120:
+// 522 us, all rows side by side 543).
+constexpr int kMxGroupTiles = 6;
+
+// Tile i: an XCD (i % 8) runs a contiguous range of the tiles in the order of
+// groups of up to kMxGroupTiles tiles of rows, then weight columns (and shares of K), then
+// the group's rows, so that the tiles that it runs at a time share both their x and
+// their weights in its L2.
+__device__ __forceinline__ bool mx_wide_tile(int i, int ncol, int mtiles, int& cz,
+                                             int& mt) {
+  int tile, one;
+  if (!grouped_tile(i, ncol * mtiles, 1, tile, one)) return false;
+  const int ng = (mtiles + kMxGroupTiles - 1) / kMxGroupTiles, h = (mtiles + ng - 1) / ng;
+  const int g = tile / (h * ncol), rest = tile - g * h * ncol, rows = min(h, mtiles - g * h);
+  cz = rest / rows;
+  mt = g * h + rest - cz * rows;
+  return true;
+}
+
+// A tile and a share z of the steps per workgroup (mx_wide_tile); where part is
+// given the sums go to its float plane part[z].
 template <int DT, bool QQ, int BM, bool TAIL>
 __global__ __launch_bounds__(256, BM <= 64 && !QQ ? 2 : 1) void mx_wide_kernel(
     const void* __restrict__ x, const uint8_t* __restrict__ xscales,
     const uint32_t* __restrict__ w, const uint8_t* __restrict__ scales,
     uint16_t* __restrict__ out, float* __restrict__ part, int M, int N, int G, int splits) {
   using Sh = MxTileShape<BM>;
-  constexpr int kBytes = Sh::kStage + (QQ ? Sh::kScales : 0);
-  __shared__ __align__(16) unsigned char A0[kBytes];
-  __shared__ __align__(16) unsigned char A1[kBytes];
-  __shared__ __align__(16) unsigned char A2[Sh::kStages > 2 ? kBytes : 16];
-  __shared__ __align__(16) unsigned char A3[Sh::kStages > 2 ? kBytes : 16];
+  using Shc = MxCodeShape<BM>;
+  __shared__ __align__(16) unsigned char A0[QQ ? Shc::kHalf : Sh::kStage];
+  __shared__ __align__(16) unsigned char A1[QQ ? Shc::kHalf : Sh::kStage];
+  __shared__ __align__(16) unsigned char A2[QQ ? Shc::kScales : Sh::kStages > 2 ? Sh::kStage : 16];
+  __shared__ __align__(16) unsigned char A3[!QQ && Sh::kStages > 2 ? Sh::kStage : 16];
   int cz, mt;
-  if (!grouped_tile(blockIdx.x, (N + 255) / 256 * splits, (M + BM - 1) / BM, cz, mt)) return;
+  if (!mx_wide_tile(blockIdx.x, (N + 255) / 256 * splits, (M + BM - 1) / BM, cz, mt)) return;
   const int col = cz / splits, z = cz - col * splits;
   const int m0 = mt * BM, n0 = col * 256;
   const int mrows = min(BM, M - m0), ncols = min(256, N - n0);
@@ -62,36 +82,47 @@ __global__ __launch_bounds__(256, BM <= 64 && !QQ ? 2 : 1) void mx_wide_kernel(
   const auto xs = wide_rsrc(QQ ? xscales + (int64_t)m0 * steps * 16 : nullptr,
                             QQ ? (int64_t)mrows * steps * 16 : 0);
   const bool vec = N % 4 == 0 && (part || (uintptr_t)out % 8 == 0);
-  mx_tile<DT, QQ, BM, TAIL>(
-      xr, [&](int i) { return i < mrows ? (uint32_t)i * rowb : 0x80000000u; }, xs,
-      [&](int i) { return i < mrows ? (uint32_t)i * (uint32_t)steps * 16u : 0x80000000u; },
-      w + (int64_t)n0 * G * 4, scales + (int64_t)n0 * G, ncols, G, kt0, kt1 - kt0,
-      [&](int i, int j, const f32x4& v) {
-        const int m = 16 * i + r, n = 64 * wave + 16 * j + 4 * c;
-        if (m >= mrows) return;
-        if (part) {
-          float* o = part + ((int64_t)z * M + m0 + m) * N + n0 + n;
-          if (vec) {
-            if (n < ncols) *reinterpret_cast<f32x4*>(o) = v;
-          } else {
+  // the four sums v of x row m and weight rows n ..
+  auto put = [&](int m, int n, const f32x4& v) {
+    if (m >= mrows) return;
+    if (part) {
+      float* o = part + ((int64_t)z * M + m0 + m) * N + n0 + n;
+      if (vec) {
+        if (n < ncols) *reinterpret_cast<f32x4*>(o) = v;
+      } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < ncols) o[e] = v[e];
-          }
-          return;
-        }
-        uint16_t* o = out + (int64_t)(m0 + m) * N + n0 + n;
-        if (vec) {
-          if (n < ncols)
-            *reinterpret_cast<u32x2*>(o) =
-                (u32x2){T16<DT>::pack2(v[0], v[1]), T16<DT>::pack2(v[2], v[3])};
-        } else {
+        for (int e = 0; e < 4; ++e)
+          if (n + e < ncols) o[e] = v[e];
+      }
+      return;
+    }
+    uint16_t* o = out + (int64_t)(m0 + m) * N + n0 + n;
+    if (vec) {
+      if (n < ncols)
+        *reinterpret_cast<u32x2*>(o) =
+            (u32x2){T16<DT>::pack2(v[0], v[1]), T16<DT>::pack2(v[2], v[3])};
+    } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < ncols) o[e] = T16<DT>::round1(v[e]);
-        }
-      },
-      A0, A1, A2, A3);
+      for (int e = 0; e < 4; ++e)
+        if (n + e < ncols) o[e] = T16<DT>::round1(v[e]);
+    }
+  };
+  const uint32_t* wt = w + (int64_t)n0 * G * 4;
+  const uint8_t* st = scales + (int64_t)n0 * G;
+  if constexpr (QQ)
+    mx_code_tile<BM, TAIL>(
+        xr, xs, wt, st, ncols, G, steps, kt0, kt1 - kt0,
+        [&](int i, int j, const f32x4& v) {
+          put(BM / 2 * (wave & 1) + 16 * i + r, 128 * (wave >> 1) + 16 * j + 4 * c, v);
+        },
+        A0, A1, A2);
+  else
+    mx_tile<DT, BM, TAIL>(
+        xr, [&](int i) { return i < mrows ? (uint32_t)i * rowb : 0x80000000u; }, wt, st, ncols, G, kt0, kt1 - kt0,
+        [&](int i, int j, const f32x4& v) {
+          put(16 * i + r, 64 * wave + 16 * j + 4 * c, v);
+        },
+        A0, A1, A2, A3);
 }
 
 template <int DT, bool QQ, int BM>
