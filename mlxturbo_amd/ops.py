@@ -1168,6 +1168,7 @@ def moe_layer(x: torch.Tensor, rhs_indices: torch.Tensor, weights: torch.Tensor,
     ``gate``, ``up``, ``down`` are ``(w, scales, biases)`` banks.  Returns
     ``(T, N)``, the bits of the two calls; up to 8 tokens run both in one
     launch (mq_moe_layer) where its tile configurations apply."""
+    group_size, bits = _format(group_size, bits, mode)
     T, K = x.shape
     idx = rhs_indices.reshape(T, -1)
     if 1 <= T <= _BLOCK_MAX_T and mode == "affine":
