@@ -94,4 +94,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_scale_rsrc(const uint8_t* f
   return wide_rsrc(reinterpret_cast<const void*>(a - skew), (bytes + skew + 3) & ~(int64_t)3);
 }
 
+// Whether a grid of n workgroups of `threads` has a launch's 32-bit thread count.
+inline bool mx_grid_ok(int64_t n, int64_t threads) { return n <= (int64_t)UINT32_MAX / threads; }
+
 }  // namespace mq

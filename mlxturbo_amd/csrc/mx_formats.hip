@@ -108,7 +108,7 @@ inline int64_t mx_blocks(int64_t units) {
 int launch_mx_quantize(const void* w, uint32_t* wq, uint8_t* scales, int64_t N, int64_t K,
                        int dtype, hipStream_t st) {
   const int64_t units = N * (K / 8), nb = mx_blocks(units);
-  if (nb > INT32_MAX) return kStatusUnsupported;
+  if (!mx_grid_ok(nb, kMxThreads)) return kStatusUnsupported;
 #define MQ_MXQ(DT)                                                                            \
   hipLaunchKernelGGL(mx_quantize_kernel<DT>, dim3((unsigned)nb), dim3(kMxThreads), 0, st, w, wq, \
                      scales, units)
@@ -122,7 +122,7 @@ int launch_mx_quantize(const void* w, uint32_t* wq, uint8_t* scales, int64_t N, 
 int launch_mx_dequantize(const uint32_t* wq, const uint8_t* scales, void* out, int64_t N,
                          int64_t K, int dtype, hipStream_t st) {
   const int64_t units = N * (K / 8), nb = mx_blocks(units);
-  if (nb > INT32_MAX) return kStatusUnsupported;
+  if (!mx_grid_ok(nb, kMxThreads)) return kStatusUnsupported;
 #define MQ_MXD(DT)                                                                              \
   hipLaunchKernelGGL(mx_dequantize_kernel<DT>, dim3((unsigned)nb), dim3(kMxThreads), 0, st, wq, \
                      scales, out, units)

@@ -262,7 +262,7 @@ int MxGroupedLaunch<DT>::run(const void* x, const uint32_t* w, const uint8_t* s,
   const bool tall = P * M / (P < E ? P : E) >= 96;
   const int64_t ncol = (N + 255) / 256, R = (tall ? 192 : 64) / M;
   const int64_t nwg = (class_seg_bound(P, R, 0, E) * ncol + 7) / 8 * 8;
-  if (nwg > INT32_MAX) return kStatusUnsupported;
+  if (!mx_grid_ok(nwg, 256)) return kStatusUnsupported;
   const bool sorted = P <= kMxSortP;
   if (!sorted) {
     if (int rc = launch_prep(rhs, lhs, P, E, B, (int)R, ws, st)) return rc;

@@ -39,11 +39,11 @@ inline size_t mx_pack_bytes(int64_t M, int64_t K) {
   return (size_t)(M * ((K + 511) / 512)) * (kMxStepBytes + 16);
 }
 
-// A tile's x rows and weight rows have to fit 31-bit buffer ranges, the grid
-// its limits.
+// A tile's x rows and weight rows have to fit 31-bit buffer ranges, the grids (the
+// packing of x has 64 threads per row and 512 codes) 32-bit thread counts.
 inline bool mx_wide_fits(int64_t M, int64_t N, int64_t K) {
-  return K < ((int64_t)1 << 21) && (M + 63) / 64 * ((N + 255) / 256) < INT32_MAX - 8 &&
-         M * ((K + 511) / 512) < ((int64_t)1 << 31) && M * N < ((int64_t)1 << 40);
+  return K < ((int64_t)1 << 21) && (M + 63) / 64 * ((N + 255) / 256) < ((int64_t)1 << 24) - 8 &&
+         M * ((K + 511) / 512) < ((int64_t)1 << 26) && M * N < ((int64_t)1 << 40);
 }
 
 // Tile height and K split of least modelled cost, fitted to K=5120 N=17408 and

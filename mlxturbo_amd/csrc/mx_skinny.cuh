@@ -383,7 +383,7 @@ int MxSkinnyLaunch<DT, QQ>::run(const void* x, const uint32_t* w, const uint8_t*
     constexpr int R = mx_rows<F>();
     const size_t lds = mx_skinny_lds<F, NT, KW>(G);
     const int64_t gx = (N + 16 * NT - 1) / (16 * NT), gy = (M + R - 1) / R;
-    if ((int64_t)lds > kMxLdsMax || gy > 65535) return kStatusUnsupported;
+    if ((int64_t)lds > kMxLdsMax || gy > 65535 || !mx_grid_ok(gx, 64 * KW)) return kStatusUnsupported;
     const auto kern = &mx_skinny_kernel<DT, QQ, F, NT, KW>;
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(kern), (int)kMxLdsMax,
@@ -417,11 +417,11 @@ int MxGatherLaunch<DT>::run(const void* x, const uint32_t* w, const uint8_t* s,
     constexpr bool FUSED = decltype(fused)::value;
     const size_t lds = mx_skinny_lds<F, NT, KW>(G);
     const int64_t ncol = (N + 16 * NT - 1) / (16 * NT), R = mx_rows<F>() / M;
-    if ((int64_t)lds > kMxLdsMax) return kStatusUnsupported;
+    if ((int64_t)lds > kMxLdsMax || !mx_grid_ok(ncol, 64 * KW)) return kStatusUnsupported;
     dim3 grid((unsigned)ncol, (unsigned)P);
     if (!FUSED) {
       const int64_t nwg = (class_seg_bound(P, R, 0, E) * ncol + 7) / 8 * 8;
-      if (nwg > INT32_MAX) return kStatusUnsupported;
+      if (!mx_grid_ok(nwg, 64 * KW)) return kStatusUnsupported;
       if (int rc = launch_prep(rhs, lhs, P, E, B, (int)R, ws, st)) return rc;
       *nlaunch += kPrepLaunches;
       grid = dim3((unsigned)nwg);

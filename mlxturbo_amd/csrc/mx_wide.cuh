@@ -130,7 +130,7 @@ inline int mx_wide_launch_bm(const void* x, const uint8_t* xs, const uint32_t* w
                              const uint8_t* s, void* out, int64_t M, int64_t N, int64_t K,
                              int splits, float* part, hipStream_t st) {
   const int64_t G = K / kMxGroup, tiles = (N + 255) / 256 * ((M + BM - 1) / BM) * splits;
-  if ((tiles + 7) / 8 * 8 > INT32_MAX) return kStatusUnsupported;
+  if (!mx_grid_ok((tiles + 7) / 8 * 8, 256)) return kStatusUnsupported;
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
   auto go = [&](auto tail) {
     hipLaunchKernelGGL((mx_wide_kernel<DT, QQ, BM, decltype(tail)::value>), grid, dim3(256), 0,

@@ -19,6 +19,7 @@ errors are theirs.
 from __future__ import annotations
 
 import math
+import threading
 from typing import Optional
 
 import torch
@@ -58,6 +59,12 @@ def _no_biases(biases) -> None:
         raise NotImplementedError("mode='mxfp4': its codes have no biases")
 
 
+def _elsewhere(dev: torch.device) -> bool:
+    """Whether the tensors live on another device than the current one (launches
+    and workspaces go by the current one)."""
+    return dev.type == "cuda" and dev.index != torch._C._cuda_getDevice()
+
+
 def _float_type(dtype: torch.dtype) -> None:
     if dtype not in ops._DTYPE_CODE:
         raise ValueError(f"mxfp4 operators take bfloat16, float16 or float32, got {dtype}")
@@ -65,6 +72,9 @@ def _float_type(dtype: torch.dtype) -> None:
 
 def quantize(w: torch.Tensor):
     dev = ops._require_gpu(w)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return quantize(w)
     if w.dtype not in ops._DTYPE_CODE:
         raise ValueError(f"w must be bfloat16, float16 or float32, got {w.dtype}")
     if w.ndim < 1:
@@ -90,6 +100,9 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None,
                dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     _no_biases(biases)
     dev = ops._require_gpu(w, scales)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return dequantize(w, scales, dtype=dtype)
     scales = _scales(scales)
     K = _check(w, scales)
     dtype = torch.bfloat16 if dtype is None else dtype
@@ -111,18 +124,37 @@ def _composed(x, w, scales, transpose: bool) -> torch.Tensor:
     return torch.nn.functional.linear(x, deq) if transpose else torch.matmul(x, deq)
 
 
+# A call's launches follow each other on the stream, as they share its workspace
+# with the calls of other threads there.
+_LAUNCH = threading.Lock()
+
+
+def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
+    """A workspace: the stream's, or in a capture one of the graph's own memory
+    (graphs captured on one stream may be replayed on two at once)."""
+    if ops._capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ops._workspace(dev, nbytes)
+
+
 def _product(call, size, x, w, s, out, M: int, N: int, K: int) -> int:
-    """One product call with this stream's workspace; its status."""
+    """One product call, with a workspace where it needs one; its status."""
+    args = (x.data_ptr(), w.data_ptr(), s.data_ptr(), out.data_ptr(), M, N, K,
+            ops._DTYPE_CODE[out.dtype])
     nbytes = int(size(M, N, K)) if M > 16 else 0     # up to 16 rows use none
-    ws = ops._workspace(out.device, nbytes) if nbytes else None
-    return call(x.data_ptr(), w.data_ptr(), s.data_ptr(), out.data_ptr(), M, N, K,
-                ops._DTYPE_CODE[out.dtype], ops._ptr(ws), ws.numel() if ws is not None else 0,
-                ops._stream_ptr(out))
+    if not nbytes:
+        return call(*args, None, 0, ops._stream_ptr(out))
+    with _LAUNCH:
+        ws = _scratch(out.device, nbytes)
+        return call(*args, ws.data_ptr(), ws.numel(), ops._stream_ptr(out))
 
 
 def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
     _no_biases(biases)
     dev = ops._require_gpu(x, w, scales)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return quantized_matmul(x, w, scales, None, transpose)
     if w.ndim != 2:
         raise NotImplementedError("batched w: only 2-D weights are on this path")
     scales = _scales(scales)
@@ -154,6 +186,9 @@ def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
 
 def qqmm(x, w, scales) -> torch.Tensor:
     dev = ops._require_gpu(x, w, scales)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return qqmm(x, w, scales)
     if w.ndim != 2:
         raise NotImplementedError("batched w: only 2-D weights are on this path")
     scales = _scales(scales)
@@ -188,12 +223,15 @@ def _gather_launch(x, flat, lhs, rhs, out, P, B, M, N, K, E, group_size, bits,
     x_ = ops._aligned(x)
     w_, s_ = (ops._aligned(t) for t in flat)
     lib = _lib.lib()
+    args = (x_.data_ptr(), w_.data_ptr(), s_.data_ptr(), ops._ptr(lhs), rhs.data_ptr(),
+            out.data_ptr(), P, B, M, N, K, E, ops._DTYPE_CODE[x.dtype])
     nbytes = int(lib.mq_mxfp4_gather_qmm_workspace_size(P, M))
-    ws = ops._workspace(out.device, nbytes) if nbytes else None
-    rc = lib.mq_mxfp4_gather_qmm(x_.data_ptr(), w_.data_ptr(), s_.data_ptr(), ops._ptr(lhs),
-                                 rhs.data_ptr(), out.data_ptr(), P, B, M, N, K, E,
-                                 ops._DTYPE_CODE[x.dtype], ops._ptr(ws),
-                                 ws.numel() if ws is not None else 0, ops._stream_ptr(out))
+    if not nbytes:
+        rc = lib.mq_mxfp4_gather_qmm(*args, None, 0, ops._stream_ptr(out))
+    else:
+        with _LAUNCH:
+            ws = _scratch(out.device, nbytes)
+            rc = lib.mq_mxfp4_gather_qmm(*args, ws.data_ptr(), ws.numel(), ops._stream_ptr(out))
     _lib.check(rc, "gather_qmm")
 
 
@@ -201,6 +239,10 @@ def gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose: bool,
                sorted_indices: bool) -> torch.Tensor:
     _no_biases(biases)
     dev = ops._require_gpu(x, w, scales)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return gather_qmm(x, w, scales, None, lhs_indices, rhs_indices, transpose,
+                              sorted_indices)
     if x.ndim < 2 or w.ndim < 3:
         raise ValueError("gather_qmm needs x (..., M, K) and w (..., N, K*bits/32) with a batch dim")
     scales = _scales(scales)
@@ -225,8 +267,12 @@ def gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose: bool,
     if not composed and M <= 16 and (
             E <= ops._GATHER_PREP_MAX_E
             or not _lib.lib().mq_mxfp4_gather_qmm_workspace_size(P, M)):
-        _gather_launch(x, bank, lhs, rhs, out, P, B, M, N, K, E, GROUP_SIZE, BITS, sorted_indices)
-        return out
+        try:
+            _gather_launch(x, bank, lhs, rhs, out, P, B, M, N, K, E, GROUP_SIZE, BITS,
+                           sorted_indices)
+            return out
+        except NotImplementedError:                  # beyond the kernels' address ranges
+            composed = True
     a = dict(x=x.reshape(B, M, K), flat=bank, lhs=lhs, rhs=rhs, P=P, B=B, M=M, N=N, K=K, E=E,
              dev=dev, transpose=transpose, shape=shape, dtype=x.dtype, launch=_gather_launch)
     if composed:

@@ -1,5 +1,7 @@
 """The MXFP4 operators on the GPU against their definitions in 64 bits."""
 
+import threading
+
 import pytest
 import torch
 
@@ -333,6 +335,17 @@ def test_gather_composed_forms():
     _check(out[0], xt[0], v[2].T.contiguous(), torch.bfloat16)
 
 
+def test_products_of_rows_too_long_for_the_kernels():
+    g = _gen(20)
+    E, N, K = 2, 8, 32 * 9216
+    w, s, v = weights(g, E, N, K)
+    x = _randn(g, 3, 1, K, dtype=torch.bfloat16)
+    rhs = torch.tensor([1, 0, 1], device="cuda")
+    _check_gather(mq.gather_qmm(x, w, s, rhs_indices=rhs, **KW), x, v,
+                  torch.arange(3, device="cuda"), rhs)
+    _check(mq.quantized_matmul(x[:, 0], w[0], s[0], **KW), x[:, 0], v[0], torch.bfloat16)
+
+
 def test_offsets_past_32_bits():
     g = _gen(10)
     # a bank whose last experts' codes lie past 4 GB
@@ -418,6 +431,50 @@ def test_graph_replays():
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_graphs_of_one_stream_replay_side_by_side():
+    """Two graphs captured on one stream do not share a workspace."""
+    st = torch.cuda.Stream()
+    calls = [_calls(_gen(16)), _calls(_gen(17))]
+    want = [run() for _, run in calls]
+    graphs = []
+    st.wait_stream(torch.cuda.current_stream())
+    for _, run in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            out = run()
+        graphs.append((graph, out))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(5):
+        for s, (graph, out) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for o in out:
+                    o.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for w, (_, out) in zip(want, graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, w)), i
+
+
+def test_threads_share_a_stream():
+    calls = [_calls(_gen(18)), _calls(_gen(19))]
+    want = [run() for _, run in calls]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        for _ in range(40):
+            got = calls[k][1]()
+            bad.extend(k for a, b in zip(got, want[k]) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
 
 
 def test_launches_are_counted():
