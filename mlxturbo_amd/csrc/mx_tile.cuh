@@ -189,7 +189,9 @@ __device__ __forceinline__ void mx_tile(__amdgpu_buffer_rsrc_t xr, XOff xoff,
     static_for<NW, NL>([&](auto vc) { load(1, I1{}, vc); });
     static_for<NW, NL>([&](auto vc) { load(2, I2{}, vc); });
   }
-  barrier(std::integral_constant<int, (ST - 2) * DM>{});
+  // all of it, also the x of steps 1 and 2: the first steps have fewer loads behind
+  // it than Flight counts
+  barrier(I0{});
   static_for<0, P>([&](auto tc) { frag(I0{}, tc); });
   static_for<0, 16>([&](auto xc) { piece(I0{}, I0{}, xc); });
 

@@ -309,6 +309,26 @@ def test_gather_sorts_any_number_of_pairs(P, E):
     _check_gather(out, x[:1], v, torch.zeros_like(rhs[1:]), rhs[1:])
 
 
+@pytest.mark.parametrize("T,k,E,N,K", [(1500, 8, 400, 512, 2048), (300, 8, 100, 768, 1024),
+                                       (2000, 4, 300, 260, 544)])
+def test_gather_of_many_short_segments(T, k, E, N, K):
+    """Tiles of few rows all over the chip, loads late under the traffic."""
+    g = _gen(T + K)
+    w, s, _ = weights(g, E * N, K)
+    x = _randn(g, T, 1, 1, K, dtype=torch.bfloat16)
+    p = torch.arange(1, E + 1, device="cuda").float() ** -1.0
+    idx = torch.multinomial(p[torch.randperm(E, generator=g, device="cuda")].expand(T, E), k,
+                            generator=g).int()
+    bank = (w.reshape(E, N, -1), s.reshape(E, N, -1))
+    for _ in range(3):
+        out = mq.gather_qmm(x, *bank, rhs_indices=idx, **KW).reshape(T * k, N)
+        flat = idx.reshape(-1)
+        for e in range(0, E, 7):
+            rows = (flat == e).nonzero().flatten()
+            v = mq.dequantize(bank[0][e], bank[1][e], dtype=torch.float32, **KW).double()
+            _check(out[rows], x.reshape(T, K)[rows // k], v, torch.bfloat16)
+
+
 def test_gather_many_experts_in_slices():
     g = _gen(8)
     E, N, K, P = 2050, 16, 32, 400
