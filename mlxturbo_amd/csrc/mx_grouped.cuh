@@ -1,6 +1,5 @@
 // gather_qmm of many pairs on the MXFP4 tile (mx_tile.cuh): a workgroup runs a
-// segment of up to BM rows of one expert (the prep kernels' tables, prep.hip)
-// times 256 weight rows.
+// segment of up to BM rows of one expert times 256 weight rows.
 //
 // x rows are gathered by the tile's LDS-form loads themselves (each lane's row
 // offset is looked up after the first weights are issued) and output rows
