@@ -124,8 +124,8 @@ def _composed(x, w, scales, transpose: bool) -> torch.Tensor:
     return torch.nn.functional.linear(x, deq) if transpose else torch.matmul(x, deq)
 
 
-# A call's launches follow each other on the stream, as they share its workspace
-# with the calls of other threads there.
+# A call's launches follow each other on the stream, as they share its workspace of
+# these operators with the calls of other threads there.
 _LAUNCH = threading.Lock()
 
 
@@ -134,7 +134,7 @@ def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
     (graphs captured on one stream may be replayed on two at once)."""
     if ops._capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return ops._workspace(dev, nbytes)
+    return ops._workspace(dev, nbytes, "mxfp4")
 
 
 def _product(call, size, x, w, s, out, M: int, N: int, K: int) -> int:

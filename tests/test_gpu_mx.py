@@ -559,3 +559,30 @@ def test_switch_glu(T, fuse):
     glu = ops.gather_glu(xe, *banks[0][:2], None, *banks[1][:2], None, rhs_indices=idx, **KW)
     want = torch.nn.functional.silu(gate.float()) * up.float()
     assert torch.equal(glu, want.to(glu.dtype))
+
+
+@pytest.mark.parametrize("T", [1, 5, 400])
+@pytest.mark.parametrize("fuse", [False, True])
+@pytest.mark.parametrize("which", ["down", "gate and up", "up"])
+def test_switch_glu_of_both_formats(T, fuse, which):
+    g = _gen(T + 30)
+    E, k, H, I = 10, 4, 192, 128
+    wf = [_randn(g, E, *s, dtype=torch.bfloat16) * 0.05 for s in ((I, H), (I, H), (H, I))]
+    mx = {"down": (2,), "gate and up": (0, 1), "up": (1,)}[which]
+    proj = []
+    for i, w in enumerate(wf):
+        kw = KW if i in mx else dict(group_size=64, bits=4)
+        q = mq.quantize(w, **kw)
+        proj.append(nn.QuantizedSwitchLinear(q[0], q[1], None if i in mx else q[2], **kw))
+    x = _randn(g, T, H, dtype=torch.bfloat16)
+    idx, wts = mq.moe_route(_randn(g, T, E), k)[:2]
+    out = nn.SwitchGLU(*proj, fuse_gate_up=fuse)(x, idx, wts)
+    xe = x[:, None, None]
+    if fuse and T < 400 and which == "down":
+        a, b = proj[:2]
+        h = ops.gather_glu(xe, a.weight, a.scales, a.biases, b.weight, b.scales, b.biases,
+                           rhs_indices=idx, group_size=64, bits=4)
+    else:
+        h = ops.swiglu(proj[0](xe, idx), proj[1](xe, idx))
+    y = proj[2](h, idx)
+    assert torch.equal(out, mq.moe_combine(y.reshape(-1, H), None, wts, T, k))
