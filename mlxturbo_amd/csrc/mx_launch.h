@@ -46,15 +46,14 @@ inline bool mx_wide_fits(int64_t M, int64_t N, int64_t K) {
          M * ((K + 511) / 512) < ((int64_t)1 << 26) && M * N < ((int64_t)1 << 40);
 }
 
-// Tile height and K split of least modelled cost, fitted to K=5120 N=17408 and
-// K=17408 N=5120 at 24 to 4096 rows, splits 1 to 12:
+// Tile height and K split of least modelled cost, fitted to 20 to 2048 rows at
+// N x K = 5120 x 17408, 17408 x 5120 and 4096 x 4096, splits 1 to 12, weights from
+// memory (chosen tiles within 1%, QQ 2.5%, of the best measured, on average):
 //  * a round of a tile per CU takes c0 and t per step (two 64-row tiles of T side by
-//    side on a CU take as long as in turn); over many rounds power and the L2 hold
-//    every CU to tp per step;
-//  * K splits sum into float planes that a second kernel adds, 3 us and (8 S + 2)
-//    M N bytes at 4.5 (QQ: 7) TB/s.
-// c0, t, tp of 64 / 128 / 192 rows: T 5 us, 0.77 / 1.25 / 1.55 and 1.1 / 1.9 / 2.1 us
-// per 128 codes; QQ 4.5, 1.45 / 1.9 / 2.2 and 1.9 / 2.15 / 3.3 per 512.
+//    side on a CU take as long as in turn), in more than one round at least tp per
+//    step and tile of a CU;
+//  * K splits sum into float planes that a second kernel adds, c1 and (8 S + 2) M N
+//    bytes at bw.
 struct MxWidePlan {
   int bm = 192, splits = 1;
   double cost_us = 0.0;
@@ -63,9 +62,9 @@ struct MxWidePlan {
 inline MxWidePlan mx_wide_plan(int64_t M, int64_t N, int64_t K, bool qq, int cus,
                                int max_splits = 16) {
   const int bms[3] = {192, 128, 64};
-  const double us[2][3] = {{1.55, 1.25, 0.77}, {2.2, 1.9, 1.45}};
-  const double held[2][3] = {{2.1, 1.9, 1.1}, {3.3, 2.15, 1.9}};
-  const double c0 = qq ? 4.5 : 5.0, bw = qq ? 7.0e6 : 4.5e6;
+  const double us[2][3] = {{1.62, 1.3, 0.8}, {2.4, 2.1, 1.53}};   // t: of 128, QQ 512 codes
+  const double held[2][3] = {{1.94, 1.04, 0.81}, {3.7, 2.06, 2.33}};     // tp
+  const double c0 = qq ? 4.8 : 3.1, c1 = qq ? 4.0 : 2.7, bw = qq ? 5.5e6 : 5.2e6;
   const int64_t nk = qq ? (K + 511) / 512 : (K + 127) / 128, cols = (N + 255) / 256;
   const int64_t unit = qq || K % 512 ? 1 : 4;   // steps that a split takes or leaves
   MxWidePlan best;
@@ -77,8 +76,8 @@ inline MxWidePlan mx_wide_plan(int64_t M, int64_t N, int64_t K, bool qq, int cus
       const double round = c0 + us[qq][i] * (double)steps;
       double cost = (double)((tiles + cus - 1) / cus) * round;
       const double many = c0 + (double)tiles / cus * held[qq][i] * (double)steps;
-      if (many > cost) cost = many;
-      if (sp > 1) cost += 3.0 + (8.0 * sp + 2.0) * (double)M * (double)N / bw;
+      if (tiles > cus && many > cost) cost = many;
+      if (sp > 1) cost += c1 + (8.0 * sp + 2.0) * (double)M * (double)N / bw;
       if (best.cost_us == 0.0 || cost < best.cost_us) {
         best.bm = bms[i];
         best.splits = sp;
