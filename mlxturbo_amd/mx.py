@@ -127,26 +127,36 @@ def _composed(x, w, scales, transpose: bool) -> torch.Tensor:
 # A call's launches follow each other on the stream, as they share its workspace of
 # these operators with the calls of other threads there.
 _LAUNCH = threading.Lock()
+_SCRATCH: dict = {}
 
 
-def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
+def _scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """A workspace: the stream's, or in a capture one of the graph's own memory
     (graphs captured on one stream may be replayed on two at once)."""
-    if ops._capturing():
+    if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return ops._workspace(dev, nbytes, "mxfp4")
+    buf = _SCRATCH.get((dev.index, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
+        _SCRATCH[dev.index, stream] = buf
+    return buf
+
+
+def _launch(call, args, out, nbytes: int) -> int:
+    """One call with a workspace of nbytes where it needs one; its status."""
+    stream = ops._stream_ptr(out)
+    if not nbytes:
+        return call(*args, None, 0, stream)
+    with _LAUNCH:
+        ws = _scratch(out.device, stream, nbytes)
+        return call(*args, ws.data_ptr(), ws.numel(), stream)
 
 
 def _product(call, size, x, w, s, out, M: int, N: int, K: int) -> int:
-    """One product call, with a workspace where it needs one; its status."""
-    args = (x.data_ptr(), w.data_ptr(), s.data_ptr(), out.data_ptr(), M, N, K,
-            ops._DTYPE_CODE[out.dtype])
-    nbytes = int(size(M, N, K)) if M > 16 else 0     # up to 16 rows use none
-    if not nbytes:
-        return call(*args, None, 0, ops._stream_ptr(out))
-    with _LAUNCH:
-        ws = _scratch(out.device, nbytes)
-        return call(*args, ws.data_ptr(), ws.numel(), ops._stream_ptr(out))
+    """One product call; its status."""
+    return _launch(call, (x.data_ptr(), w.data_ptr(), s.data_ptr(), out.data_ptr(), M, N, K,
+                          ops._DTYPE_CODE[out.dtype]), out,
+                   size(M, N, K) if M > 16 else 0)   # up to 16 rows use none
 
 
 def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
@@ -225,13 +235,8 @@ def _gather_launch(x, flat, lhs, rhs, out, P, B, M, N, K, E, group_size, bits,
     lib = _lib.lib()
     args = (x_.data_ptr(), w_.data_ptr(), s_.data_ptr(), ops._ptr(lhs), rhs.data_ptr(),
             out.data_ptr(), P, B, M, N, K, E, ops._DTYPE_CODE[x.dtype])
-    nbytes = int(lib.mq_mxfp4_gather_qmm_workspace_size(P, M))
-    if not nbytes:
-        rc = lib.mq_mxfp4_gather_qmm(*args, None, 0, ops._stream_ptr(out))
-    else:
-        with _LAUNCH:
-            ws = _scratch(out.device, nbytes)
-            rc = lib.mq_mxfp4_gather_qmm(*args, ws.data_ptr(), ws.numel(), ops._stream_ptr(out))
+    rc = _launch(lib.mq_mxfp4_gather_qmm, args, out,
+                 lib.mq_mxfp4_gather_qmm_workspace_size(P, M))
     _lib.check(rc, "gather_qmm")
 
 

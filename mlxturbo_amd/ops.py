@@ -433,16 +433,16 @@ def _dev_index(dev: torch.device) -> int:
     return torch.cuda.current_device() if dev.type == "cuda" else 0
 
 
-def _workspace(dev: torch.device, nbytes: int, use: str = "") -> torch.Tensor:
+def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
     """The gather workspace of the current stream (kernels on one stream run
     in order, so consecutive calls can share it; calls on other streams get
     their own, as concurrent calls must not share one).  A buffer outgrown
     after a graph capture is kept alive (captured kernels may use it).  The
     capture check runs on every call, cache hits included: a capture that
     only ever found the buffer cached (warm-up on the capture stream, then
-    capture) still pins it.  ``use`` names a buffer of its own."""
+    capture) still pins it."""
     _capturing()
-    key = (dev.type, _dev_index(dev), _stream_of(dev)) + ((use,) if use else ())
+    key = (dev.type, _dev_index(dev), _stream_of(dev))
     buf = _WS_CACHE.get(key)
     if buf is None or buf.numel() < nbytes:
         if buf is not None:
