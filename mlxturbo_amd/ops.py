@@ -510,9 +510,7 @@ def _gather_pairs(dev, bx: tuple, bw: tuple, lhs_indices, rhs_indices):
         # the layers' call, tokens (T, 1) against experts (T, top_k): nothing to
         # broadcast (torch.broadcast_shapes alone takes as long as a launch)
         shape = tuple(rhs_indices.shape)
-        full = (1,) * (len(shape) - len(bx)) + bx
-        if (len(full) == len(shape) and _repeat_broadcast(bx, shape)
-                and all(b == s or b == 1 for b, s in zip(full, shape))):
+        if len(bx) <= len(shape) and _repeat_broadcast(bx, shape):
             P = math.prod(shape)
             return shape, P, None, rhs_indices.reshape(-1) if P else None
     lhs = None if lhs_indices is None else _as_index(lhs_indices, dev)
