@@ -45,17 +45,22 @@ def _check_quantized(weight: torch.Tensor, scales: torch.Tensor,
 
 
 class QuantizedLinear(torch.nn.Module):
-    """``mlx.nn.QuantizedLinear`` on MLX-format tensors (affine mode).
+    """``mlx.nn.QuantizedLinear`` on MLX-format tensors.
 
     Parameters are registered as buffers under MLX's names (``weight``,
     ``scales``, ``biases``, ``bias``) so weights loaded from an MLX checkpoint
     keep their keys.
+
+    ``dtype``: the float type that :meth:`dequantized_weight` gives in mode
+    mxfp4, whose scale bytes carry none (default: the bias's, else bfloat16;
+    conversions of the module change it as they do a float tensor's).  Affine
+    weights have that of their scales.
     """
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor,
                  biases: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None,
                  group_size: Optional[int] = None, bits: Optional[int] = None,
-                 mode: str = "affine"):
+                 mode: str = "affine", dtype: Optional[torch.dtype] = None):
         super().__init__()
         group_size, bits = ops._format(group_size, bits, mode)
         self.input_dims = _check_quantized(weight, scales, biases, group_size, bits, mode)
@@ -67,6 +72,15 @@ class QuantizedLinear(torch.nn.Module):
         self.register_buffer("scales", scales)
         self.register_buffer("biases", biases)
         self.register_buffer("bias", bias)
+        if mode == "mxfp4":
+            if dtype is None:
+                dtype = (bias.dtype if bias is not None and bias.dtype in ops._DTYPE_CODE
+                         else torch.bfloat16)
+            # an empty tensor of the type, so that .half() and .to() change it
+            self.register_buffer("_like", torch.empty(0, dtype=dtype, device=weight.device),
+                                 persistent=False)
+        elif dtype not in (None, scales.dtype):
+            raise ValueError(f"affine weights have their scales' dtype {scales.dtype}, not {dtype}")
 
     def prepared_weights(self) -> Optional["ops.PreparedWeights"]:
         """The layer's weights validated once (:class:`ops.PreparedWeights`),
@@ -112,13 +126,14 @@ class QuantizedLinear(torch.nn.Module):
         the weight's dtype (mxfp4: scales are bytes, no biases)."""
         group_size, bits = ops._format(group_size, bits, mode)
         wq, s, *b = ops.quantize(weight, group_size=group_size, bits=bits, mode=mode)
+        kw = {} if b else {"dtype": weight.dtype}
         return cls(wq, s, b[0] if b else None, bias=bias, group_size=group_size, bits=bits,
-                   mode=mode)
+                   mode=mode, **kw)
 
     def dequantized_weight(self) -> torch.Tensor:
         """The layer's weight as ``mx.dequantize`` gives it, ``[N, K]``."""
         return ops.dequantize(self.weight, self.scales, self.biases, self.group_size, self.bits,
-                              self.mode)
+                              self.mode, self._like.dtype if self.mode == "mxfp4" else None)
 
     def extra_repr(self) -> str:
         return (f"input_dims={self.input_dims}, output_dims={self.output_dims}, "
@@ -132,10 +147,10 @@ class QQLinear(QuantizedLinear):
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor,
                  biases: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                  group_size: Optional[int] = None, bits: Optional[int] = None,
-                 mode: str = "mxfp4"):
+                 mode: str = "mxfp4", dtype: Optional[torch.dtype] = None):
         if mode != "mxfp4":
             raise NotImplementedError(f"mode={mode!r}: QQLinear is mxfp4 on this path")
-        super().__init__(weight, scales, biases, bias, group_size, bits, mode)
+        super().__init__(weight, scales, biases, bias, group_size, bits, mode, dtype)
 
     def quantized_forward(self, x: torch.Tensor) -> torch.Tensor:
         out = ops.qqmm(x, self.weight, self.scales, self.group_size, self.bits, self.mode)
