@@ -268,8 +268,8 @@ def gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose: bool,
     if w.ndim != 3:
         w, scales = w.reshape(E, *w.shape[-2:]), scales.reshape(E, *scales.shape[-2:])
     bank = [w, scales]
-    composed = not transpose or x.dtype == torch.float32
-    if not composed and M <= 16 and (
+    kernels = transpose and x.dtype != torch.float32
+    if kernels and M <= 16 and (
             E <= ops._GATHER_PREP_MAX_E
             or not _lib.lib().mq_mxfp4_gather_qmm_workspace_size(P, M)):
         try:
@@ -277,12 +277,13 @@ def gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose: bool,
                            sorted_indices)
             return out
         except NotImplementedError:                  # beyond the kernels' address ranges
-            composed = True
+            kernels = False
     a = dict(x=x.reshape(B, M, K), flat=bank, lhs=lhs, rhs=rhs, P=P, B=B, M=M, N=N, K=K, E=E,
              dev=dev, transpose=transpose, shape=shape, dtype=x.dtype, launch=_gather_launch)
-    if composed:
-        return ops._gather_composed(
-            a, out, lambda e: dequantize(w[e], scales[e], dtype=x.dtype))
-    if M > 16:
-        return ops._gather_rows(a, out, GROUP_SIZE, BITS, sorted_indices)
-    return ops._gather_slices(a, out, GROUP_SIZE, BITS, sorted_indices)
+    if kernels:
+        form = ops._gather_rows if M > 16 else ops._gather_slices
+        try:
+            return form(a, out, GROUP_SIZE, BITS, sorted_indices)
+        except NotImplementedError:                  # the same
+            pass
+    return ops._gather_composed(a, out, lambda e: dequantize(w[e], scales[e], dtype=x.dtype))

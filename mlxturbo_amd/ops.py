@@ -726,7 +726,8 @@ def _lhs_table(P: int, B: int, dev) -> torch.Tensor:
 def _gather_rows(a, out, group_size, bits, sorted_indices) -> torch.Tensor:
     """More than 16 rows per pair: row m of pair p is the one-row pair
     (lhs[p] * M + m, rhs[p]) of x viewed as B*M one-row batches, so the call
-    is one gather of P*M one-row pairs (prefill-sized, the grouped kernel)."""
+    is one gather of P*M one-row pairs (prefill-sized, the grouped kernel), or
+    of as many slices as the experts need."""
     P, B, M, N, K = a["P"], a["B"], a["M"], a["N"], a["K"]
     dev = a["dev"]
     rows = torch.arange(M, device=dev, dtype=torch.int32)
@@ -734,8 +735,13 @@ def _gather_rows(a, out, group_size, bits, sorted_indices) -> torch.Tensor:
     lhs1 = (lhs[:, None] * M + rows[None, :]).reshape(-1).contiguous()
     rhs1 = a["rhs"][:, None].expand(P, M).reshape(-1).contiguous()
     o = out.reshape(P * M, 1, N)
-    a.get("launch", _gather_launch)(a["x"].reshape(B * M, 1, K), a["flat"], lhs1, rhs1, o, P * M,
-                                    B * M, 1, N, K, a["E"], group_size, bits, sorted_indices)
+    x1 = a["x"].reshape(B * M, 1, K)
+    if P * M > _GATHER_FUSED_MAX_P and a["E"] > _GATHER_PREP_MAX_E:
+        _gather_slices(dict(a, x=x1, lhs=lhs1, rhs=rhs1, P=P * M, B=B * M, M=1, shape=(P * M,)),
+                       o, group_size, bits, sorted_indices)
+        return out
+    a.get("launch", _gather_launch)(x1, a["flat"], lhs1, rhs1, o, P * M, B * M, 1, N, K, a["E"],
+                                    group_size, bits, sorted_indices)
     return out
 
 

@@ -69,3 +69,61 @@ def test_the_float_type_of_a_layer():
         assert set(lin.state_dict()) == {"weight", "scales"}
         f = cls.from_linear(_randn(g, 48, 64, dtype=torch.float16), **KW)
         assert f.dequantized_weight().dtype == torch.float16
+
+
+# ---- gather_qmm's other forms ----------------------------------------------------
+
+@pytest.mark.parametrize("mode", ["affine", "mxfp4"])
+def test_many_experts_and_many_rows(mode):
+    """More experts than the pair tables hold and more than 16 rows per pair."""
+    g = _gen(3)
+    E, N, K, M, P = 2050, 16, 64, 20, 20
+    q = mq.quantize(_randn(g, E, N, K, dtype=torch.bfloat16), mode=mode)
+    x = _randn(g, P, M, K, dtype=torch.bfloat16)
+    rhs = torch.randint(0, E, (P,), generator=g, device="cuda")
+    rhs[:3] = torch.tensor([E - 1, 2048, E], device="cuda")
+    out = mq.gather_qmm(x, *q[:2], *q[2:], rhs_indices=rhs, mode=mode)
+    assert not out[2].any()
+    for p in range(P):
+        if p != 2:
+            e = int(rhs[p])
+            v = mq.dequantize(*(t[e] for t in q), mode=mode).double()
+            _check(out[p], x[p], v, torch.bfloat16)
+
+
+def test_many_rows_of_long_weights():
+    """More than 16 rows per pair and K beyond the few-pairs kernel."""
+    g = _gen(4)
+    E, N, K, M = 2, 8, 32 * 9216, 20
+    w, s, v = weights(g, E, N, K)
+    x = _randn(g, 3, M, K, dtype=torch.bfloat16)
+    out = mq.gather_qmm(x, w, s, rhs_indices=torch.tensor([1, 0, 2], device="cuda"), **KW)
+    _check(out[0], x[0], v[1], torch.bfloat16)
+    _check(out[1], x[1], v[0], torch.bfloat16)
+    assert not out[2].any()
+
+
+def test_many_experts_beyond_the_kernels_ranges():
+    """More experts than the pair tables hold, with x of 2 GB and more and K beyond
+    the few-pairs kernel: nothing but the composed form takes it."""
+    g = _gen(5)
+    E, N, K, P = 2050, 1, 32 * 9216, 300
+    B = (1 << 31) // (2 * K) + 1
+    w = torch.zeros(E, N, K // 8, dtype=torch.int32, device="cuda")
+    s = torch.full((E, N, K // 32), 127, dtype=torch.uint8, device="cuda")
+    w1, s1, v1 = weights(g, 1, K)
+    for e in (7, E - 1):
+        w[e], s[e] = w1.view(torch.int32), s1
+    x = torch.zeros(B, 1, K, dtype=torch.bfloat16, device="cuda")
+    x[B - 1, 0] = _randn(g, K, dtype=torch.bfloat16)
+    lhs = torch.full((P,), B - 1, dtype=torch.int32, device="cuda")
+    lhs[1] = 0
+    rhs = torch.arange(P, dtype=torch.int32, device="cuda")
+    rhs[P - 1] = E - 1
+    out = mq.gather_qmm(x, w.view(torch.uint32), s, lhs_indices=lhs, rhs_indices=rhs,
+                        **KW).reshape(P)
+    hit = torch.zeros(P, dtype=torch.bool, device="cuda")
+    hit[7] = hit[P - 1] = True
+    assert not out[~hit].any()
+    _check(out[7].reshape(1, 1), x[B - 1], v1, torch.bfloat16)
+    _check(out[P - 1].reshape(1, 1), x[B - 1], v1, torch.bfloat16)
