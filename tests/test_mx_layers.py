@@ -48,3 +48,21 @@ def test_affine_layers_have_their_scales_type():
     assert nn.QuantizedLinear(w, s, s, dtype=torch.float16).mode == "affine"
     with pytest.raises(ValueError, match="scales' dtype"):
         nn.QuantizedLinear(w, s, s, dtype=torch.bfloat16)
+
+
+def test_requantize_takes_the_modes_own_group_size(monkeypatch):
+    seen = []
+    monkeypatch.setattr(nn.QuantizedLinear, "from_linear",
+                        classmethod(lambda cls, w, bias=None, **kw: seen.append(kw)))
+    lin = torch.nn.Linear(96, 8, bias=False)
+    rebit.requantize(lin, 4, mode="mxfp4")               # 96 is groups of 32 alone
+    rebit.requantize(torch.nn.Linear(128, 8), 8)
+    rebit.requantize(lin, 8, 32)
+    assert seen == [dict(group_size=32, bits=4, mode="mxfp4"),
+                    dict(group_size=64, bits=8, mode="affine"),
+                    dict(group_size=32, bits=8, mode="affine")]
+    with pytest.raises(ValueError, match="multiple of group_size=64"):
+        rebit.requantize(lin, 8)
+    for bad in (dict(bits=4, group_size=64), dict(bits=8)):
+        with pytest.raises(ValueError, match="groups of 32"):
+            rebit.requantize(lin, mode="mxfp4", **bad)
