@@ -10,7 +10,8 @@ bits first) and one E8M0 scale byte per group; no biases.  A value is
   holds a NaN or an infinity gets ``e = 255`` and zero codes.
 * products: float sums over ``T(code * 2**(e - 127))`` with T the activations'
   type, what :func:`ops.dequantize` gives, rounded once to T.  In float16 a
-  scale beyond 2**13 overflows as its dequantized values do.
+  scale beyond 2**13 overflows as its dequantized values do.  qqmm multiplies
+  codes and scales as they are, with no rounding to T before the sums.
 
 The operators of :mod:`mlxturbo_amd.ops` call these for the mode; arguments and
 errors are theirs.
@@ -221,7 +222,9 @@ def qqmm(x, w, scales) -> torch.Tensor:
         rc = _product(lib.mq_mxfp4_qqmm, lib.mq_mxfp4_qqmm_workspace_size, x_, w_, s_, out, M, N,
                       K)
     if rc == ops._EUNSUPPORTED:
-        return _composed(dequantize(*quantize(x), dtype=x.dtype), w, scales, True)
+        # in float, which holds what both sides' codes and scales stand for
+        return _composed(dequantize(*quantize(x), dtype=torch.float32), w, scales,
+                         True).to(x.dtype)
     _lib.check(rc, "qqmm")
     return out
 

@@ -320,9 +320,9 @@ def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
          mode: str = "mxfp4") -> torch.Tensor:
     """``mx.qqmm``: ``x`` is quantized along its last axis in the weight's
     format and multiplied there, ``dequantize(quantize(x)) @ dequantize(w).T``
-    with float sums, rounded once to x's dtype.  ``w`` ``[N, K/8]`` and
-    ``scales`` ``[N, K/32]`` are :func:`quantize`'s.  Both operands enter the
-    MFMAs as codes with their scales; the mode is mxfp4."""
+    with float sums over the exact values, rounded once to x's dtype.  ``w``
+    ``[N, K/8]`` and ``scales`` ``[N, K/32]`` are :func:`quantize`'s.  Both
+    operands enter the MFMAs as codes with their scales; the mode is mxfp4."""
     _format(group_size, bits, mode)
     if mode != "mxfp4":
         raise NotImplementedError(f"mode={mode!r}: qqmm is mxfp4 on this path")

@@ -127,3 +127,25 @@ def test_many_experts_beyond_the_kernels_ranges():
     assert not out[~hit].any()
     _check(out[7].reshape(1, 1), x[B - 1], v1, torch.bfloat16)
     _check(out[P - 1].reshape(1, 1), x[B - 1], v1, torch.bfloat16)
+
+
+# ---- qqmm -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M", [3, 20])
+def test_qqmm_of_long_rows_at_far_scales(M):
+    """float16 x, weights beyond half's range: exact codes at every K, also where K
+    is beyond the few-rows kernel (3 rows are composed).  Every product is a whole
+    number of halves and their magnitudes sum to less than 2^23, so the float sums
+    are exact in any order and the outputs match bit for bit."""
+    g = _gen(7)
+    N, K = 8, 32 * 9216
+    code = torch.randint(0, 16, (N, K), generator=g, device="cuda")
+    e = torch.randint(144, 146, (N, K // 32), generator=g, device="cuda")
+    v = values_ref(code, e)
+    assert float(v.abs().max()) > torch.finfo(torch.float16).max
+    x = (torch.randint(-1, 2, (M, K), generator=g, device="cuda") * 2.0 ** -17).half()
+    assert torch.equal(values_ref(*quantize_ref(x)), x.double())
+    assert bool((x.double().abs() @ v.abs().T.contiguous() < 2 ** 23).all())
+    y = x.double() @ v.T.contiguous()
+    out = mq.qqmm(x, pack(code), e.to(torch.uint8))
+    assert torch.equal(out, y.float().half())
