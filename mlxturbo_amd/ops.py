@@ -731,7 +731,11 @@ def _gather_rows(a, out, group_size, bits, sorted_indices) -> torch.Tensor:
     P, B, M, N, K = a["P"], a["B"], a["M"], a["N"], a["K"]
     dev = a["dev"]
     rows = torch.arange(M, device=dev, dtype=torch.int32)
-    lhs = a["lhs"] if a["lhs"] is not None else _lhs_table(P, B, dev)
+    if a["lhs"] is None:
+        lhs = _lhs_table(P, B, dev)
+    else:
+        # batches that do not exist: times M they could wrap into ones that do
+        lhs = torch.where((a["lhs"] >= 0) & (a["lhs"] < B), a["lhs"], -1)
     lhs1 = (lhs[:, None] * M + rows[None, :]).reshape(-1).contiguous()
     rhs1 = a["rhs"][:, None].expand(P, M).reshape(-1).contiguous()
     o = out.reshape(P * M, 1, N)

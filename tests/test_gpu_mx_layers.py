@@ -149,3 +149,19 @@ def test_qqmm_of_long_rows_at_far_scales(M):
     y = x.double() @ v.T.contiguous()
     out = mq.qqmm(x, pack(code), e.to(torch.uint8))
     assert torch.equal(out, y.float().half())
+
+
+@pytest.mark.parametrize("mode", ["affine", "mxfp4"])
+def test_far_batch_indices_of_many_rows(mode):
+    """An x batch that does not exist gives zeros, however far off it is (times the
+    rows of a pair, these pass 32 bits)."""
+    g = _gen(6)
+    M, N, K = 20, 16, 64
+    q = mq.quantize(_randn(g, 3, N, K, dtype=torch.bfloat16), mode=mode)
+    x = _randn(g, 4, M, K, dtype=torch.bfloat16)
+    lhs = torch.tensor([3, 1 << 30, 2 ** 31 - 1, -(1 << 30), -(2 ** 31), 4, -1], device="cuda")
+    out = mq.gather_qmm(x, *q[:2], *q[2:], lhs_indices=lhs,
+                        rhs_indices=torch.ones(7, dtype=torch.int32, device="cuda"), mode=mode)
+    v = mq.dequantize(*(t[1] for t in q), mode=mode).double()
+    _check(out[0], x[3], v, torch.bfloat16)
+    assert not out[1:].any()
