@@ -667,7 +667,7 @@ def gather_swiglu(x: torch.Tensor, gate, up, rhs_indices: torch.Tensor,
     """A prefill MoE layer's gate and up projections and its activation:
     ``swiglu(gather_qmm(x, *gate, rhs_indices=rhs_indices, tables=tables),
     gather_qmm(x, *up, ...))``, bit for bit, in one launch over the layer's
-    tables where the tables' kernel takes the call
+    tables where there are any and the tables' kernel takes the call
     (mq_gather_swiglu_tables: each gathered x tile is read once for both
     banks), else as those three calls.  ``gate`` and ``up`` are
     ``(w, scales, biases)`` banks of one shape; x reaches pair p through
@@ -683,7 +683,7 @@ def gather_swiglu(x: torch.Tensor, gate, up, rhs_indices: torch.Tensor,
                           bits, mode)
     if a is None:
         return out
-    if (a["route"] == "kernel" and a["lhs"] is None
+    if (tables is not None and a["route"] == "kernel" and a["lhs"] is None
             and (tables.P, tables.M, tables.E) == (a["P"], a["M"], a["E"])):
         x_ = _aligned(a["x"])
         rc = _lib.lib().mq_gather_swiglu_tables(

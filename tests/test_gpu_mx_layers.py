@@ -165,3 +165,21 @@ def test_far_batch_indices_of_many_rows(mode):
     v = mq.dequantize(*(t[1] for t in q), mode=mode).double()
     _check(out[0], x[3], v, torch.bfloat16)
     assert not out[1:].any()
+
+
+# ---- the mixture-of-experts operators ----------------------------------------------
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_gather_swiglu_without_tables(T):
+    g = _gen(T)
+    E, k, H, I = 12, 8, 128, 64
+    gate, up = (mq.quantize(_randn(g, E, I, H, dtype=torch.bfloat16)) for _ in range(2))
+    x = _randn(g, T, 1, 1, H, dtype=torch.bfloat16)
+    idx = torch.randint(0, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    out = ops.gather_swiglu(x, gate, up, idx, None)
+    want = ops.swiglu(mq.gather_qmm(x, *gate, rhs_indices=idx),
+                      mq.gather_qmm(x, *up, rhs_indices=idx))
+    assert torch.equal(out, want)
+    tables = ops.gather_tables(idx, E)
+    if tables is not None:
+        assert torch.equal(ops.gather_swiglu(x, gate, up, idx, tables), want)
