@@ -531,6 +531,12 @@ def _gather_pairs(dev, bx: tuple, bw: tuple, lhs_indices, rhs_indices):
     return shape, P, lhs_f, rhs_f
 
 
+def _same_banks(w: torch.Tensor, other: torch.Tensor) -> None:
+    if w.shape != other.shape:
+        raise ValueError(f"expert banks differ in shape: {tuple(w.shape)} and "
+                         f"{tuple(other.shape)}")
+
+
 def _gather_prep(x, banks, lhs_indices, rhs_indices, transpose, group_size, bits, mode,
                  alloc=True):
     """Validation and flattening shared by gather_qmm and gather_glu; ``banks``
@@ -547,8 +553,7 @@ def _gather_prep(x, banks, lhs_indices, rhs_indices, transpose, group_size, bits
     if x.ndim < 2 or w0.ndim < 3:
         raise ValueError("gather_qmm needs x (..., M, K) and w (..., N, K*bits/32) with a batch dim")
     for w, s, b in banks:
-        if w.shape != w0.shape:
-            raise ValueError(f"expert banks differ in shape: {tuple(w.shape)} and {tuple(w0.shape)}")
+        _same_banks(w, w0)
         Kq = _check_quant(w, s, b, group_size, bits)
         if s.dtype != banks[0][1].dtype:
             raise ValueError("expert banks differ in scale dtype")
@@ -677,6 +682,7 @@ def gather_swiglu(x: torch.Tensor, gate, up, rhs_indices: torch.Tensor,
     calls."""
     group_size, bits = _format(group_size, bits, mode)
     if mode == "mxfp4":
+        _same_banks(gate[0], up[0])
         kw = dict(rhs_indices=rhs_indices, transpose=transpose, mode=mode)
         return swiglu(gather_qmm(x, *gate, **kw), gather_qmm(x, *up, **kw))
     out, a = _gather_prep(x, [tuple(gate), tuple(up)], None, rhs_indices, transpose, group_size,
@@ -864,7 +870,9 @@ def gather_glu(x: torch.Tensor, gate_w: torch.Tensor, gate_scales: torch.Tensor,
     path outside decode widths (fused.py:2476-2479)."""
     group_size, bits = _format(group_size, bits, mode)
     a = None
-    if mode != "mxfp4":
+    if mode == "mxfp4":
+        _same_banks(gate_w, up_w)
+    else:
         out, a = _gather_prep(x, [(gate_w, gate_scales, gate_biases),
                                   (up_w, up_scales, up_biases)],
                               lhs_indices, rhs_indices, transpose, group_size, bits, mode)

@@ -66,3 +66,17 @@ def test_requantize_takes_the_modes_own_group_size(monkeypatch):
     for bad in (dict(bits=4, group_size=64), dict(bits=8)):
         with pytest.raises(ValueError, match="groups of 32"):
             rebit.requantize(lin, mode="mxfp4", **bad)
+
+
+@pytest.mark.parametrize("E,N", [(3, 1), (2, 48), (1, 48)])
+def test_gate_and_up_banks_of_other_shapes_are_refused(on_cpu, E, N):
+    gate, up = (*_w(E=3), None), (*_w(E=E, N=N), None)
+    x = torch.zeros(4, 1, 1, 256, dtype=torch.bfloat16)
+    idx = torch.zeros(4, 2, dtype=torch.int32)
+    wts = torch.zeros(4, 2)
+    with pytest.raises(ValueError, match="banks differ in shape"):
+        mq.gather_glu(x, *gate, *up, rhs_indices=idx, **KW)
+    with pytest.raises(ValueError, match="banks differ in shape"):
+        ops.gather_swiglu(x, gate, up, idx, None, **KW)
+    with pytest.raises(ValueError, match="banks differ in shape"):
+        ops.moe_layer(x.reshape(4, 256), idx, wts, gate, up, (*_w(E=3, N=256, K=64), None), **KW)
