@@ -183,3 +183,31 @@ def test_gather_swiglu_without_tables(T):
     tables = ops.gather_tables(idx, E)
     if tables is not None:
         assert torch.equal(ops.gather_swiglu(x, gate, up, idx, tables), want)
+
+
+@pytest.mark.parametrize("T", [1, 5, 12, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_moe_operators(T, dtype):
+    """gather_swiglu, gather_glu, gather_qmm_combine and moe_layer are their steps,
+    bit for bit."""
+    g = _gen(T + 40)
+    E, k, H, I = 10, 4, 192, 96
+    gate, up, down = ((*weights(g, E, *s)[:2], None) for s in ((I, H), (I, H), (H, I)))
+    x = _randn(g, T, H, dtype=dtype) * 4
+    idx, wts = mq.moe_route(_randn(g, T, E), k)[:2]
+    xe = x[:, None, None]
+    a, b = (mq.gather_qmm(xe, *bank, rhs_indices=idx, **KW) for bank in (gate, up))
+    assert torch.equal(ops.gather_swiglu(xe, gate, up, idx, None, **KW), ops.swiglu(a, b))
+    h = ops.gather_glu(xe, *gate, *up, rhs_indices=idx, **KW)
+    assert torch.equal(h, (torch.nn.functional.silu(a.float()) * b.float()).to(dtype))
+    y = mq.gather_qmm(h, *down, rhs_indices=idx, **KW).reshape(T * k, H)
+    want = mq.moe_combine(y, None, wts, T, k)
+    assert want.shape == (T, H) and want.dtype == dtype
+    assert torch.equal(mq.gather_qmm_combine(h, *down, idx, wts, **KW), want)
+    assert torch.equal(ops.moe_layer(x, idx, wts, gate, up, down, **KW), want)
+    sgate = torch.rand((T, 1), generator=g, device="cuda").to(dtype)
+    shared = _randn(g, T, H, dtype=dtype)
+    out = mq.gather_qmm_combine(h, *down, idx, wts, sgate=sgate, shared=shared, **KW)
+    assert torch.equal(out, mq.moe_combine(y, None, wts, T, k, sgate, shared))
+    with pytest.raises(ValueError, match="together"):
+        mq.gather_qmm_combine(h, *down, idx, wts, sgate=sgate, **KW)
