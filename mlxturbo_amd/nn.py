@@ -44,7 +44,25 @@ def _check_quantized(weight: torch.Tensor, scales: torch.Tensor,
     return k
 
 
-class QuantizedLinear(torch.nn.Module):
+def _scale_bytes(scales: torch.Tensor, mode: str) -> torch.Tensor:
+    """mxfp4 scales as uint8: a float type's values, and not its bytes, go through
+    conversions and copies of a module's tensors."""
+    if mode == "mxfp4" and scales.dtype == torch.float8_e8m0fnu:
+        return scales.view(torch.uint8)
+    return scales
+
+
+class _Quantized(torch.nn.Module):
+    """Loads a state dict's scales as the layer holds them."""
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        s = state_dict.get(prefix + "scales")
+        if isinstance(s, torch.Tensor):
+            state_dict[prefix + "scales"] = _scale_bytes(s, self.mode)
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+
+
+class QuantizedLinear(_Quantized):
     """``mlx.nn.QuantizedLinear`` on MLX-format tensors.
 
     Parameters are registered as buffers under MLX's names (``weight``,
@@ -69,7 +87,7 @@ class QuantizedLinear(torch.nn.Module):
         self.bits = bits
         self.mode = mode
         self.register_buffer("weight", weight)
-        self.register_buffer("scales", scales)
+        self.register_buffer("scales", _scale_bytes(scales, mode))
         self.register_buffer("biases", biases)
         self.register_buffer("bias", bias)
         if mode == "mxfp4":
@@ -166,7 +184,7 @@ class QQLinear(QuantizedLinear):
         return super().from_linear(weight, bias, group_size, bits, mode)
 
 
-class QuantizedSwitchLinear(torch.nn.Module):
+class QuantizedSwitchLinear(_Quantized):
     """mlx-lm's ``QuantizedSwitchLinear``: an expert bank applied per index.
 
     ``forward(x, indices, sorted_indices=False)`` with ``x`` ``(..., M, K)``
@@ -188,7 +206,7 @@ class QuantizedSwitchLinear(torch.nn.Module):
         self.bits = bits
         self.mode = mode
         self.register_buffer("weight", weight)
-        self.register_buffer("scales", scales)
+        self.register_buffer("scales", _scale_bytes(scales, mode))
         self.register_buffer("biases", biases)
         self.register_buffer("bias", bias)
 

@@ -80,3 +80,26 @@ def test_gate_and_up_banks_of_other_shapes_are_refused(on_cpu, E, N):
         ops.gather_swiglu(x, gate, up, idx, None, **KW)
     with pytest.raises(ValueError, match="banks differ in shape"):
         ops.moe_layer(x.reshape(4, 256), idx, wts, gate, up, (*_w(E=3, N=256, K=64), None), **KW)
+
+
+@pytest.mark.parametrize("E", [None, 3])
+def test_layers_hold_scale_bytes(E):
+    """float8_e8m0fnu scales are the same bytes as uint8 ones, through the module's
+    conversions and state dicts of either type."""
+    cls = nn.QuantizedSwitchLinear if E else nn.QuantizedLinear
+    w, s = _w(E=E)
+    s = torch.randint(0, 256, s.shape, dtype=torch.uint8)
+    e8 = s.view(torch.float8_e8m0fnu)
+    lin = torch.nn.ModuleDict({"a": cls(w, e8, None, **KW)})
+    assert torch.equal(lin["a"].scales, s)
+    assert torch.equal(lin.half()["a"].scales, s)
+    for assign in (False, True):
+        for given in (s, e8):
+            new = torch.nn.ModuleDict({"a": cls(w, torch.zeros_like(s), None, **KW)})
+            state = {"a.weight": w, "a.scales": given}
+            new.load_state_dict(state, assign=assign)
+            assert torch.equal(new["a"].scales, s) and state["a.scales"] is given
+    aff = nn.QuantizedLinear(torch.zeros(8, 32, dtype=torch.int32), *[torch.zeros(8, 4)] * 2)
+    aff.load_state_dict({"weight": aff.weight, "scales": torch.ones(8, 4, dtype=torch.float16),
+                         "biases": torch.ones(8, 4)})
+    assert aff.scales.dtype == torch.float32 and bool((aff.scales == 1).all())
