@@ -18,7 +18,7 @@ tensor shapes disagree with the default bit width has its width inferred
 from the shapes (``weight_cols * 32 / (scales_cols * group_size)``).
 ``"mode": "mxfp4"`` layers have uint8 ``scales`` and no ``biases``, and the
 config's ``torch_dtype`` (or ``dtype``), where it names one, as their float type;
-an override in another width without a mode of its own is affine.
+a module in another width without a mode of its own is affine.
 
 Tensors are memory-mapped from the shards and copied to the device once;
 nothing is converted or repacked.
@@ -106,6 +106,8 @@ def quant_params(config: dict, prefix: str, weight_cols: int,
             raise ValueError(f"{prefix}: weight cols {weight_cols} and scales cols "
                              f"{scales_cols} fit no bit width at group_size {gs}")
         bits = num // den
+        if mode == "mxfp4":              # has one width
+            mode = "affine"
     return gs, bits, mode
 
 

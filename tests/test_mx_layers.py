@@ -103,3 +103,18 @@ def test_layers_hold_scale_bytes(E):
     aff.load_state_dict({"weight": aff.weight, "scales": torch.ones(8, 4, dtype=torch.float16),
                          "biases": torch.ones(8, 4)})
     assert aff.scales.dtype == torch.float32 and bool((aff.scales == 1).all())
+
+
+def test_checkpoint_width_from_the_shapes_is_affine(tmp_path):
+    """A module without an entry and of another width, in an MXFP4 checkpoint."""
+    from safetensors.torch import save_file
+    w, s = _w()
+    b16 = torch.zeros(48, 8, dtype=torch.bfloat16)
+    save_file({"a.weight": w.view(torch.uint32), "a.scales": s,
+               "h.weight": torch.zeros(48, 64, dtype=torch.int32).view(torch.uint32),
+               "h.scales": b16, "h.biases": b16.clone()}, str(tmp_path / "model.safetensors"))
+    (tmp_path / "config.json").write_text(json.dumps({"quantization": {"mode": "mxfp4"}}))
+    layers = checkpoint.quantized_layers(str(tmp_path), device="cpu")
+    assert layers["a"].mode == "mxfp4"
+    h = layers["h"]
+    assert (h.mode, h.bits, h.group_size, h.input_dims) == ("affine", 8, 32, 256)
