@@ -432,9 +432,9 @@ int mq_moe_route(const float* logits, int32_t* idx, float* weights, int64_t rows
                  void* hip_stream);
 
 /*
- * MXFP4 (OCP Microscaling formats v1.0; MLX's mode="mxfp4"): groups of 32
- * values along K share a power of two, 2^(e - 127) with e one byte (255: NaN);
- * a value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6, sign in bit 3) times it.
+ * MXFP4 (OCP Microscaling formats v1.0; the format of MLX's mode="mxfp4"):
+ * groups of 32 values along K share a power of two, 2^(e - 127) with e one byte
+ * (255: NaN); a value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6, sign in bit 3) times it.
  *   w       uint32 [N, K/8]   code j of word i = element 8 i + j at bit 4 j
  *   scales  uint8 [N, K/32]   no biases
  *   deq     T(code * 2^(e - 127)), rounded to nearest even
@@ -444,7 +444,8 @@ int mq_moe_route(const float* logits, int32_t* idx, float* weights, int64_t rows
  * reference's kernels; its layers pass `mode` through to stock MLX
  * (mlxturbo/kernels/dispatch.py:317-327).
  *
- * mq_mxfp4_quantize: w [N, K] of any of the three dtypes.  Per group, with max
+ * mq_mxfp4_quantize: w [N, K] of any of the three dtypes.  Per group, as the
+ * specification has it (MLX's own quantizer may choose other scales), with max
  * the largest magnitude: e = max(floor(log2(max)) - 2, -127) + 127, codes
  * rounded to nearest, ties to even, saturating at 6; a group that holds a NaN or
  * an infinity has e = 255 and zero codes.
@@ -470,9 +471,9 @@ int mq_mxfp4_matmul(const void* x, const uint32_t* w, const uint8_t* scales, voi
                     void* hip_stream);
 
 /*
- * mq_mxfp4_matmul with x quantized too: out = deq(q(x)) . deq(w)^T with q as
- * mq_mxfp4_quantize, both operands entering the MFMAs as codes and scales
- * (mx.qqmm, mode="mxfp4").  Without the workspace (x's codes, and K splits) the
+ * mq_mxfp4_matmul with x quantized too: out = q(x) . w^T with q as
+ * mq_mxfp4_quantize, both operands entering the MFMAs as codes and scales, with no
+ * rounding to T before the sums (mx.qqmm, mode="mxfp4").  Without the workspace (x's codes, and K splits) the
  * call runs at any size, slower above 16 rows.
  */
 size_t mq_mxfp4_qqmm_workspace_size(int64_t M, int64_t N, int64_t K);

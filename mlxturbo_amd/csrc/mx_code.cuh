@@ -18,9 +18,10 @@
 //    the other half has landed.  A round's scale bytes travel likewise.
 //  * What is not an MFMA is placed between them (sched_barrier).
 //
-// 4096 rows, N=17408 K=5120: 215 us, 3.4 PFLOP/s, at 2.0 GHz; a round takes 2.3 us
-// against 1.5 of MFMAs (without the loads of the loop 177 us, without the fragment
-// reads 200), a tile's start and stores about 12.
+// 4096 rows, N=17408 K=5120: 234 us in a row of calls, 3.1 PFLOP/s.  A launch by
+// itself, at 2.0 GHz, 215: a round takes 2.3 us against 1.5 of MFMAs (without the loads
+// of the loop 177 us, without the fragment reads 200), a tile's start and stores about
+// 12.
 //
 // Groups past K: zero codes of x (the quantizer's padding), scale bytes 0.
 #pragma once

@@ -6,8 +6,9 @@
 // scattered back to pair order.  Bound by the weights: experts with few rows
 // make a tile mostly weights, whole lines of 16 rows per two loads, four steps
 // ahead, two workgroups per CU; a tile is as tall as its rows need (16, 32 or
-// 64).  2408 pairs over 128 experts of N=768 K=2048: 31 us, 3.5 TB/s of weights;
-// 16384 over 512 of N=512 K=2048: 87 us, 3.3 TB/s.
+// 64).  2408 pairs over 128 experts of N=768 K=2048: 32 us, 3.4 TB/s of weights;
+// 16384 over 512 of N=512 K=2048: 91 us, 3.1 TB/s; K that is not whole 512s (N=2048
+// K=768, 2408 pairs over 128): 41 us, 2.6 TB/s.
 #pragma once
 #include "mx_tile.cuh"
 

@@ -47,7 +47,8 @@ inline bool mx_wide_fits(int64_t M, int64_t N, int64_t K) {
 }
 
 // Tile height and K split of least modelled cost, fitted to 20 to 2048 rows at
-// N x K = 5120 x 17408, 17408 x 5120 and 4096 x 4096, splits 1 to 12, weights from
+// N x K = 5120 x 17408, 17408 x 5120 and 4096 x 4096 (whole 512s; the same plan
+// serves other K, whose steps take somewhat longer), splits 1 to 12, weights from
 // memory (chosen tiles within 1%, QQ 2.5%, of the best measured, on average):
 //  * a round of a tile per CU takes c0 and t per step (two 64-row tiles of T side by
 //    side on a CU take as long as in turn), in more than one round at least tp per

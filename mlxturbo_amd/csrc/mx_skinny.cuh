@@ -29,10 +29,11 @@
 // chunks permuted (xswz) so that fragment reads hit distinct banks; the
 // fragments are read to registers before the next step's x replaces them.  The
 // tile's scale bytes are one contiguous block, copied to LDS first.  N=17408
-// K=5120, us at 8 rows, weights from memory: 16.7 (from the last-level cache 13.5).  Fragments straight from memory, 16 bytes of 64
-// different pieces per load, cost as much as the weights (18.4; 12.0 without
-// the loads of x); a second step in flight is slower (18.0), and so are
-// contiguous K slices per wave (17.5: a workgroup's waves then read far apart)
+// K=5120, us at 8 rows, weights from memory: 16.7 (on another card 16.0; partly from
+// the last-level cache 13.8), and as much at one row.  Fragments straight from
+// memory, 16 bytes of 64 different pieces per load, cost as much as the weights
+// (18.4; 12.0 without the loads of x); a second step in flight is slower (18.0), and
+// so are contiguous K slices per wave (17.5: a workgroup's waves then read far apart)
 // and 16 or 64 weight rows per wave (17.9, 18.7).
 //
 // Groups past K: zero codes (outside the buffer range), scale byte 0 and x from

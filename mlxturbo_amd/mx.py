@@ -1,9 +1,11 @@
 """The ``mode="mxfp4"`` side of :mod:`mlxturbo_amd.ops`.
 
-MXFP4 (OCP Microscaling formats v1.0; MLX's ``mode="mxfp4"``): groups of 32
-values along the last axis, 4-bit E2M1 codes packed eight to a uint32 word (low
-bits first) and one E8M0 scale byte per group; no biases.  A value is
-``code * 2**(e - 127)``, ``e == 255`` is NaN.
+MXFP4 (OCP Microscaling formats v1.0; the format of MLX's ``mode="mxfp4"``):
+groups of 32 values along the last axis, 4-bit E2M1 codes packed eight to a
+uint32 word (low bits first) and one E8M0 scale byte per group; no biases.  A
+value is ``code * 2**(e - 127)``, ``e == 255`` is NaN.  The quantizer's choice of
+a group's scale is the specification's; whether MLX's own takes the same byte for
+every group is not pinned by any test here.
 
 * quantize: ``e - 127 = floor(log2(max|w|)) - 2`` of the group, at least -127;
   codes are rounded to nearest, ties to even, and saturate at 6.  A group that

@@ -151,7 +151,8 @@ def quantize(w: torch.Tensor, group_size: Optional[int] = None, bits: Optional[i
     calls it when it requantizes a layer (mlxturbo/rebit.py:119) or builds
     test weights (kernels/moe_verify_gather.py:887).  One HIP kernel; the
     per-group arithmetic is the C ABI's ``mq_quantize``.  ``mode="mxfp4"``
-    returns ``(w_q, scales)``, the scales uint8 exponents (mq_mxfp4_quantize)."""
+    returns ``(w_q, scales)``, the scales uint8 exponents as the format's
+    specification chooses them (mq_mxfp4_quantize)."""
     group_size, bits = _format(group_size, bits, mode)
     if mode == "mxfp4":
         return _mx.quantize(w)
