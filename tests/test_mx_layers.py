@@ -118,3 +118,15 @@ def test_checkpoint_width_from_the_shapes_is_affine(tmp_path):
     assert layers["a"].mode == "mxfp4"
     h = layers["h"]
     assert (h.mode, h.bits, h.group_size, h.input_dims) == ("affine", 8, 32, 256)
+
+
+def test_checkpoint_bias_has_the_float_type(tmp_path):
+    from safetensors.torch import save_file
+    w, s = _w()
+    save_file({"a.weight": w.view(torch.uint32), "a.scales": s,
+               "a.bias": torch.zeros(48, dtype=torch.float16)},
+              str(tmp_path / "model.safetensors"))
+    cfg = {"quantization": {"mode": "mxfp4"}, "torch_dtype": "bfloat16"}
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    layers = checkpoint.quantized_layers(str(tmp_path), device="cpu")
+    assert layers["a"]._like.dtype == torch.float16
