@@ -17,7 +17,7 @@ rebit.py re-quantizes such classes in place).  A module with no entry whose
 tensor shapes disagree with the default bit width has its width inferred
 from the shapes (``weight_cols * 32 / (scales_cols * group_size)``).
 ``"mode": "mxfp4"`` layers have uint8 ``scales`` and no ``biases``; their float type
-is their ``bias``'s, or the config's ``torch_dtype`` (or ``dtype``) where it names
+is that of a 16-bit ``bias``, or the config's ``torch_dtype`` (or ``dtype``) where it names
 one; a module in another width without a mode of its own is affine.
 
 Tensors are memory-mapped from the shards and copied to the device once;
@@ -33,7 +33,7 @@ from typing import Dict, Iterable, Optional, Tuple, Union
 import torch
 from safetensors import safe_open
 
-from .nn import QuantizedLinear, QuantizedSwitchLinear
+from .nn import QuantizedLinear, QuantizedSwitchLinear, _model_type
 
 _BITS = (2, 3, 4, 5, 6, 8)
 _FLOATS = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32}
@@ -137,7 +137,7 @@ def quantized_layers(path: str, device: Union[str, torch.device] = "cuda",
         if w.dtype != torch.uint32:
             w = w.view(torch.uint32) if w.dtype == torch.int32 else w
         cls, kw = (QuantizedSwitchLinear if w.ndim == 3 else QuantizedLinear), {}
-        if mode == "mxfp4" and cls is QuantizedLinear and prefix + ".bias" not in t:
+        if mode == "mxfp4" and cls is QuantizedLinear and not _model_type(t.get(prefix + ".bias")):
             kw["dtype"] = _FLOATS.get(config.get("torch_dtype") or config.get("dtype"))
         layers[prefix] = cls(w, s, t.get(prefix + ".biases"), t.get(prefix + ".bias"),
                              group_size=gs, bits=bits, mode=mode, **kw)

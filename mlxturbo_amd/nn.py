@@ -52,6 +52,12 @@ def _scale_bytes(scales: torch.Tensor, mode: str) -> torch.Tensor:
     return scales
 
 
+def _model_type(bias: Optional[torch.Tensor]) -> bool:
+    """Whether a bias shows the model's type: some models keep float32 ones beside
+    16-bit weights."""
+    return bias is not None and bias.dtype in (torch.bfloat16, torch.float16)
+
+
 class _Quantized(torch.nn.Module):
     """Loads a state dict's scales as the layer holds them."""
 
@@ -70,9 +76,9 @@ class QuantizedLinear(_Quantized):
     keep their keys.
 
     ``dtype``: the float type that :meth:`dequantized_weight` gives in mode
-    mxfp4, whose scale bytes carry none (default: the bias's, else bfloat16;
-    conversions of the module change it as they do a float tensor's).  Affine
-    weights have that of their scales.
+    mxfp4, whose scale bytes carry none (default: that of a 16-bit bias, else
+    bfloat16; conversions of the module change it as they do a float tensor's).
+    Affine weights have that of their scales.
     """
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor,
@@ -92,8 +98,7 @@ class QuantizedLinear(_Quantized):
         self.register_buffer("bias", bias)
         if mode == "mxfp4":
             if dtype is None:
-                dtype = (bias.dtype if bias is not None and bias.dtype in ops._DTYPE_CODE
-                         else torch.bfloat16)
+                dtype = bias.dtype if _model_type(bias) else torch.bfloat16
             # an empty tensor of the type, so that .half() and .to() change it
             self.register_buffer("_like", torch.empty(0, dtype=dtype, device=weight.device),
                                  persistent=False)

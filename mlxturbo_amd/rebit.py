@@ -43,10 +43,10 @@ CLASS_PATTERNS: Dict[str, Tuple[str, ...]] = {
 def requantize(layer, bits: int, group_size: Optional[int] = None,
                mode: str = "affine") -> QuantizedLinear:
     """A new :class:`QuantizedLinear` holding ``layer``'s weight at ``bits`` /
-    ``group_size`` (the mode's own by default, 64 in affine): a quantized layer is dequantized first (double
-    quantization, as rebit.py:96-120 does); a ``torch.nn.Linear`` or any
-    module with a float ``weight`` is quantized directly.  ``bias`` is kept.
-    ``mode="mxfp4"`` takes 4 bits in groups of 32."""
+    ``group_size`` (the mode's own by default, 64 in affine): a quantized
+    layer is dequantized first (double quantization, as rebit.py:96-120 does);
+    a ``torch.nn.Linear`` or any module with a float ``weight`` is quantized
+    directly.  ``bias`` is kept.  ``mode="mxfp4"`` takes 4 bits in groups of 32."""
     group_size, bits = ops._format(group_size, bits, mode)
     if isinstance(layer, QuantizedLinear):
         # both steps in one pass over the codes where the kernel takes them

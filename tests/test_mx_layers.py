@@ -130,3 +130,16 @@ def test_checkpoint_bias_has_the_float_type(tmp_path):
     (tmp_path / "config.json").write_text(json.dumps(cfg))
     layers = checkpoint.quantized_layers(str(tmp_path), device="cpu")
     assert layers["a"]._like.dtype == torch.float16
+
+
+def test_a_float32_bias_does_not_set_the_float_type(tmp_path):
+    from safetensors.torch import save_file
+    w, s = _w()
+    bias = torch.zeros(48)
+    assert nn.QuantizedLinear(w, s, None, bias, **KW)._like.dtype == torch.bfloat16
+    save_file({"a.weight": w.view(torch.uint32), "a.scales": s, "a.bias": bias},
+              str(tmp_path / "model.safetensors"))
+    cfg = {"quantization": {"mode": "mxfp4"}, "torch_dtype": "float16"}
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    layers = checkpoint.quantized_layers(str(tmp_path), device="cpu")
+    assert layers["a"]._like.dtype == torch.float16
