@@ -494,6 +494,78 @@ int mq_mxfp4_gather_qmm(const void* x, const uint32_t* w, const uint8_t* scales,
                         int64_t P, int64_t B, int64_t M, int64_t N, int64_t K, int64_t E,
                         int dtype, void* workspace, size_t workspace_bytes, void* hip_stream);
 
+/*
+ * The first half of a dense gated feed-forward block, the dense form of
+ * mq_gather_glu: out[M, N] = act(x . deq(gate)^T) * (x . deq(up)^T) over two affine
+ * matrices of one format (4 or 8 bits, bf16 / fp16; deq as mq_dequantize).  Float
+ * sums, act in float (MQ_ACT_SILU: g / (1 + exp(-g)); MQ_ACT_GELU_TANH: 0.5 g (1 +
+ * tanh(sqrt(2 / pi) (g + 0.044715 g^3)))), one rounding.  gate_sums and up_sums
+ * (float [M, N], both or neither) also receive the two products, which the
+ * gradient needs.  workspace of mq_quantized_glu_workspace_size(M, N, K, group_size,
+ * bits) bytes, 16-byte aligned, may be NULL (then nothing splits K); calls sharing
+ * one must be ordered.  x and w 16-byte aligned; K < 2^28.
+ */
+enum { MQ_ACT_SILU = 0, MQ_ACT_GELU_TANH = 1 };
+size_t mq_quantized_glu_workspace_size(int64_t M, int64_t N, int64_t K, int group_size, int bits);
+int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_scales,
+                     const void* gate_biases, const uint32_t* up_w, const void* up_scales,
+                     const void* up_biases, void* out, float* gate_sums, float* up_sums, int64_t M,
+                     int64_t N, int64_t K, int group_size, int bits, int dtype, int activation,
+                     void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/*
+ * x's gradient through mq_quantized_matmul (the weights are constants): dx[M, K] =
+ * d[M, N] . deq(w), float sums, one rounding.  workspace of
+ * mq_quantized_matmul_grad_workspace_size(M, N, K, group_size, bits) bytes, 16-byte
+ * aligned; it may be NULL where N % 64 == 0 (then nothing splits N).  d and w
+ * 16-byte aligned.  MQ_EUNSUPPORTED: no columns, codes of 2^31 bytes and more, rows
+ * of d of 2^22 elements and more (padded to whole 64s), 2, 3, 5 and 6 bits, float32.
+ */
+size_t mq_quantized_matmul_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
+                                               int bits);
+int mq_quantized_matmul_grad(const void* d, const uint32_t* w, const void* scales,
+                             const void* biases, void* dx, int64_t M, int64_t N, int64_t K,
+                             int group_size, int bits, int dtype, void* workspace,
+                             size_t workspace_bytes, void* hip_stream);
+
+/*
+ * x's gradient through mq_quantized_glu: dx = dg . deq(gate) + du . deq(up) with dg =
+ * T(d u act'(g)) and du = T(d act(g)) of the forward's float sums g and u.  The workspace
+ * (mq_quantized_glu_grad_workspace_size bytes, 16-byte aligned) holds dg and du, so it
+ * is needed; MQ_EUNSUPPORTED as above (rows of 2 N elements here).
+ */
+size_t mq_quantized_glu_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
+                                            int bits);
+int mq_quantized_glu_grad(const void* d, const float* gate_sums, const float* up_sums,
+                          const uint32_t* gate_w, const void* gate_scales,
+                          const void* gate_biases, const uint32_t* up_w, const void* up_scales,
+                          const void* up_biases, void* dx, int64_t M, int64_t N, int64_t K,
+                          int group_size, int bits, int dtype, int activation, void* workspace,
+                          size_t workspace_bytes, void* hip_stream);
+
+/*
+ * A token for each row of logits [rows, vocabulary] (any of the three dtypes, rows
+ * row_stride elements apart) from a uniform number u[row] in [0, 1): int32 tokens and
+ * their float log probabilities among the kept words.  With w_i = exp((l_i - max) /
+ * temperature), and words in order of value (equal ones: the lower index first), kept are
+ *   top_k >= 1: the first top_k words (otherwise all),
+ *   top_p < 1: of those, the words before which the mass is less than top_p of theirs,
+ *   min_p: of those, the words with w_i >= min_p,
+ * always the first.  The token is the first word, in index order, up to which the kept
+ * mass is more than u times all of it.  temperature 0: the first word.  A NaN logit
+ * counts as -inf; a row of nothing else gives token -1 and -inf.  Masses are
+ * integers of 2^-44 (vocabularies over 2^18: of 2^62 / vocabulary, rounded to a power of
+ * two), so a result depends on its row alone.  A setting is an array of `rows` values, or
+ * NULL and one value for all.  workspace of mq_sample_workspace_size bytes, 16-byte
+ * aligned; calls sharing one must be ordered. 
+ */
+size_t mq_sample_workspace_size(int64_t rows, int64_t vocabulary);
+int mq_sample(const void* logits, int64_t row_stride, int64_t rows, int64_t vocabulary, int dtype,
+              const float* u, const float* temperature, float temperature_value,
+              const int32_t* top_k, int32_t top_k_value, const float* top_p, float top_p_value,
+              const float* min_p, float min_p_value, int32_t* tokens, float* logprobs,
+              void* workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,8 @@ hand-written HIP kernels behind a C ABI (``include/mlxturbo_amd.h``):
 * :func:`dequantize`       - bit-exact MLX affine dequantization (every width)
 * :func:`quantize`         - MLX affine quantization (``mx.quantize``)
 * :func:`qqmm`             - both operands quantized (MXFP4, ``mx.qqmm``)
+* :func:`quantized_glu`    - a dense gated feed-forward block's gate, up, activation
+  and product in one, with x's gradient
 * :func:`gather_glu`       - fused MoE gate+up+SiLU at decode widths
 * :func:`moe_combine`      - MoE unsort + router weight + top-k sum epilogue
   (optionally merging the shared expert)
@@ -15,6 +17,9 @@ hand-written HIP kernels behind a C ABI (``include/mlxturbo_amd.h``):
   (one kernel at decode widths)
 * :func:`moe_route`        - MoE top-k routing with softmax weights and the
   shared-expert gate
+
+* :func:`sample`           - a token for each row of logits: temperature, top-k, top-p,
+  min-p and a given uniform number
 
 ``mode="mxfp4"`` of quantize, dequantize, quantized_matmul and gather_qmm is the
 block-scaled 4-bit floating point format (:mod:`mlxturbo_amd.mx`).
@@ -29,13 +34,13 @@ layers to another width (dequantize + quantize on the GPU).
 
 from . import checkpoint, dispatch, nn, rebit
 from .ops import (dequantize, gather_glu, gather_qmm, gather_qmm_combine, launch_count,
-                  moe_combine, moe_route, qqmm, quantize, quantized_matmul, row_identity,
-                  set_row_identity)
+                  moe_combine, moe_route, qqmm, quantize, quantized_glu, quantized_matmul,
+                  row_identity, sample, set_row_identity)
 
 __version__ = "0.2.0"
 
 __all__ = ["checkpoint", "rebit", "dequantize", "dispatch", "gather_glu", "gather_qmm",
            "gather_qmm_combine", "launch_count",
            "moe_combine", "moe_route",
-           "nn", "qqmm", "quantize", "quantized_matmul", "row_identity", "set_row_identity",
+           "nn", "qqmm", "quantize", "quantized_glu", "quantized_matmul", "row_identity", "sample", "set_row_identity",
            "__version__"]

@@ -21,6 +21,9 @@ MQ_BFLOAT16 = 0
 MQ_FLOAT16 = 1
 MQ_FLOAT32 = 2
 
+MQ_ACT_SILU = 0
+MQ_ACT_GELU_TANH = 1
+
 # every symbol include/mlxturbo_amd.h declares
 EXPORTED = (
     "mq_version",
@@ -56,6 +59,14 @@ EXPORTED = (
     "mq_mxfp4_qqmm",
     "mq_mxfp4_gather_qmm_workspace_size",
     "mq_mxfp4_gather_qmm",
+    "mq_quantized_glu_workspace_size",
+    "mq_quantized_glu",
+    "mq_quantized_matmul_grad_workspace_size",
+    "mq_quantized_matmul_grad",
+    "mq_quantized_glu_grad_workspace_size",
+    "mq_quantized_glu_grad",
+    "mq_sample_workspace_size",
+    "mq_sample",
 )
 
 _lock = threading.Lock()
@@ -65,6 +76,8 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _sz = ctypes.c_size_t
+_f32 = ctypes.c_float
+_i32 = ctypes.c_int32
 
 
 class LibraryMissing(RuntimeError):
@@ -147,6 +160,19 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mq_mxfp4_gather_qmm_workspace_size.argtypes = [_i64, _i64]
     lib.mq_mxfp4_gather_qmm.restype = _int
     lib.mq_mxfp4_gather_qmm.argtypes = [_vp] * 6 + [_i64] * 6 + [_int, _vp, _sz, _vp]
+    for name in ("mq_quantized_glu", "mq_quantized_matmul_grad", "mq_quantized_glu_grad"):
+        size = getattr(lib, name + "_workspace_size")
+        size.restype = _sz
+        size.argtypes = [_i64] * 3 + [_int] * 2
+        getattr(lib, name).restype = _int
+    lib.mq_quantized_glu.argtypes = [_vp] * 10 + [_i64] * 3 + [_int] * 4 + [_vp, _sz, _vp]
+    lib.mq_quantized_matmul_grad.argtypes = [_vp] * 5 + [_i64] * 3 + [_int] * 3 + [_vp, _sz, _vp]
+    lib.mq_quantized_glu_grad.argtypes = [_vp] * 10 + [_i64] * 3 + [_int] * 4 + [_vp, _sz, _vp]
+    lib.mq_sample_workspace_size.restype = _sz
+    lib.mq_sample_workspace_size.argtypes = [_i64] * 2
+    lib.mq_sample.restype = _int
+    lib.mq_sample.argtypes = [_vp, _i64, _i64, _i64, _int, _vp, _vp, _f32, _vp, _i32, _vp, _f32,
+                              _vp, _f32, _vp, _vp, _vp, _sz, _vp]
 
 
 def lib() -> ctypes.CDLL:

@@ -63,6 +63,11 @@ UNITS = [("abi.hip", []), ("formats.hip", []), ("prep.hip", []), ("route.hip", [
 ] + [
     ("mx_wide.hip", [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_QQ={qq}", "-fno-slp-vectorize"])
     for dt in (0, 1) for qq in (0, 1)
+] + [("glu_grad.hip", []), ("sample.hip", [])] + [
+    (src, [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_BITS={bits}", f"-DMQ_INST_GS={gs}",
+           "-fno-slp-vectorize"])
+    for src in ("glu.hip", "qmm_grad.hip") for dt in (0, 1) for bits in (4, 8)
+    for gs in (32, 64, 128)
 ] + [
     ("mx_grouped.hip", [f"-DMQ_INST_DT={dt}", "-fno-slp-vectorize"]) for dt in (0, 1)
 ]

@@ -10,8 +10,10 @@
 #include "../../include/mlxturbo_amd.h"
 #include "combine.cuh"
 #include "dequant.cuh"
+#include "glu_launch.h"
 #include "launch.h"
 #include "mx_launch.h"
+#include "sample_launch.h"
 
 namespace {
 
@@ -209,6 +211,75 @@ int mx_done(int rc, int nl, const char* what) {
   if (e != hipSuccess) return fail((int)e, "%s: launch failed: %s", what, hipGetErrorString(e));
   g_launches.fetch_add((uint64_t)nl, std::memory_order_relaxed);
   return MQ_OK;
+}
+
+// Arguments of the gated feed-forward block: two matrices of one format.
+int check_glu(const void* wg, const void* sg, const void* bg, const void* wu, const void* su,
+              const void* bu, int64_t M, int64_t N, int64_t K, int group_size, int bits, int dtype,
+              int activation, const void* workspace) {
+  int rc = check_common(wg, sg, bg, N, K, group_size, bits, dtype);
+  if (!rc) rc = check_common(wu, su, bu, N, K, group_size, bits, dtype);
+  if (rc) return rc;
+  if (dtype == MQ_FLOAT32)
+    return fail(MQ_EUNSUPPORTED, "float32 activations are not implemented on this path");
+  if (activation != MQ_ACT_SILU && activation != MQ_ACT_GELU_TANH)
+    return fail(MQ_EINVAL, "unknown activation code %d", activation);
+  if (M < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX / 8)
+    return fail(MQ_EINVAL, "invalid sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N,
+                (long long)K);
+  if (workspace && !aligned16(workspace)) return fail(MQ_EINVAL, "workspace must be 16-byte aligned");
+  return MQ_OK;
+}
+
+// dx = d . W, or with sums given the gated block's gradient, which makes d's halves in
+// the workspace first.
+int grad_product(const void* d, const float* gate_sums, const float* up_sums, const uint32_t* w1,
+                 const void* s1, const void* b1, const uint32_t* w2, const void* s2,
+                 const void* b2, void* dx, int64_t M, int64_t N, int64_t K, int group_size,
+                 int bits, int dtype, int activation, void* workspace, size_t workspace_bytes,
+                 void* hip_stream, const char* what) {
+  const int banks = w2 ? 2 : 1;
+  int rc = check_common(w1, s1, b1, N, K, group_size, bits, dtype);
+  if (rc) return rc;
+  if (dtype == MQ_FLOAT32)
+    return fail(MQ_EUNSUPPORTED, "float32 gradients are not implemented on this path");
+  if (!d || !dx) return fail(MQ_EINVAL, "d and dx must be non-null");
+  if (!aligned16(d)) return fail(MQ_EINVAL, "d must be 16-byte aligned");
+  if (M < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX / 8)
+    return fail(MQ_EINVAL, "invalid sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N,
+                (long long)K);
+  if (workspace && !aligned16(workspace)) return fail(MQ_EINVAL, "workspace must be 16-byte aligned");
+  if (M == 0) return MQ_OK;
+  if (N == 0) return fail(MQ_EUNSUPPORTED, "%s of no columns is all zeros", what);
+  const size_t rows = mq::grad_rows_bytes(M, N, banks);
+  const int64_t ld = rows ? banks * 64 * mq::grad_steps(N) : N;
+  if (!mq::grad_eligible(M, N, K, bits, ld))
+    return fail(MQ_EUNSUPPORTED, "%s: the matrix or a tile's rows pass a 31-bit range", what);
+  if (rows && (!workspace || workspace_bytes < rows))
+    return fail(MQ_EINVAL, "%s needs a workspace of %zu bytes, 16-byte aligned", what, rows);
+  const hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+  const int cus = mq::device_cu_count();
+  mq::WidePlan plan = mq::grad_plan(M, N, K, bits, banks, cus, 16);
+  if (plan.splits > 1 &&
+      (!workspace || workspace_bytes < rows + mq::wide_workspace_bytes(plan, M, K)))
+    plan = mq::grad_plan(M, N, K, bits, banks, cus, 1);
+  int nl = 0;
+  const void* dr = d;
+  if (banks == 2) {
+    rc = mq::launch_glu_grad(d, gate_sums, up_sums, workspace, M, N, activation, dtype, st);
+    dr = workspace;
+    ++nl;
+  } else if (rows) {
+    rc = mq::launch_pad_rows(d, workspace, M, N, st);
+    dr = workspace;
+    ++nl;
+  }
+  const mq::GradArgs a{dr, ld, w1, s1, b1, w2, s2, b2, dx, M, N, K};
+  if (!rc)
+    rc = dispatch_16<mq::GradLaunch>(dtype, bits, group_size, a, plan,
+                                     workspace ? static_cast<char*>(workspace) + rows : nullptr,
+                                     st, &nl);
+  return mx_done(rc, nl, what);
 }
 
 }  // namespace
@@ -889,6 +960,128 @@ int mq_mxfp4_gather_qmm(const void* x, const uint32_t* w, const uint8_t* scales,
              : mq::MxGatherLaunch<mq::kF16>::run(x, w, scales, lhs_indices, rhs_indices, out, P, B,
                                                  M, N, K, E, workspace, st, &nl);
   return mx_done(rc, nl, "mxfp4 gather_qmm");
+}
+
+size_t mq_quantized_glu_workspace_size(int64_t M, int64_t N, int64_t K, int group_size, int bits) {
+  if (M <= 0 || N <= 0 || K <= 0 || (bits != 4 && bits != 8) || group_size <= 0) return 0;
+  return mq::glu_workspace_bytes(M, N, K, bits, mq::device_cu_count());
+}
+
+int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_scales,
+                     const void* gate_biases, const uint32_t* up_w, const void* up_scales,
+                     const void* up_biases, void* out, float* gate_sums, float* up_sums, int64_t M,
+                     int64_t N, int64_t K, int group_size, int bits, int dtype, int activation,
+                     void* workspace, size_t workspace_bytes, void* hip_stream) {
+  int rc = check_glu(gate_w, gate_scales, gate_biases, up_w, up_scales, up_biases, M, N, K,
+                     group_size, bits, dtype, activation, workspace);
+  if (rc) return rc;
+  if (!x || !out) return fail(MQ_EINVAL, "x and out must be non-null");
+  if (!gate_sums != !up_sums) return fail(MQ_EINVAL, "gate_sums and up_sums are given together");
+  if (!aligned16(x)) return fail(MQ_EINVAL, "x must be 16-byte aligned");
+  if (M == 0 || N == 0) return MQ_OK;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
+  const mq::GluArgs a{x,  gate_w, gate_scales, gate_biases, up_w, up_scales, up_biases, out, gate_sums,
+                      up_sums, M, N, K, activation};
+  int nl = 0;
+  if (mq::glu_wide_route(M, N, K)) {
+    const int cus = mq::device_cu_count();
+    mq::WidePlan plan = mq::glu_wide_plan(M, N, K, bits, cus, 16);
+    if (plan.splits > 1 && (!workspace || workspace_bytes < mq::glu_workspace_bytes(M, N, K, bits, cus)))
+      plan = mq::glu_wide_plan(M, N, K, bits, cus, 1);
+    rc = dispatch_16<mq::GluWideLaunch>(dtype, bits, group_size, a, plan, workspace, st, &nl);
+  } else {
+    for (int64_t m0 = 0; m0 < M && !rc; m0 += mq::kGluSkinnyRows) {
+      const int64_t m = M - m0 < mq::kGluSkinnyRows ? M - m0 : mq::kGluSkinnyRows;
+      rc = dispatch_16<mq::GluSkinnyLaunch>(dtype, bits, group_size, a, m0, m, st);
+      ++nl;
+    }
+  }
+  return mx_done(rc, nl, "quantized_glu");
+}
+
+size_t mq_quantized_matmul_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
+                                               int bits) {
+  if (M <= 0 || N <= 0 || K <= 0 || (bits != 4 && bits != 8) || group_size <= 0) return 0;
+  return mq::grad_workspace_bytes(M, N, K, bits, 1, mq::device_cu_count());
+}
+
+int mq_quantized_matmul_grad(const void* d, const uint32_t* w, const void* scales,
+                             const void* biases, void* dx, int64_t M, int64_t N, int64_t K,
+                             int group_size, int bits, int dtype, void* workspace,
+                             size_t workspace_bytes, void* hip_stream) {
+  return grad_product(d, nullptr, nullptr, w, scales, biases, nullptr, nullptr, nullptr, dx, M, N,
+                      K, group_size, bits, dtype, 0, workspace, workspace_bytes, hip_stream,
+                      "quantized_matmul_grad");
+}
+
+size_t mq_quantized_glu_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
+                                            int bits) {
+  if (M <= 0 || N <= 0 || K <= 0 || (bits != 4 && bits != 8) || group_size <= 0) return 0;
+  return mq::grad_workspace_bytes(M, N, K, bits, 2, mq::device_cu_count());
+}
+
+int mq_quantized_glu_grad(const void* d, const float* gate_sums, const float* up_sums,
+                          const uint32_t* gate_w, const void* gate_scales,
+                          const void* gate_biases, const uint32_t* up_w, const void* up_scales,
+                          const void* up_biases, void* dx, int64_t M, int64_t N, int64_t K,
+                          int group_size, int bits, int dtype, int activation, void* workspace,
+                          size_t workspace_bytes, void* hip_stream) {
+  if (!gate_sums || !up_sums) return fail(MQ_EINVAL, "gate_sums and up_sums must be non-null");
+  const int rc = check_glu(gate_w, gate_scales, gate_biases, up_w, up_scales, up_biases, M, N, K,
+                           group_size, bits, dtype, activation, workspace);
+  if (rc) return rc;
+  return grad_product(d, gate_sums, up_sums, gate_w, gate_scales, gate_biases, up_w, up_scales,
+                      up_biases, dx, M, N, K, group_size, bits, dtype, activation, workspace,
+                      workspace_bytes, hip_stream, "quantized_glu_grad");
+}
+
+size_t mq_sample_workspace_size(int64_t rows, int64_t vocabulary) {
+  if (rows <= 0 || vocabulary <= 0) return 0;
+  return mq::sample_workspace_bytes(rows, vocabulary);
+}
+
+int mq_sample(const void* logits, int64_t row_stride, int64_t rows, int64_t vocabulary, int dtype,
+              const float* u, const float* temperature, float temperature_value,
+              const int32_t* top_k, int32_t top_k_value, const float* top_p, float top_p_value,
+              const float* min_p, float min_p_value, int32_t* tokens, float* logprobs,
+              void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (!logits || !u || !tokens || !logprobs)
+    return fail(MQ_EINVAL, "logits, u, tokens and logprobs must be non-null");
+  if (dtype != MQ_BFLOAT16 && dtype != MQ_FLOAT16 && dtype != MQ_FLOAT32)
+    return fail(MQ_EINVAL, "unknown dtype code %d", dtype);
+  if (rows < 0 || vocabulary <= 0 || row_stride < 0)
+    return fail(MQ_EINVAL, "invalid sizes rows=%lld vocabulary=%lld row_stride=%lld",
+                (long long)rows, (long long)vocabulary, (long long)row_stride);
+  if (vocabulary > ((int64_t)1 << 30))
+    return fail(MQ_EUNSUPPORTED, "sample supports vocabularies of up to 2^30 words");
+  if ((uintptr_t)logits % (dtype == MQ_FLOAT32 ? 4 : 2))
+    return fail(MQ_EINVAL, "logits must be aligned to their type");
+  if (rows == 0) return MQ_OK;
+  const size_t need = mq::sample_workspace_bytes(rows, vocabulary);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(MQ_EINVAL, "workspace of %zu bytes, 16-byte aligned, needed", need);
+  int bits = 0;                                 // of the vocabulary: sums stay below 2^62
+  while (((int64_t)1 << bits) < vocabulary) ++bits;
+  mq::SampleArgs a{};
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.R = rows;
+  a.V = vocabulary;
+  a.u = u;
+  a.temperature = temperature;
+  a.temperature0 = temperature_value;
+  a.top_k = top_k;
+  a.top_k0 = top_k_value;
+  a.top_p = top_p;
+  a.top_p0 = top_p_value;
+  a.min_p = min_p;
+  a.min_p0 = min_p_value;
+  a.scale = (double)((uint64_t)1 << (62 - bits < 44 ? 62 - bits : 44));
+  a.token = tokens;
+  a.logprob = logprobs;
+  int nl = 0;
+  const int rc = mq::launch_sample(a, dtype, workspace, reinterpret_cast<hipStream_t>(hip_stream), &nl);
+  return mx_done(rc, nl, "sample");
 }
 
 }  // extern "C"

@@ -1,0 +1,116 @@
+// Launchers of the dense gated feed-forward block (glu.cuh, glu_wide.cuh) and of
+// products past quantized weights (qmm_grad.cuh), shared by their translation
+// units and the C ABI.
+#pragma once
+#include "launch.h"
+
+namespace mq {
+
+enum GluAct { kActSilu = 0, kActGeluTanh = 1 };
+
+// the tanh GELU: g / (1 + exp(-kGeluZ (g + kGeluCubic g^3))), kGeluZ = 2 sqrt(2 / pi)
+constexpr float kGeluZ = 1.5957691216057308f, kGeluCubic = 0.044715f;
+
+// out[M, N] = act(x . Wg^T) * (x . Wu^T); gf and uf (both or neither): the two
+// products in float, [M, N].
+struct GluArgs {
+  const void* x;
+  const uint32_t* wg;
+  const void *sg, *bg;
+  const uint32_t* wu;
+  const void *su, *bu;
+  void* out;
+  float *gf, *uf;
+  int64_t M, N, K;
+  int act;
+};
+
+// Rows m0 .. m0 + M - 1 (M <= kGluSkinnyRows), one launch.
+constexpr int kGluSkinnyRows = 16;
+template <int DT, int BITS, int GS>
+struct GluSkinnyLaunch {
+  static int run(const GluArgs& a, int64_t m0, int64_t M, hipStream_t st);
+};
+
+// All rows on the MFMA tile, 64 .. 256 rows by 128 columns of both matrices; with
+// plan.splits > 1 over K splits, whose float planes ws holds.
+template <int DT, int BITS, int GS>
+struct GluWideLaunch {
+  static int run(const GluArgs& a, const WidePlan& plan, void* ws, hipStream_t st, int* nlaunch);
+};
+
+inline bool glu_wide_eligible(int64_t M, int64_t K) {
+  return K % 64 == 0 && K * 2 * 256 < ((int64_t)1 << 31) && M <= ((int64_t)65535) * 64;
+}
+
+inline WidePlan glu_wide_plan(int64_t M, int64_t N, int64_t K, int bits, int cus, int max_splits) {
+  return wide_plan(M, 2 * N, K, bits, cus, max_splits);
+}
+
+// Rows from which the MFMA tile runs.
+inline bool glu_wide_route(int64_t M, int64_t N, int64_t K) {
+  (void)N;
+  return M > kGluSkinnyRows && glu_wide_eligible(M, K);
+}
+
+inline size_t glu_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int cus) {
+  if (!glu_wide_route(M, N, K)) return 0;
+  const WidePlan p = glu_wide_plan(M, N, K, bits, cus, 16);
+  return p.splits > 1 ? (size_t)p.splits * 2 * (size_t)M * (size_t)N * sizeof(float) : 0;
+}
+
+// ---- gradients past the weights ---------------------------------------------
+
+// Steps of 64 weight rows that N rows take.
+inline int64_t grad_steps(int64_t N) { return (N + 63) / 64; }
+
+// dgu[M, 2 * 64 * grad_steps(N)] (T): d * u * act'(g) in the first half, d * act(g)
+// in the second, zeros past N columns (glu_grad.hip).
+int launch_glu_grad(const void* d, const float* gf, const float* uf, void* dgu, int64_t M,
+                    int64_t N, int act, int dtype, hipStream_t st);
+
+// Rows of N elements of a 16-bit type to rows of 64 * grad_steps(N), zeros past N.
+int launch_pad_rows(const void* d, void* out, int64_t M, int64_t N, hipStream_t st);
+
+// out[M, K] = d[:, first half] . W1 + d[:, second half] . W2 (w2 NULL: d . W1) for
+// quantized W [N, K]; d's rows of ld elements, a half padded to whole steps of
+// 64 columns with zeros.
+struct GradArgs {
+  const void* d;
+  int64_t ld;
+  const uint32_t* w1;
+  const void *s1, *b1;
+  const uint32_t* w2;
+  const void *s2, *b2;
+  void* out;
+  int64_t M, N, K;
+};
+
+template <int DT, int BITS, int GS>
+struct GradLaunch {
+  static int run(const GradArgs& a, const WidePlan& plan, void* ws, hipStream_t st, int* nlaunch);
+};
+
+// one tile's rows of d, and the matrices, must fit 31-bit buffer ranges
+inline bool grad_eligible(int64_t M, int64_t N, int64_t K, int bits, int64_t ld) {
+  return N * (K * bits / 8) < ((int64_t)1 << 31) && ld * 2 * 256 < ((int64_t)1 << 31) &&
+         M <= (int64_t)65535 * 64;
+}
+
+inline WidePlan grad_plan(int64_t M, int64_t N, int64_t K, int bits, int banks, int cus,
+                          int max_splits) {
+  return wide_plan(M, K, banks * 64 * grad_steps(N), bits, cus, max_splits);
+}
+
+// Workspace of a product past one matrix (banks 1) or two: d's padded rows where N is
+// not whole steps (banks 2: dgu), then the split planes.
+inline size_t grad_rows_bytes(int64_t M, int64_t N, int banks) {
+  if (banks == 1 && N % 64 == 0) return 0;
+  return ((size_t)M * banks * 64 * (size_t)grad_steps(N) * 2 + 255) & ~(size_t)255;
+}
+inline size_t grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int banks, int cus) {
+  return grad_rows_bytes(M, N, banks) +
+         wide_workspace_bytes(grad_plan(M, N, K, bits, banks, cus, 16), M, K);
+}
+
+}  // namespace mq

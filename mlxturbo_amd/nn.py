@@ -12,6 +12,9 @@ Torch counterparts of the layers the reference routes through its kernels:
   qwen4_exp.py:1795-1802), including the ``_gather_sort`` path that sorts
   pairs by expert and passes ``sorted_indices=True`` (fused.py:2402-2418).
 
+* :class:`QuantizedMLP` - a dense model's gated feed-forward block over three
+  :class:`QuantizedLinear` (mlx-lm's ``MLP``).
+
 With ``mode="mxfp4"`` the same layers hold block-scaled 4-bit weights (uint8
 ``scales``, no ``biases``, groups of 32); :class:`QQLinear` (``mlx.nn.QQLinear``)
 brings its activations into that format as well.
@@ -26,6 +29,7 @@ from typing import Optional
 import torch
 
 from . import ops
+from . import glu as _glu  # after ops, which imports it
 
 
 def _check_quantized(weight: torch.Tensor, scales: torch.Tensor,
@@ -187,6 +191,40 @@ class QQLinear(QuantizedLinear):
                     group_size: Optional[int] = None, bits: Optional[int] = None,
                     mode: str = "mxfp4") -> "QQLinear":
         return super().from_linear(weight, bias, group_size, bits, mode)
+
+
+class QuantizedMLP(torch.nn.Module):
+    """mlx-lm's dense ``MLP``: ``down_proj(act(gate_proj(x)) * up_proj(x))``, the first
+    half as :func:`ops.quantized_glu` where gate and up are affine layers of one
+    format without bias, else as the two layers and the activation in float.
+    Where x requires grad, the backward pass gives its gradient."""
+
+    def __init__(self, gate_proj: QuantizedLinear, up_proj: QuantizedLinear,
+                 down_proj: QuantizedLinear, activation: str = "silu"):
+        super().__init__()
+        if activation not in _glu.ACTIVATIONS:
+            raise ValueError(f"activation must be one of {tuple(_glu.ACTIVATIONS)}, "
+                             f"got {activation!r}")
+        self.gate_proj = gate_proj
+        self.up_proj = up_proj
+        self.down_proj = down_proj
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        g, u = self.gate_proj, self.up_proj
+        if (g.mode == "affine" and g.bias is None and u.bias is None
+                and g.weight.shape == u.weight.shape and g.scales.dtype == u.scales.dtype
+                and (g.group_size, g.bits, g.mode) == (u.group_size, u.bits, u.mode)):
+            h = ops.quantized_glu(x, (g.weight, g.scales, g.biases),
+                                  (u.weight, u.scales, u.biases), self.activation,
+                                  group_size=g.group_size, bits=g.bits)
+        else:
+            gv, uv = g(x), u(x)
+            h = (_glu._activation(gv.float(), self.activation) * uv.float()).to(gv.dtype)
+        return self.down_proj(h)
+
+    def extra_repr(self) -> str:
+        return f"activation={self.activation!r}"
 
 
 class QuantizedSwitchLinear(_Quantized):
@@ -393,4 +431,4 @@ class SwitchGLU(torch.nn.Module):
         return y
 
 
-__all__ = ["QQLinear", "QuantizedLinear", "QuantizedSwitchLinear", "SwitchGLU"]
+__all__ = ["QQLinear", "QuantizedLinear", "QuantizedMLP", "QuantizedSwitchLinear", "SwitchGLU"]

@@ -278,6 +278,10 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     the matmul kernels; every other MLX configuration runs as the library's
     dequantize plus one GPU GEMM (:func:`_composed_qmm`).  ``mode="mxfp4"``
     (uint8 scales, no biases) takes the same x and gives x's dtype.
+
+    Where ``x`` requires grad, so does the affine result: the backward pass gives x's
+    gradient ``d @ dequantize(w)`` (mq_quantized_matmul_grad where the forward ran on
+    the kernels); the weights are constants.
     """
     group_size, bits = _format(group_size, bits, mode)
     if mode == "mxfp4":
@@ -295,6 +299,8 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
             f"x last dimension {x.shape[-1]} does not match the quantized weight K={K}")
     if not (transpose and bits in (4, 8) and _kernel_dtype(x.dtype, scales.dtype)):
         return _composed_qmm(x, w, scales, biases, transpose, group_size, bits)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _glu.quantized_matmul_differentiable(x, w, scales, biases, group_size, bits)
     code = _DTYPE_CODE[x.dtype]
     lead = tuple(x.shape[:-1])
     M = math.prod(lead)
@@ -374,7 +380,7 @@ def quantized_matmul_prepared(x: torch.Tensor, p: PreparedWeights) -> torch.Tens
     shape = x.shape
     N, K = p.N, p.K
     if (p.code is None or x.dtype != p.dtype or x.get_device() != p.index or not shape
-            or shape[-1] != K):
+            or shape[-1] != K or x.requires_grad and torch.is_grad_enabled()):
         return quantized_matmul(x, p.w, p.s, p.b, group_size=p.group_size, bits=p.bits)
     M = x.numel() // K
     out = torch.empty((*shape[:-1], N), dtype=p.dtype, device=p.dev)
@@ -1321,8 +1327,11 @@ def row_identity(on: bool = True):
 __all__: Sequence[str] = ("quantize", "dequantize", "quantized_matmul", "quantized_matmul_prepared",
                           "PreparedWeights", "gather_qmm", "gather_glu", "moe_combine",
                           "gather_tables", "GatherTables", "swiglu", "moe_block",
-                          "launch_count", "set_row_identity", "row_identity")
+                          "launch_count", "set_row_identity", "row_identity", "quantized_glu", "sample")
 
 
-# after the helpers that it uses
+# after the helpers that they use
+from . import glu as _glu  # noqa: E402
 from . import mx as _mx  # noqa: E402
+from .glu import quantized_glu  # noqa: E402
+from .sampling import sample  # noqa: E402
