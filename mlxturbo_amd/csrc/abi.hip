@@ -1037,7 +1037,7 @@ int mq_quantized_glu_grad(const void* d, const float* gate_sums, const float* up
 
 size_t mq_sample_workspace_size(int64_t rows, int64_t vocabulary) {
   if (rows <= 0 || vocabulary <= 0) return 0;
-  return mq::sample_workspace_bytes(rows, vocabulary);
+  return mq::sample_workspace_bytes(rows);
 }
 
 int mq_sample(const void* logits, int64_t row_stride, int64_t rows, int64_t vocabulary, int dtype,
@@ -1057,7 +1057,7 @@ int mq_sample(const void* logits, int64_t row_stride, int64_t rows, int64_t voca
   if ((uintptr_t)logits % (dtype == MQ_FLOAT32 ? 4 : 2))
     return fail(MQ_EINVAL, "logits must be aligned to their type");
   if (rows == 0) return MQ_OK;
-  const size_t need = mq::sample_workspace_bytes(rows, vocabulary);
+  const size_t need = mq::sample_workspace_bytes(rows);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(MQ_EINVAL, "workspace of %zu bytes, 16-byte aligned, needed", need);
   int bits = 0;                                 // of the vocabulary: sums stay below 2^62

@@ -18,6 +18,7 @@ struct SampleArgs {
   float temperature0, top_p0, min_p0;
   int32_t top_k0;
   double scale;                                 // mass of the most probable word
+  int tile;                                     // log2 of a tile's 16-byte granules
   int32_t* token;
   float* logprob;
 };
@@ -25,23 +26,32 @@ struct SampleArgs {
 // Rows of one sequence of launches, whose workspace they share.
 constexpr int kSampleRows = 256;
 
-// Chunks of a row: about 1024 workgroups over the rows of a sequence, of 2048 words
+// Chunks of a row: about 1024 workgroups over the rows of a sequence, of 4096 words
 // at least.
 inline int sample_chunks(int64_t R, int64_t V) {
   const int64_t rows = R < kSampleRows ? R : kSampleRows;
   int64_t c = 1024 / (rows > 0 ? rows : 1);
-  if (c > (V + 2047) / 2048) c = (V + 2047) / 2048;
+  if (c > (V + 4095) / 4096) c = (V + 4095) / 4096;
   return c < 1 ? 1 : (int)c;
 }
 
-// Bytes of a row's workspace: two arrays of C, masses of 2048 bins, a list of 4096, and
-// 2048 counts and the list's length.
-__host__ __device__ inline size_t sample_row_bytes(int C) {
-  return ((size_t)C * 16 + 2048 * 8 + 4096 * 8 + 2049 * 4 + 15) & ~(size_t)15;
+// A row's tiles: of 64 granules, or more where that would be over 1024 of them.
+constexpr int kSampleTiles = 1024;
+inline int sample_tile(int64_t V, int dtype) {
+  const int64_t e = dtype == kF32 ? 4 : 8, n = (V + 2 * e - 2) / e;
+  int tile = 6;
+  while ((n + ((int64_t)1 << tile) - 1) >> tile > kSampleTiles) ++tile;
+  return tile;
 }
 
-inline size_t sample_workspace_bytes(int64_t R, int64_t V) {
-  return (size_t)(R < kSampleRows ? R : kSampleRows) * sample_row_bytes(sample_chunks(R, V));
+// A row's workspace: the tiles' first words and masses, masses of the bins, the list,
+// the row's first word and bound, and counts of the bins, the list's length and the workgroups that are done.
+constexpr int kSampleBins = 2048, kSampleList = 4096;
+constexpr size_t kSampleRowBytes =
+    (2 * kSampleTiles + kSampleBins + kSampleList + 2) * 8 + (kSampleBins + 4) * 4;
+
+inline size_t sample_workspace_bytes(int64_t R) {
+  return (size_t)(R < kSampleRows ? R : kSampleRows) * kSampleRowBytes;
 }
 
 int launch_sample(const SampleArgs& a, int dtype, void* ws, hipStream_t st, int* nlaunch);

@@ -18,6 +18,10 @@ from . import _lib, glu, ops
 def _setting(name: str, v, lead: tuple, dev: torch.device, dtype: torch.dtype, least, most):
     """``(pointer or None, value, the tensor)`` of one setting."""
     if isinstance(v, torch.Tensor):
+        # a tensor of the rows' own: nothing to convert
+        if (v.dtype == dtype and v.shape == lead and v.get_device() == dev.index
+                and v.is_contiguous()):
+            return v.data_ptr(), 0, v
         ops._require_gpu(v)
         if v.device != dev:
             raise ValueError(f"{name} is on {v.device}, logits on {dev}")
@@ -72,8 +76,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     if u.dtype != torch.float32 or tuple(u.shape) != lead:
         raise ValueError(f"u must be float32 {lead}, got {u.dtype} {tuple(u.shape)}")
     R = math.prod(lead)
-    inf = math.inf
-    t = _setting("temperature", temperature, lead, dev, torch.float32, 0.0, inf)
+    t = _setting("temperature", temperature, lead, dev, torch.float32, 0.0, math.inf)
     k = _setting("top_k", top_k, lead, dev, torch.int32, 0, 2 ** 31 - 1)
     p = _setting("top_p", top_p, lead, dev, torch.float32, 0.0, 1.0)
     m = _setting("min_p", min_p, lead, dev, torch.float32, 0.0, 1.0)
@@ -82,17 +85,19 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     if R == 0:
         return tokens, logprobs
     # rows where they lie, if one stride leads from each to the next
-    l = logits.detach()
-    if V > 1 and l.stride(-1) != 1:
-        l = l.contiguous()
-    try:
-        l = l.view(R, V)
-    except RuntimeError:
-        l = l.reshape(R, V)
-    stride = l.stride(0) if R > 1 else V
-    u_ = u.detach().contiguous()
+    l, stride = logits, V
+    if not l.is_contiguous():
+        if l.stride(-1) != 1:
+            l = l.contiguous()
+        try:
+            l = l.view(R, V)
+        except RuntimeError:
+            l = l.reshape(R, V)
+        if R > 1:
+            stride = l.stride(0)
+    u_ = u.contiguous()
     lib = _lib.lib()
-    ws = torch.empty(int(lib.mq_sample_workspace_size(R, V)), dtype=torch.uint8, device=dev)
+    ws = torch.empty(lib.mq_sample_workspace_size(R, V), dtype=torch.uint8, device=dev)
     rc = lib.mq_sample(l.data_ptr(), stride, R, V, ops._DTYPE_CODE[l.dtype], u_.data_ptr(),
                        *t[:2], *k[:2], *p[:2], *m[:2], tokens.data_ptr(), logprobs.data_ptr(),
                        ws.data_ptr(), ws.numel(), ops._stream_ptr(tokens))
