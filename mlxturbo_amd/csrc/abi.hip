@@ -259,7 +259,7 @@ int grad_product(const void* d, const float* gate_sums, const float* up_sums, co
     return fail(MQ_EINVAL, "%s needs a workspace of %zu bytes, 16-byte aligned", what, rows);
   const hipStream_t st = reinterpret_cast<hipStream_t>(hip_stream);
   const int cus = mq::device_cu_count();
-  mq::WidePlan plan = mq::grad_plan(M, N, K, bits, banks, cus, 16);
+  mq::WidePlan plan = mq::grad_plan(M, N, K, bits, banks, cus, mq::kGradSplits);
   if (plan.splits > 1 &&
       (!workspace || workspace_bytes < rows + mq::wide_workspace_bytes(plan, M, K)))
     plan = mq::grad_plan(M, N, K, bits, banks, cus, 1);
