@@ -4,22 +4,33 @@
 // Sums in float over the dequantized T weights, act in float, one rounding to
 // T; with gf and uf the two sums are written as well (float, for the gradient).
 //
-// Up to 16 rows the weight stream bounds the call.  A workgroup of 16 waves, one
+// Up to 16 rows, a workgroup of 16 waves, one
 // per CU, runs up to 16 tiles of 8 output columns.  A tile's A operand of
 // v_mfma_f32_16x16x32 is 8 rows of the gate matrix and the same 8 of the up
 // matrix, so both sums of a column are in one accumulator.
-//  * The x rows lie in LDS once for all tiles (in slices of K where they do not
-//    fit), so no step loads x.
-//  * A tile's K range is cut into units of 256 bytes of each row; the units of
+//  * The x rows lie in LDS once for all tiles, and so do the tiles' scales and biases
+//    (a dword per group), both in slices of K where they do not fit: no step loads
+//    either.  Read per step, 16 bytes of 16 rows at a time, the scales alone cost 6.8 of
+//    27.7 us (loads without the arithmetic; N=17408 K=5120, weights from memory).
+//  * A tile's K range is cut into units of one 128-byte line of each row; the units of
 //    all the workgroup's tiles, in order, are dealt to the waves in contiguous
-//    runs that differ by one unit at most.  A wave streams its run without a
-//    stop at the tiles' ends; a run of at most one tile's units touches at
-//    most two tiles, whose sums go to two places of LDS, and one wave per
-//    tile adds them in wave order.  The order depends on N, K and the CU count
+//    runs that differ by one unit at most.  A wave
+//    streams its run one unit ahead, without a stop at the tiles' ends: 16 waves
+//    hold 64 KB of loads in flight per CU; two, three and four units ahead took 0.9, 1.9 and
+//    2.9 us more of 28, as the scales then wait for behind the weights.  A run of at most
+//    one tile's units touches at most two tiles, whose sums meet the other waves' in LDS
+//    at the end, added in wave order: an order that depends on N, K and the CU count
 //    alone.
-//  * Lane (r = lane & 15, c = lane >> 4) takes of row r's unit the 16-byte
-//    pieces at 64 p + 16 c, p = 0..3: a load instruction reads whole 64-byte
-//    sectors, the four of them whole lines.
+//  * A load instruction reads one whole line of 8 rows of one matrix, non-temporal: lane
+//    (r = lane & 15, c = lane >> 4) the 16-byte chunk 2 c + (r >> 3) of row r & 7.  The
+//    operand wants rows 8 .. 15 to be the up matrix's: lanes r < 8 and r >= 8 of a
+//    gate and an up register change places by one DPP move each, after which both hold
+//    chunk 2 c, or 2 c + 1, of 16 rows.
+// Bound by the exact dequantization (20 VALU per 8 codes; v_fma_mix, v_cvt_pk and DPP moves
+// issue every 4.9 cycles, and and shift every 2.8) over the 15 us after the scales, whose
+// read and barrier take 5.5, and by the last workgroups' 9 tiles against 8.5 on average:
+// N=17408 K=5120, 4 bits, 25.9, 26.6 and 34.3 us for 2, 8 and 16 rows (100 MB: 20 us at the
+// rate of a copy); 8 bits 36.7, 37.4 and 44.7; N=4096 K=4096 11.4, 12.3 and 13.3.
 #pragma once
 #include "glu_launch.h"
 #include "stream_tile.cuh"
@@ -39,21 +50,38 @@ constexpr int kGluCols = 8;                     // output columns of a tile
 
 template <int BITS>
 struct GluGeom {
-  static constexpr int UC = 2048 / BITS;        // codes per row and unit
-  static constexpr int PC = 128 / BITS;         // codes per 16-byte piece
+  static constexpr int PC = 128 / BITS;         // codes per 16-byte chunk
+  static constexpr int UC = 8 * PC;             // codes per row and unit
 };
 
-// LDS: the waves' two sums, the tiles' sums (K slices), x rows.
+// LDS: the waves' two sums (in place of x and scales, at the end), then the tiles' sums
+// where K is sliced.
 constexpr int kGluPart = kGluWaves * 2 * 1024;
 constexpr int kGluSum = kGluTiles * 1024;
 
 // Bytes between x rows of a slice of `codes` codes: an odd number of 16-byte
 // chunks, so that a fragment's 16 rows lie in distinct banks.
 __host__ __device__ inline int glu_xstride(int codes) { return (codes * 2 + 31) / 32 * 32 + 16; }
+// Dwords between rows' scales of a slice: an odd multiple of 4, so that 16 rows' and 4
+// groups' lie in distinct banks.
+__host__ __device__ inline int glu_sstride(int groups) { return (groups + 3) / 8 * 8 + 4; }
 
-// SV: a unit's scales are read as dwords (whole units of K, 4-byte aligned scales
-// and biases), else one by one.
-template <int DT, int BITS, int GS, bool SV>
+// LDS of a slice of `units` units: x of M rows, scales of `tiles` tiles.
+template <int BITS, int GS>
+__host__ __device__ inline size_t glu_slice_bytes(int64_t M, int tiles, int units) {
+  constexpr int UC = GluGeom<BITS>::UC;
+  const size_t n = (size_t)M * glu_xstride(units * UC) +
+                   (size_t)tiles * 2 * kGluCols * 4 * glu_sstride(units * (UC / GS));
+  return ((n > (size_t)kGluPart ? n : (size_t)kGluPart) + 15) & ~(size_t)15;
+}
+
+// Lanes 8 .. 15 of every 16 of a from lanes 0 .. 7 of b (HIGH), or the reverse.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t swap_halves(uint32_t a, uint32_t b) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xf, HIGH ? 0xc : 0x3, false);
+}
+
+template <int DT, int BITS, int GS>
 __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
     const uint16_t* __restrict__ x, const uint32_t* __restrict__ wg,
     const uint16_t* __restrict__ sg, const uint16_t* __restrict__ bg,
@@ -63,13 +91,10 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
   using T = T16<DT>;
   constexpr int UC = GluGeom<BITS>::UC, PC = GluGeom<BITS>::PC;
   constexpr int GU = UC / GS;                   // groups per unit
-  constexpr int WP = BITS == 4 ? 4 : 2;         // MFMAs per piece
-  constexpr int ND = GU / 2;                    // their dwords
-  static_assert(GU >= 2, "whole dwords of scales");
+  constexpr int WP = BITS == 4 ? 4 : 2;         // MFMAs per chunk
+  constexpr int R = 2;                          // units in registers
   extern __shared__ __align__(16) unsigned char lds[];
   f32x4* part = reinterpret_cast<f32x4*>(lds);
-  f32x4* sums = reinterpret_cast<f32x4*>(lds + kGluPart);
-  unsigned char* xl = lds + kGluPart + (slice * UC < K ? kGluSum : 0);
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int t0 = (int)((int64_t)tiles * blockIdx.x / gridDim.x);
@@ -77,157 +102,216 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
   const int S = (K + UC - 1) / UC;              // units of a row
   const int G = K / GS;
   const uint32_t rowB = (uint32_t)K * BITS / 8;
-  // gate rows in lanes r < 8, up rows in the others
-  const unsigned char* wb = reinterpret_cast<const unsigned char*>(r < 8 ? wg : wu);
-  const uint16_t* sb = r < 8 ? sg : su;
-  const uint16_t* bb = r < 8 ? bg : bu;
+  const int xs = glu_xstride(slice * UC), ss = glu_sstride(slice * GU);
+  unsigned char* xl = lds;
+  uint32_t* sl = reinterpret_cast<uint32_t*>(lds + M * xs);
+  f32x4* sums = reinterpret_cast<f32x4*>(
+      lds + glu_slice_bytes<BITS, GS>(M, (tiles + (int)gridDim.x - 1) / (int)gridDim.x, slice));
 
-  u32x4 W[2][4];
-  uint32_t sc[2][2][SV ? ND : 4];               // [ring][scale, bias]: SV dwords, else the pieces'
-  // unit s of tile t0 + j into slot b
-  auto load = [&](auto bc, int j, int s) {
+  u32x4 W[R][2];                                // a line of the gate's rows, and of the up's
+  const uint32_t lo = 16u * (2 * c + (r >> 3));
+  const unsigned char *pg = nullptr, *pu = nullptr;
+  uint32_t ro = 0;
+  // tile j's first row in both matrices, and this lane's row (the last, past N)
+  auto tile_at = [&](int j) {
+    const int64_t n0 = (int64_t)(t0 + j) * kGluCols;
+    pg = reinterpret_cast<const unsigned char*>(wg) + n0 * rowB;
+    pu = reinterpret_cast<const unsigned char*>(wu) + n0 * rowB;
+    ro = (uint32_t)min(r & 7, (int)(N - 1 - n0)) * rowB;
+  };
+  // unit s of that tile into slot b; chunks past the row read its last one
+  auto load = [&](auto bc, int s) {
     constexpr int b = decltype(bc)::value;
-    const int row = min((t0 + j) * kGluCols + (r & 7), N - 1);
-    const unsigned char* wr = wb + (int64_t)row * rowB;
-    const uint16_t* sr = sb + (int64_t)row * G;
-    const uint16_t* br = bb + (int64_t)row * G;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      uint32_t o = 256u * (uint32_t)s + 64u * p + 16u * c;
-      if constexpr (!SV) o = o < rowB ? o : 0u;
-      W[b][p] = *reinterpret_cast<const u32x4*>(wr + o);
-    }
-    if constexpr (SV) {
-      const uint32_t* s32 = reinterpret_cast<const uint32_t*>(sr + s * GU);
-      const uint32_t* b32 = reinterpret_cast<const uint32_t*>(br + s * GU);
-#pragma unroll
-      for (int q = 0; q < ND; ++q) {
-        sc[b][0][q] = s32[q];
-        sc[b][1][q] = b32[q];
-      }
-    } else {
-      // a piece past the row: zero scale and bias, so zero weights
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int k = s * UC + p * 4 * PC + c * PC, g = k < K ? k / GS : 0;
-        const uint32_t sv = sr[g], bv = br[g];
-        sc[b][0][p] = k < K ? sv : 0u;
-        sc[b][1][p] = k < K ? bv : 0u;
-      }
-    }
-  };
-  // scale (i = 0) or bias (1) of piece p as a float
-  auto param = [&](int b, int i, int p) -> float {
-    uint16_t v;
-    if constexpr (!SV) {
-      v = (uint16_t)sc[b][i][p];
-    } else if constexpr (4 * PC / GS == 4) {    // group 4 p + c
-      const uint32_t d = c & 2 ? sc[b][i][2 * p + 1] : sc[b][i][2 * p];
-      v = (uint16_t)(c & 1 ? d >> 16 : d);
-    } else if constexpr (4 * PC / GS == 2) {    // 2 p + (c >> 1)
-      v = (uint16_t)(c & 2 ? sc[b][i][p] >> 16 : sc[b][i][p]);
-    } else {
-      constexpr int per = GS / (4 * PC);        // p / per
-      const int g = p / per;
-      v = (uint16_t)(sc[b][i][g >> 1] >> (16 * (g & 1)));
-    }
-    return T::to_f32(v);
+    const uint32_t o = ro + min(128u * (uint32_t)s + lo, rowB - 16u);
+    W[b][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(pg + o));
+    W[b][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(pu + o));
   };
 
-  const int xs = glu_xstride(slice * UC);
-  for (int ph = 0, s0 = 0; s0 < S; ++ph, s0 += slice) {
+  for (int s0 = 0; s0 < S; s0 += slice) {
     const int ns = min(slice, S - s0);
     const int units = nt * ns;
     const int i0 = units * wave / kGluWaves, i1 = units * (wave + 1) / kGluWaves;
-    int j = i0 / ns, s = i0 - j * ns;
-    const int j0 = j;
-    if (i0 < i1) load(std::integral_constant<int, 0>{}, j, s0 + s);
-    if (ph) __syncthreads();                    // the last slice's x and sums are read
-    {
-      const int k0 = s0 * UC, ch = ns * UC / 8; // 16-byte chunks of a row
-      for (int i = t; i < M * ch; i += 64 * kGluWaves) {
-        const int m = i / ch, q = i - m * ch, k = k0 + 8 * q;
-        u32x4 v = {0, 0, 0, 0};
-        if (k < K) v = *reinterpret_cast<const u32x4*>(x + (int64_t)m * K + k);
-        *reinterpret_cast<u32x4*>(xl + m * xs + 16 * q) = v;
-      }
-    }
-    __syncthreads();
-    // rows past M repeat the last one: their columns are not stored
-    const unsigned char* xf = xl + min(r, M - 1) * xs + 2 * PC * c;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    auto step = [&](auto bc, int i) {
-      constexpr int b = decltype(bc)::value;
-      int jn = j, sn = s + 1;
-      if (sn == ns) {
-        sn = 0;
-        ++jn;
-      }
-      const bool more = i + 1 < i1;
-      load(std::integral_constant<int, b ^ 1>{}, more ? jn : j, s0 + (more ? sn : s));
-      float sv[4], bv[4];
-      bool big = false;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        sv[p] = param(b, 0, p);
-        bv[p] = param(b, 1, p);
-        big |= needs_plain(sv[p]);
-      }
-      const unsigned char* xu = xf + s * (2 * UC);
-      auto mma = [&](int p, int q, const uint32_t* o) {
-        const u32x4 xv = *reinterpret_cast<const u32x4*>(xu + 2 * (4 * PC * p + 8 * q));
-        acc = T::mfma((u32x4){o[0], o[1], o[2], o[3]}, xv, acc);
-      };
-      if (__builtin_expect(!__any(big), 1)) {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const GroupScale g = make_group(sv[p], bv[p]);
-#pragma unroll
-          for (int q = 0; q < WP; ++q) {
-            uint32_t o[4];
-            if constexpr (BITS == 4) {
-              deq4_word<DT>(W[b][p][q], g, o);
-            } else {
-              deq8_word<DT>(W[b][p][2 * q], g, o);
-              deq8_word<DT>(W[b][p][2 * q + 1], g, o + 2);
-            }
-            mma(p, q, o);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const GroupScale g = make_group(sv[p], bv[p]);
-#pragma unroll
-          for (int q = 0; q < WP; ++q) {
-            uint32_t o[4];
-            if constexpr (BITS == 4) {
-              deq_word_plain<DT, 4>(W[b][p][q], g, o);
-            } else {
-              deq_word_plain<DT, 8>(W[b][p][2 * q], g, o);
-              deq_word_plain<DT, 8>(W[b][p][2 * q + 1], g, o + 2);
-            }
-            mma(p, q, o);
-          }
+    int j = i0 / ns, s = i0 - j * ns;           // the unit computed
+    int jl = j, sl_ = s;                        // and the one loaded next
+    // the next load, which stays at the run's last unit
+    auto advance = [&](int i) {
+      if (i + 1 < i1) {
+        if (++sl_ == ns) {
+          sl_ = 0;
+          tile_at(++jl);
         }
       }
-      if (!more || sn == 0) {                   // the run's or the tile's end
-        part[(wave * 2 + j - j0) * 64 + lane] = acc;
-        acc = (f32x4){0.f, 0.f, 0.f, 0.f};
-      }
-      j = jn;
-      s = sn;
     };
-    for (int i = i0; i < i1; i += 2) {
-      step(std::integral_constant<int, 0>{}, i);
-      if (i + 1 < i1) step(std::integral_constant<int, 1>{}, i + 1);
-    }
+    // The slice's scales and biases, gate rows, then up rows, in pieces of P groups, and x:
+    // the first SB and XB pieces of each thread are read ahead of the weights.  Reads past the
+    // slice's pieces are of the last rows again, those past K leave zeros.
+    bool big = false;
+    const int rows = nt * kGluCols, g0 = s0 * GU, ng = ns * GU;
+    const int k0 = s0 * UC, ch = ns * UC / 8;   // 16-byte chunks of a row of x
+    auto x_at = [&](int i) {
+      const int m = i / ch, k = k0 + 8 * (i - m * ch);
+      const u32x4 v =
+          *reinterpret_cast<const u32x4*>(x + (int64_t)min(m, M - 1) * K + min(k, K - 8));
+      return k < K ? v : (u32x4){0, 0, 0, 0};
+    };
+    auto x_put = [&](int i, u32x4 v) {
+      const int m = i / ch;
+      if (i < M * ch) *reinterpret_cast<u32x4*>(xl + m * xs + 16 * (i - m * ch)) = v;
+    };
+    auto start = [&] {
+      tile_at(jl);
+      load(std::integral_constant<int, 0>{}, s0 + sl_);
+      advance(i0);
+      if (s0) __syncthreads();                  // the last slice's sums are read
+    };
+    auto fill = [&](auto pc) {
+      constexpr int P = decltype(pc)::value, SB = 2, XB = 2, TH = 64 * kGluWaves;
+      using V = std::conditional_t<P == 8, u32x4, uint16_t>;
+      const int per = ng / P, n = 2 * rows * per;
+      struct Piece { V s, b; };
+      auto at = [&](int i) {
+        const int q = i / per, g = g0 + (i - q * per) * P;
+        const bool up = q >= rows;
+        const int64_t o =
+            (int64_t)min(t0 * kGluCols + (up ? q - rows : q), N - 1) * G + min(g, G - P);
+        Piece v;
+        v.s = *reinterpret_cast<const V*>((up ? su : sg) + o);
+        v.b = *reinterpret_cast<const V*>((up ? bu : bg) + o);
+        return g < G ? v : Piece{};
+      };
+      auto put = [&](int i, const Piece& v) {
+        if (i >= n) return;
+        const int q = i / per;
+        const bool up = q >= rows;
+        const int k = up ? q - rows : q;
+        // row k of its matrix is row k % 8, or 8 + k % 8, of tile k / 8
+        uint32_t* d = sl + ((k >> 3) * 16 + (up ? 8 : 0) + (k & 7)) * ss + (i - q * per) * P;
+        if constexpr (P == 8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t s2 = v.s[2 * h + e], b2 = v.b[2 * h + e];
+              o[2 * e] = (s2 & 0xffffu) | b2 << 16;
+              o[2 * e + 1] = s2 >> 16 | (b2 & 0xffff0000u);
+              big |= needs_plain(T::to_f32((uint16_t)s2)) |
+                     needs_plain(T::to_f32((uint16_t)(s2 >> 16)));
+            }
+            *reinterpret_cast<u32x4*>(d + 4 * h) = o;
+          }
+        } else {
+          *d = v.s | (uint32_t)v.b << 16;
+          big |= needs_plain(T::to_f32(v.s));
+        }
+      };
+      Piece sv[SB];
+      u32x4 xv[XB];
+#pragma unroll
+      for (int u = 0; u < SB; ++u) sv[u] = at(t + u * TH);
+#pragma unroll
+      for (int u = 0; u < XB; ++u) xv[u] = x_at(t + u * TH);
+      start();
+#pragma unroll
+      for (int u = 0; u < SB; ++u) put(t + u * TH, sv[u]);
+#pragma unroll
+      for (int u = 0; u < XB; ++u) x_put(t + u * TH, xv[u]);
+#pragma unroll 4
+      for (int i = t + SB * TH; i < n; i += TH) put(i, at(i));
+    };
+    if (G % 8 == 0 && g0 % 8 == 0 && ng % 8 == 0 &&
+        (((uintptr_t)sg | (uintptr_t)bg | (uintptr_t)su | (uintptr_t)bu) & 15u) == 0)
+      fill(std::integral_constant<int, 8>{});
+    else
+      fill(std::integral_constant<int, 1>{});
+#pragma unroll 4
+    for (int i = t + 2 * 64 * kGluWaves; i < M * ch; i += 64 * kGluWaves) x_put(i, x_at(i));
+    const bool plain = __syncthreads_or(big);
+    // rows past M repeat the last one: their columns are not stored
+    const unsigned char* xu = xl + min(r, M - 1) * xs + 4 * PC * c + s * (2 * UC);
+    const uint32_t* sr = sl + (j * 16 + r) * ss + s * GU;
+    const int xwrap = ns * 2 * UC, swrap = 16 * ss - ns * GU;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f}, head = acc;
+    const int j0 = j;
+    // A SIMD's waves take turns by their progress: issued oldest first, the first ended
+    // 13 us before the last, which then waited for memory alone (28.1 against 26.6 us).
+    const int p1 = i0 + (i1 - i0) / 4, p2 = i0 + (i1 - i0) / 2, p3 = p2 + (i1 - i0) / 4;
+    auto prio = [&](int i) {
+      if (i < p1) __builtin_amdgcn_s_setprio(3);
+      else if (i < p2) __builtin_amdgcn_s_setprio(2);
+      else if (i < p3) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+    };
+    auto step = [&](auto bc, auto plainc, int i) {
+      constexpr int b = decltype(bc)::value;
+      constexpr bool PLAIN = decltype(plainc)::value;
+      load(std::integral_constant<int, (b + R - 1) % R>{}, s0 + sl_);
+      advance(i + R - 1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {             // codes (2 c + u) PC .. of the unit
+        const uint32_t sb = sr[(2 * c + u) * PC / GS];
+        const GroupScale g = make_group(T::to_f32((uint16_t)sb), T::to_f32((uint16_t)(sb >> 16)));
+        uint32_t w[4], o[WP][4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          w[d] = u ? swap_halves<false>(W[b][1][d], W[b][0][d])
+                   : swap_halves<true>(W[b][0][d], W[b][1][d]);
+#pragma unroll
+        for (int q = 0; q < WP; ++q) {
+          if constexpr (BITS == 4) {
+            if constexpr (PLAIN) deq_word_plain<DT, 4>(w[q], g, o[q]);
+            else deq4_word<DT>(w[q], g, o[q]);
+          } else {
+            if constexpr (PLAIN) {
+              deq_word_plain<DT, 8>(w[2 * q], g, o[q]);
+              deq_word_plain<DT, 8>(w[2 * q + 1], g, o[q] + 2);
+            } else {
+              deq8_word<DT>(w[2 * q], g, o[q]);
+              deq8_word<DT>(w[2 * q + 1], g, o[q] + 2);
+            }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < WP; ++q) {
+          const u32x4 xv = *reinterpret_cast<const u32x4*>(xu + 2 * (PC * u + 8 * q));
+          acc = T::mfma((u32x4){o[q][0], o[q][1], o[q][2], o[q][3]}, xv, acc);
+        }
+      }
+      xu += 2 * UC;
+      sr += GU;
+      if (++s == ns) {                          // the next tile
+        s = 0;
+        ++j;
+        xu -= xwrap;
+        sr += swrap;
+        if (i + 1 < i1) {
+          head = acc;
+          acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+        }
+      }
+    };
+    auto run = [&](auto plainc) {
+      int i = i0;
+      for (; i + R <= i1; i += R) {
+        prio(i);
+        step(std::integral_constant<int, 0>{}, plainc, i);
+        step(std::integral_constant<int, 1>{}, plainc, i + 1);
+      }
+      if (i < i1) step(std::integral_constant<int, 0>{}, plainc, i);
+    };
+    if (__builtin_expect(!plain, 1)) run(std::false_type{});
+    else run(std::true_type{});
+    // the run's last tile's sum is in acc, that of the tile before it, if there is one, in head
+    const bool two = i0 < i1 && (i1 - 1) / ns > j0;
+    __syncthreads();                            // x and the scales are read
+    part[wave * 128 + lane] = two ? head : acc;
+    if (two) part[wave * 128 + 64 + lane] = acc;
     __syncthreads();
     // wave w: tile w's sums, in the order of the runs
     if (wave < nt) {
       const int u0 = wave * ns, u1 = u0 + ns;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (ph) v = sums[wave * 64 + lane];
+      if (s0) v = sums[wave * 64 + lane];
       for (int w = 0; w < kGluWaves; ++w) {
         const int a0 = units * w / kGluWaves, a1 = units * (w + 1) / kGluWaves;
         if (a0 < u1 && a1 > u0 && a0 < a1) v += part[(w * 2 + wave - a0 / ns) * 64 + lane];
@@ -257,7 +341,7 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
   }
 }
 
-// Most LDS of a workgroup that holds x rows of one slice.
+// Most LDS of a workgroup.
 constexpr int kGluLdsMax = 160 * 1024 - 1024;
 
 template <int DT, int BITS, int GS>
@@ -268,30 +352,26 @@ int GluSkinnyLaunch<DT, BITS, GS>::run(const GluArgs& a, int64_t m0, int64_t M, 
   // one workgroup per CU, more where that would be over 16 tiles each
   const int64_t per = (tiles + (int64_t)cus * kGluTiles - 1) / ((int64_t)cus * kGluTiles);
   const int64_t wgs = tiles < cus * per ? tiles : cus * per;
-  // x in equal slices of whole units
+  // x and scales in equal slices of whole units
+  const int most = (int)((tiles + wgs - 1) / wgs);
   int64_t slice = S;
   size_t lds = 0;
   for (int64_t n = 1;; ++n) {
     slice = (S + n - 1) / n;
-    lds = (size_t)kGluPart + (n > 1 ? kGluSum : 0) + (size_t)M * glu_xstride((int)(slice * UC));
+    lds = glu_slice_bytes<BITS, GS>(M, most, (int)slice) + (slice < S ? kGluSum : 0);
     if (lds <= (size_t)kGluLdsMax) break;
   }
-  const uintptr_t any = (uintptr_t)a.sg | (uintptr_t)a.bg | (uintptr_t)a.su | (uintptr_t)a.bu;
-  const bool sv = a.K % UC == 0 && any % 4 == 0;    // a row's groups are whole dwords then
-  auto go = [&](auto svc) -> int {
-    const auto kern = &glu_skinny_kernel<DT, BITS, GS, decltype(svc)::value>;
-    static std::atomic<uint64_t> lds_set{0};
-    if (hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(kern), kGluLdsMax, lds_set))
-      return (int)e;
-    const int64_t o = m0 * a.N;
-    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * kGluWaves), lds, st,
-                       (const uint16_t*)a.x + m0 * a.K, a.wg, (const uint16_t*)a.sg,
-                       (const uint16_t*)a.bg, a.wu, (const uint16_t*)a.su, (const uint16_t*)a.bu,
-                       (uint16_t*)a.out + o, a.gf ? a.gf + o : nullptr, a.uf ? a.uf + o : nullptr,
-                       (int)M, (int)a.N, (int)a.K, a.act, (int)tiles, (int)slice);
-    return 0;
-  };
-  return sv ? go(std::true_type{}) : go(std::false_type{});
+  const auto kern = &glu_skinny_kernel<DT, BITS, GS>;
+  static std::atomic<uint64_t> lds_set{0};
+  if (hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(kern), kGluLdsMax, lds_set))
+    return (int)e;
+  const int64_t o = m0 * a.N;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * kGluWaves), lds, st,
+                     (const uint16_t*)a.x + m0 * a.K, a.wg, (const uint16_t*)a.sg,
+                     (const uint16_t*)a.bg, a.wu, (const uint16_t*)a.su, (const uint16_t*)a.bu,
+                     (uint16_t*)a.out + o, a.gf ? a.gf + o : nullptr, a.uf ? a.uf + o : nullptr,
+                     (int)M, (int)a.N, (int)a.K, a.act, (int)tiles, (int)slice);
+  return 0;
 }
 
 }  // namespace mq
