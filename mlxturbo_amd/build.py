@@ -55,9 +55,8 @@ UNITS = [("abi.hip", []), ("formats.hip", []), ("prep.hip", []), ("route.hip", [
     for dt in (0, 1) for bits in (4, 8) for gs in (32, 64, 128)
 ] + [
     # the quad kernel keeps its MFMA accumulators in VGPRs (qmv_quad.cuh)
-    ("quad.hip", [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_BITS={bits}", "-mllvm",
-                  "-amdgpu-mfma-vgpr-form"])
-    for dt in (0, 1) for bits in (4, 8)
+    (src, [f"-DMQ_INST_DT={dt}", f"-DMQ_INST_BITS={bits}", "-mllvm", "-amdgpu-mfma-vgpr-form"])
+    for src in ("quad.hip", "glu_quad.hip") for dt in (0, 1) for bits in (4, 8)
 ] + [("mx_formats.hip", [])] + [
     ("mx_skinny.hip", [f"-DMQ_INST_DT={dt}"]) for dt in (0, 1)
 ] + [

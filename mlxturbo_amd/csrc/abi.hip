@@ -990,7 +990,17 @@ int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_sca
       plan = mq::glu_wide_plan(M, N, K, bits, cus, 1);
     rc = dispatch_16<mq::GluWideLaunch>(dtype, bits, group_size, a, plan, workspace, st, &nl);
   } else {
-    for (int64_t m0 = 0; m0 < M && !rc; m0 += mq::kGluSkinnyRows) {
+    int64_t m0 = 0;
+    if (M == 1) {
+      rc = dispatch_16<mq::GluQuadLaunch>(dtype, bits, group_size, a, st);
+      if (rc == mq::kStatusUnsupported) {
+        rc = MQ_OK;
+      } else {
+        m0 = 1;
+        ++nl;
+      }
+    }
+    for (; m0 < M && !rc; m0 += mq::kGluSkinnyRows) {
       const int64_t m = M - m0 < mq::kGluSkinnyRows ? M - m0 : mq::kGluSkinnyRows;
       rc = dispatch_16<mq::GluSkinnyLaunch>(dtype, bits, group_size, a, m0, m, st);
       ++nl;

@@ -4,7 +4,7 @@
 // Sums in float over the dequantized T weights, act in float, one rounding to
 // T; with gf and uf the two sums are written as well (float, for the gradient).
 //
-// Up to 16 rows, a workgroup of 16 waves, one
+// One row runs qmv_quad.cuh's gated form.  Up to 16 rows, a workgroup of 16 waves, one
 // per CU, runs up to 16 tiles of 8 output columns.  A tile's A operand of
 // v_mfma_f32_16x16x32 is 8 rows of the gate matrix and the same 8 of the up
 // matrix, so both sums of a column are in one accumulator.
@@ -32,17 +32,10 @@
 // N=17408 K=5120, 4 bits, 25.9, 26.6 and 34.3 us for 2, 8 and 16 rows (100 MB: 20 us at the
 // rate of a copy); 8 bits 36.7, 37.4 and 44.7; N=4096 K=4096 11.4, 12.3 and 13.3.
 #pragma once
-#include "glu_launch.h"
+#include "glu_act.cuh"
 #include "stream_tile.cuh"
 
 namespace mq {
-
-// act(g), in float.
-__device__ __forceinline__ float glu_act(float g, int act) {
-  // the tanh form 0.5 g (1 + tanh(z / 2)) is g / (1 + exp(-z))
-  const float z = act == kActSilu ? g : kGeluZ * (g + kGeluCubic * g * g * g);
-  return g / (1.0f + expf(-z));
-}
 
 constexpr int kGluWaves = 16;
 constexpr int kGluTiles = 16;                   // most tiles of a workgroup

@@ -32,6 +32,13 @@ struct GluSkinnyLaunch {
   static int run(const GluArgs& a, int64_t m0, int64_t M, hipStream_t st);
 };
 
+// One row, in waves of 4 rows of either matrix (qmv_quad.cuh), one launch;
+// kStatusUnsupported where a row's scales are too many for its LDS.
+template <int DT, int BITS, int GS>
+struct GluQuadLaunch {
+  static int run(const GluArgs& a, hipStream_t st);
+};
+
 // All rows on the MFMA tile, 64 .. 256 rows by 128 columns of both matrices; with
 // plan.splits > 1 over K splits, whose float planes ws holds.
 template <int DT, int BITS, int GS>

@@ -55,7 +55,7 @@
 #pragma once
 #include <type_traits>
 
-#include "launch.h"
+#include "glu_act.cuh"
 
 namespace mq {
 
@@ -120,17 +120,38 @@ __host__ __device__ inline int quad_lds_chunks(int nI, int G, int lw, bool full)
   return whole > split ? whole : split;
 }
 
+// What a gated launch (glu_quad.hip) has besides the first matrix: the second, the two
+// sums' places (or NULL) and the activation.
+template <bool GLU>
+struct QuadGlu {};
+template <>
+struct QuadGlu<true> {
+  const uint32_t* wu;
+  const uint16_t *su, *bu;
+  float *gf, *uf;
+  int act;
+  int odd;                                      // scales or biases not 16-byte aligned
+};
+
 // Workgroups of W waves (a power of two).  The first full_wgs run W whole
 // quads each (wave w: quad W g + w, all of K); the rest run one quad each
 // (quad W full_wgs + g - full_wgs), K split over its W waves.  Dynamic LDS
 // W * 2 KB * SB (scales and biases of 4 rows x 16 SB chunks per wave; every
 // lane stores its chunks, zeros past the copy); the copy of a wave at most
 // 16 SB chunks per row; x, scales and biases 16-byte aligned.
-template <int DT, int BITS, int GS, int SB, bool LATE>
+//
+// GLU: out = act(x . W^T) * (x . Wu^T), W <= 4: each of the W waves above is two, the
+// even one on the first matrix, the odd one on the second, with the same rows and K
+// range, and the even one takes the odd one's sums from LDS.  Scales and biases at any
+// address: where one is not 16-byte aligned, the copy reads them one by one.
+// N=17408 K=5120, 4 bits, 20.4 us from memory (glu.cuh's 16-row workgroups 26.3), 8 bits 31.8
+// (37.2); N=4096 K=4096 6.4 (10.4), N=1024 K=2048 3.4 (8.5): the rate of the one-matrix
+// launch of 2 N rows.
+template <int DT, int BITS, int GS, int SB, bool LATE, bool GLU = false>
 __global__ __launch_bounds__(64 * kQuadMaxKS) void qmv_quad_kernel(
     const uint16_t* __restrict__ x, const uint32_t* __restrict__ w,
     const uint16_t* __restrict__ scales, const uint16_t* __restrict__ biases,
-    uint16_t* __restrict__ out, int N, int K, int full_wgs) {
+    uint16_t* __restrict__ out, int N, int K, int full_wgs, QuadGlu<GLU> glu) {
   using Q = QuadGeom<BITS, GS>;
   using T = T16<DT>;
   constexpr int D = kQuadDepth;
@@ -142,8 +163,16 @@ __global__ __launch_bounds__(64 * kQuadMaxKS) void qmv_quad_kernel(
 
   // (the K split is a power of two, so its divisions are scalar shifts)
   const int lane = threadIdx.x & 63;
-  const int lw = __builtin_ctz(blockDim.x >> 6);
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lw = __builtin_ctz(blockDim.x >> 6) - GLU;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wid = wave >> GLU;
+  if constexpr (GLU) {
+    if (wave & 1) {
+      w = glu.wu;
+      scales = glu.su;
+      biases = glu.bu;
+    }
+  }
   const bool split = (int)blockIdx.x >= full_wgs;
   const int lks = split ? lw : 0;
   const int KS = 1 << lks;
@@ -169,7 +198,7 @@ __global__ __launch_bounds__(64 * kQuadMaxKS) void qmv_quad_kernel(
   // branch, behind the weight loads.
   const int CH = quad_sb_chunks<BITS, GS>(nmax, quad_tight<BITS, GS>(G, lks));
   constexpr int CS = 16 * SB;                      // LDS chunks per row (every lane stores)
-  lds8* ls = (lds8*)qq_smem + wid * (2 * 4 * 16 * CS);
+  lds8* ls = (lds8*)qq_smem + wave * (2 * 4 * 16 * CS);
   u32x4 sq[SB], bq[SB];
   const int cr = lane & 3, cc0 = lane >> 2;
   // (32-bit offsets: the launch keeps the arrays below 2^31 bytes)
@@ -179,11 +208,14 @@ __global__ __launch_bounds__(64 * kQuadMaxKS) void qmv_quad_kernel(
   const auto rs = make_rsrc(scales, sbytes);
   const auto rb = make_rsrc(biases, sbytes);
   uint32_t go[SB];
+  bool odd = false;
+  if constexpr (GLU) odd = glu.odd != 0;
 #pragma unroll
   for (int u = 0; u < SB; ++u) {
     go[u] = cc0 + 16 * u < CH && cr < nrows ? ca0 + 256u * u : 0x80000000u;
-    sq[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, go[u], 0, 0);
-    bq[u] = __builtin_amdgcn_raw_buffer_load_b128(rb, go[u], 0, 0);
+    const uint32_t o = odd ? 0x80000000u : go[u];
+    sq[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0);
+    bq[u] = __builtin_amdgcn_raw_buffer_load_b128(rb, o, 0, 0);
   }
   // this lane's scale at instruction s0: row j, group s0 GPI + gb
   const int gb = 16 * bb * (8 / BITS) / GS;
@@ -279,7 +311,7 @@ __global__ __launch_bounds__(64 * kQuadMaxKS) void qmv_quad_kernel(
   // so no copy load waits behind this branch)
 #pragma unroll
   for (int u = 0; u < SB; ++u) {
-    if (go[u] < sbytes && go[u] + 16 > sbytes) {
+    if (go[u] < sbytes && (odd || go[u] + 16 > sbytes)) {
       u32x4 sv, bv;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -388,6 +420,23 @@ __global__ __launch_bounds__(64 * kQuadMaxKS) void qmv_quad_kernel(
                                                              0x128, 0xf, 0xf, false));
   v += __shfl_xor(v, 16);
   v += __shfl_xor(v, 32);
+  if constexpr (GLU) {
+    if (bb == 0) red[wave][j] = v;
+    __syncthreads();
+    if (kp == 0 && !(wave & 1) && lane < nrows) {
+      float g = red[wave][lane], u = red[wave + 1][lane];
+      for (int q = 1; q < KS; ++q) {
+        g += red[2 * q][lane];
+        u += red[2 * q + 1][lane];
+      }
+      out[row0 + lane] = T::round1(glu_act(g, glu.act) * u);
+      if (glu.gf) {
+        glu.gf[row0 + lane] = g;
+        glu.uf[row0 + lane] = u;
+      }
+    }
+    return;
+  }
   if (KS == 1) {
     if (bb == 0 && j < nrows) out[row0 + j] = T::round1(v);
     return;
@@ -465,8 +514,56 @@ int QuadLaunch<DT, BITS, GS>::run(const void* x, const uint32_t* w, const void* 
                                : qmv_quad_kernel<DT, BITS, GS, 2, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * W), lds, st, (const uint16_t*)x, w,
                      (const uint16_t*)s, (const uint16_t*)b, (uint16_t*)out, (int)N, (int)K,
-                     (int)full_wgs);
+                     (int)full_wgs, QuadGlu<false>{});
   ++*nlaunch;
+  return 0;
+}
+
+// The gated launch: two waves per quad and K slice, so splits as of twice the quads.
+template <int DT, int BITS, int GS>
+int GluQuadLaunch<DT, BITS, GS>::run(const GluArgs& a, hipStream_t st) {
+  auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  if (!a16(a.x)) return kStatusUnsupported;
+  const int odd = !a16(a.sg) || !a16(a.bg) || !a16(a.su) || !a16(a.bu);
+  const int64_t N = a.N, K = a.K;
+  if (N * (K / GS) * 2 >= ((int64_t)1 << 31)) return kStatusUnsupported;
+  const int cus = device_cu_count();
+  const int G = (int)(K / GS);
+  const int nI = (int)((K * BITS / 8 + 255) / 256);
+  const int64_t quads = (N + 3) / 4;
+  constexpr int kMaxW = kQuadMaxKS / 2;
+  int W = quad_ks(8 * quads, K, BITS, cus);
+  if (W > kMaxW) W = kMaxW;
+  int64_t full_wgs = 0, wgs = quads;
+  if (W == 1 && quad_lds_chunks<BITS, GS>(nI, G, 0, false) <= 16 * kQuadMaxSb) {
+    const int Wt = quad_tail_split(8 * quads, K, BITS, cus);
+    const int64_t L = quads % (2 * (int64_t)cus);
+    if (Wt > 1 && (quads - L) % Wt == 0) {
+      W = Wt;
+      full_wgs = (quads - L) / W;
+      wgs = full_wgs + L;
+    }
+  }
+  int CHW = quad_lds_chunks<BITS, GS>(nI, G, __builtin_ctz(W), full_wgs > 0);
+  if (full_wgs == 0) {
+    while (W < kMaxW && CHW > 16 * kQuadMaxSb) {
+      W *= 2;
+      CHW = quad_lds_chunks<BITS, GS>(nI, G, __builtin_ctz(W), false);
+    }
+  }
+  if (CHW > 16 * kQuadMaxSb) return kStatusUnsupported;
+  const int SBn = CHW <= 16 ? 1 : 2;
+  const size_t lds = (size_t)2 * W * 2 * 4 * 16 * 16 * SBn;
+  const bool late = (full_wgs > 0 ? nI : (nI + W - 1) / W) >= 4;
+  auto kern = SBn == 1 ? (late ? qmv_quad_kernel<DT, BITS, GS, 1, true, true>
+                               : qmv_quad_kernel<DT, BITS, GS, 1, false, true>)
+                       : (late ? qmv_quad_kernel<DT, BITS, GS, 2, true, true>
+                               : qmv_quad_kernel<DT, BITS, GS, 2, false, true>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(128 * W), lds, st, (const uint16_t*)a.x, a.wg,
+                     (const uint16_t*)a.sg, (const uint16_t*)a.bg, (uint16_t*)a.out, (int)N, (int)K,
+                     (int)full_wgs,
+                     QuadGlu<true>{a.wu, (const uint16_t*)a.su, (const uint16_t*)a.bu, a.gf, a.uf,
+                                   a.act, odd});
   return 0;
 }
 
