@@ -131,37 +131,63 @@ def _glu_grad(d, g, u, flat, act: int, group_size: int, bits: int) -> torch.Tens
     return dx
 
 
+def _versions(ts) -> list:
+    return [None if t.is_inference() else t._version for t in ts]
+
+
+def _constants(ctx, ts) -> None:
+    """Keeps the weights for the backward pass.  They are constants, so they go past the
+    engine's saved tensors, whose packing and unpacking cost 2 us each a step; like those they
+    may not have changed by then."""
+    ctx.flat, ctx.versions = ts, _versions(ts)
+
+
+def _same_constants(ctx):
+    if ctx.versions != _versions(ctx.flat):
+        raise RuntimeError("a quantized weight needed for the gradient has been modified by an "
+                           "inplace operation since the forward pass")
+    return ctx.flat
+
+
+def _first_order(backward):
+    """``backward`` of kernels, which has no gradient of its own: asked for one
+    (create_graph) it refuses a second pass, else it runs as it is."""
+    twice = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, d: (twice if torch.is_grad_enabled() else backward)(ctx, d)
+
+
 class _Glu(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, act, group_size, bits, *flat):
+    def forward(ctx, x, flat, act, group_size, bits):
         r = _glu_forward(x, flat, act, group_size, bits, True)
         if r is None:
             raise NotImplementedError("quantized_glu: no kernel of these sizes for the gradient")
         out, g, u = r
         ctx.args = act, group_size, bits
-        ctx.save_for_backward(g, u, *flat)
+        ctx.save_for_backward(g, u)
+        _constants(ctx, flat)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, d):
-        g, u, *flat = ctx.saved_tensors
-        return (_glu_grad(d, g, u, flat, *ctx.args), *[None] * 9)
+        g, u = ctx.saved_tensors
+        return _glu_grad(d, g, u, _same_constants(ctx), *ctx.args), None, None, None, None
 
 
 class _Matmul(torch.autograd.Function):
     """quantized_matmul of ``(M, K)`` rows by its own kernels, with x's gradient."""
 
     @staticmethod
-    def forward(ctx, x, w, scales, biases, group_size, bits):
+    def forward(ctx, x, flat, group_size, bits):
         ctx.args = group_size, bits
-        ctx.save_for_backward(w, scales, biases)
-        return ops.quantized_matmul(x, w, scales, biases, True, group_size, bits)
+        _constants(ctx, flat)
+        return ops.quantized_matmul(x, *flat, True, group_size, bits)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, d):
-        return (matmul_grad(d, *ctx.saved_tensors, *ctx.args), *[None] * 5)
+        return matmul_grad(d, *_same_constants(ctx), *ctx.args), None, None, None
 
 
 def quantized_matmul_differentiable(x, w, scales, biases, group_size: int, bits: int):
@@ -171,8 +197,8 @@ def quantized_matmul_differentiable(x, w, scales, biases, group_size: int, bits:
         raise NotImplementedError("quantized_matmul: scales and biases are constants here; "
                                   "gradients go to x")
     note_leaf(x)
-    y = _Matmul.apply(x.reshape(-1, x.shape[-1]), ops._aligned(w), ops._aligned(scales),
-                      ops._aligned(biases), group_size, bits)
+    flat = [ops._aligned(t) for t in (w, scales, biases)]
+    y = _Matmul.apply(x.reshape(-1, x.shape[-1]), flat, group_size, bits)
     return y.reshape(*x.shape[:-1], w.shape[0])
 
 
@@ -247,7 +273,7 @@ def quantized_glu(x: torch.Tensor, gate, up, activation: str = "silu",
     flat = [ops._aligned(t) for t in (*gate, *up)]
     if grad:
         note_leaf(x)
-        y = _Glu.apply(ops._aligned(x2), ACTIVATIONS[activation], group_size, bits, *flat)
+        y = _Glu.apply(ops._aligned(x2), flat, ACTIVATIONS[activation], group_size, bits)
         return y.reshape(*lead, N)
     r = _glu_forward(ops._aligned(x2), flat, ACTIVATIONS[activation], group_size, bits, False)
     if r is None:
