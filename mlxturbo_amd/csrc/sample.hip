@@ -18,7 +18,10 @@
 //
 // One row of 248320 16-bit words is half a megabyte: latency bounds a few rows, so a
 // row is spread over workgroups (chunks of its tiles, up to 1024 of 64 granules or
-// more), and the passes are launches for all rows whatever their settings:
+// more), and the passes are launches for all rows whatever their settings.  (us of the
+// steps, 248320 bf16 words: one row with k and p 3.2, 7.1 and 10.9 for 3 and 4; 64 rows of
+// mixed settings 10.6, at 3 TB/s of logits, 22.8, of which 13 are the double arithmetic
+// of the masses, 18.3 and 16.2.)
 //   1 each tile's first word.  Where k tiles hold a word, the k-th largest of their
 //     first words is no larger than the k-th largest word: a bound (step 2 finds it)
 //     above which lie few more than k words;
@@ -28,8 +31,9 @@
 //   3 rows with k or p: a list of the words among which the cut falls: from the bound
 //     on; up to the bin that holds the k-th word; or those of the bin in which p is
 //     reached, and each tile's mass in the bins before it;
-//   4 the list sorted, the cut by a scan of its masses, and the word that u points at:
-//     among the kept words in index order (k), or in the tile that holds it.
+//   4 rows with k: the list sorted, the cut by a scan of its masses, and the word that u
+//     points at among the kept words in index order.  Others: the cut by the list's
+//     masses, and the word in the tile that u points at.
 // Few workgroups (512) run 3 and 4 as one launch: the row's last one to have listed
 // goes on.  A list of more than 4096 words (many equal logits, k in the thousands)
 // overflows: step 4 then selects by radix over the row.
@@ -150,8 +154,8 @@ __device__ const double kExpTable[64] = {
 // exp(x) for -40 < x <= 0, by table (P. T. P. Tang, Table-driven implementation of the
 // exponential function in IEEE floating-point arithmetic, 1989): x = k ln 2 / 64 + r,
 // exp(x) = 2^(k / 64) (1 + p(r)), |r| < 0.0055, p to r^5 / 120 (r^6 / 720 < 2^-54).
-// Half the instructions of the library's, which has all arguments to answer for: 64
-// rows of 248320 words, masses MEASURED.
+// Half the instructions of the library's, which has all arguments to answer for: the
+// masses of 64 rows of 248320 words 29 us for 33.
 __device__ __forceinline__ double exp_of(double x, const double* table) {
   const double kd0 = __builtin_fma(x, 0x1.71547652b82fep+6, 0x1.8p52);
   const int k = (int)(uint32_t)__double_as_longlong(kd0);
@@ -507,10 +511,18 @@ __device__ __forceinline__ void list_words(const SampleArgs& a, const RowView<DT
   const float per = kBinsPerNat / set.T;
   const int t = threadIdx.x, tiles = row_tiles(row, a.tile), i1 = chunk_at(tiles, c + 1, C);
   for (int i = chunk_at(tiles, c, C) + (t >> 6); i < i1; i += kThreads / 64) {
+    // a tile whose first word lies behind the cut has nothing to list or add
+    const u64 top = s.tops[i];
+    if (!top || (cut.bin < 0 ? key_value(top) < cut.low
+                             : bin_of(key_value(top), mass.m, per) > cut.bin)) {
+      if (!set.by_k && (t & 63) == 0) put_agent(&s.csum[i], (u64)0);
+      continue;
+    }
     u64 sum = 0;
     each_granule(row, a.tile, i, [&](int g) {
       float v[RowView<DT>::E];
       row.load(g, v);
+      uint32_t mine = 0;                        // its words that are listed
 #pragma unroll
       for (int e = 0; e < RowView<DT>::E; ++e) {
         bool listed = v[e] >= cut.low;
@@ -523,11 +535,25 @@ __device__ __forceinline__ void list_words(const SampleArgs& a, const RowView<DT
               sum += mass.of(w);
           }
         }
-        if (listed) {
-          const uint32_t at = atomicAdd(&s.count[kBins], 1u);
-          if (at < kList) put_agent(&s.list[at], order_key(v[e], row.first(g) + e));
-        }
+        mine |= (uint32_t)listed << e;
       }
+      // the wave's places on the list by one atomic, whose answer takes a microsecond
+      if (!__ballot(mine != 0)) return;
+      uint32_t n = 0, before[RowView<DT>::E];
+#pragma unroll
+      for (int e = 0; e < RowView<DT>::E; ++e) {
+        const u64 b = __ballot(mine >> e & 1);
+        before[e] = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32),
+                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        n += __popcll(b);
+      }
+      uint32_t at = 0;
+      if ((t & 63) == (int)__builtin_ctzll(__ballot(true))) at = atomicAdd(&s.count[kBins], n);
+      at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+      for (int e = 0; e < RowView<DT>::E; ++e)
+        if ((mine >> e & 1) && at + before[e] < kList)
+          put_agent(&s.list[at + before[e]], order_key(v[e], row.first(g) + e));
     });
     if (!set.by_k) {
       sum = wave_sum(sum);
@@ -727,6 +753,76 @@ __device__ __forceinline__ void sort_falling(u64* keys, int n, u64* tmp, uint32_
   __syncthreads();
 }
 
+// Of n keys, the last in falling order before which the mass (from `before` on) is less
+// than goal, up to which it is not: by the 11 highest bits in which those still asked
+// about differ (bins: 2048 masses), until one is left.  Keys of a bin of a p row have
+// few values, and differ in the index's 18 bits: three rounds of 1.5 us, where sorting
+// 2048 took 16.
+__device__ __forceinline__ u64 cut_of_list(const u64* keys, int n, u64* bins, const Mass& mass,
+                                           u64 before, double goal, u64* tmp, u64* res) {
+  const int t = threadIdx.x;
+  u64 prefix = 0;
+  int top = 64;                                 // asked about: keys with prefix's bits from top on
+  auto asked = [&](u64 key) { return top == 64 || key >> top == prefix >> top; };
+#pragma unroll 1
+  for (;;) {
+    u64 ones = 0, zeros = 0;                    // bits that are one, or zero, in any
+#pragma unroll 1
+    for (int i = t; i < n; i += kThreads) {
+      const u64 key = keys[i];
+      if (asked(key)) {
+        ones |= key;
+        zeros |= ~key;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+      ones |= __shfl_xor(ones, o);
+      zeros |= __shfl_xor(zeros, o);
+    }
+    if ((t & 63) == 0) {
+      tmp[t >> 6] = ones;
+      tmp[kThreads / 64 + (t >> 6)] = zeros;
+    }
+    for (int i = t; i < kBins; i += kThreads) bins[i] = 0;
+    if (t == 0) res[0] = res[1] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+      ones |= tmp[w];
+      zeros |= tmp[kThreads / 64 + w];
+    }
+    const u64 differ = ones & zeros;
+    if (!differ) return ones;                   // one key
+    const int high = 63 - __builtin_clzll(differ), shift = high > 10 ? high - 10 : 0;
+#pragma unroll 1
+    for (int i = t; i < n; i += kThreads) {
+      const u64 key = keys[i];
+      if (asked(key)) atomicAdd(&bins[kBins - 1 - (key >> shift & (kBins - 1))],
+                                mass.of(mass.w(key_value(key))));
+    }
+    __syncthreads();
+    u64 v[kBinsPer], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < kBinsPer; ++i) sum += v[i] = bins[t * kBinsPer + i];
+    u64 b = before + block_scan(sum, all, tmp);
+#pragma unroll
+    for (int i = 0; i < kBinsPer; ++i) {
+      if ((double)b < goal && (double)(b + v[i]) >= goal) {
+        res[0] = (u64)(kBins - 1 - (t * kBinsPer + i));
+        res[1] = b;
+      }
+      b += v[i];
+    }
+    __syncthreads();
+    // the bits above the 11 are those of all that were asked about
+    prefix = (ones >> shift & ~(u64)(kBins - 1) | res[0]) << shift;
+    before = res[1];
+    top = shift;
+    __syncthreads();
+  }
+}
+
 // LIST: step 3 as well, by C workgroups per row; else one per row.
 template <int DT, bool LIST>
 __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, void* ws, int C) {
@@ -776,10 +872,27 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   Kept kept{first, 0, min_p};
   if (list && whole) {
     for (int i = t; i < n; i += kThreads) keys[i] = get_agent(&s.list[i]);
+    __syncthreads();
+  }
+  if (list && whole && !set.by_k) {
+    // the bins before the cut's are in the tiles' sums; its kept words join theirs (words
+    // of the bins before it precede the last word that p keeps)
+    kept.end = cut_of_list(keys, n, masses, mass, cut.before, (double)set.p * (double)cut.total,
+                           tmp, res);
+    for (int i = t; i < tiles; i += kThreads) part[i] = get_agent(&s.csum[i]);
+    __syncthreads();
+#pragma unroll 1
+    for (int i = t; i < n; i += kThreads) {
+      const double w = mass.w(key_value(keys[i]));
+      if (kept(keys[i], w))
+        atomicAdd(&part[(key_index(keys[i]) + row.off) / RowView<DT>::E >> a.tile], mass.of(w));
+    }
+    __syncthreads();
+  } else if (list && whole) {
     sort_falling(keys, n, masses, hc);
     // the kept words are a prefix: of k, of those before which p's mass is not reached,
     // and of those of min_p
-    const int nk = set.by_k && set.k < n ? set.k : n;
+    const int nk = set.k < n ? set.k : n;
     uint32_t of_p = 0, of_min = 0;
 #pragma unroll 1
     for (int i = t; i < nk; i += kThreads) {
@@ -797,8 +910,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     };
     int per = (nk + kThreads - 1) / kThreads;
     u64 total;
-    u64 b = scan(nk, per, total) + (set.by_k ? 0 : cut.before);
-    const double goal = (double)set.p * (double)(set.by_k ? total : cut.total);
+    u64 b = scan(nk, per, total);
+    const double goal = (double)set.p * (double)total;
 #pragma unroll 1
     for (int i = t * per; i < (t + 1) * per && i < nk; ++i) {
       of_p += !set.by_p || (double)b < goal || keys[i] == first;
@@ -807,35 +920,23 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     const u64 both = block_sum((u64)of_p << 32 | of_min, tmp);
     const int kept_p = (int)(both >> 32);
     const int m = min(kept_p, (int)(uint32_t)both);
-    if (set.by_k) {
-      // the kept words in index order (the index, complemented in the key already, above
-      // the value), and the one whose share holds the place
+    // the kept words in index order (the index, complemented in the key already, above
+    // the value), and the one whose share holds the place
 #pragma unroll 1
-      for (int i = t; i < m; i += kThreads) keys[i] = keys[i] << 32 | keys[i] >> 32;
-      sort_falling(keys, m, masses, hc);
+    for (int i = t; i < m; i += kThreads) keys[i] = keys[i] << 32 | keys[i] >> 32;
+    sort_falling(keys, m, masses, hc);
 #pragma unroll 1
-      for (int i = t; i < m; i += kThreads)
-        masses[i] = mass.of(mass.w(key_value(keys[i] << 32)));
-      __syncthreads();
-      per = (m + kThreads - 1) / kThreads;
-      b = scan(m, per, S);
-      place_at = place(set.u, S);
+    for (int i = t; i < m; i += kThreads)
+      masses[i] = mass.of(mass.w(key_value(keys[i] << 32)));
+    __syncthreads();
+    per = (m + kThreads - 1) / kThreads;
+    b = scan(m, per, S);
+    place_at = place(set.u, S);
 #pragma unroll 1
-      for (int i = t * per; i < (t + 1) * per && i < m; ++i) {
-        if (b <= place_at && place_at < b + masses[i])
-          pick = Pick{key_index(keys[i] >> 32), key_value(keys[i] << 32)};
-        b += masses[i];
-      }
-    } else {
-      // the bins before the cut's are in the tiles' sums; its kept words join theirs
-      for (int i = t; i < tiles; i += kThreads) part[i] = get_agent(&s.csum[i]);
-      __syncthreads();
-#pragma unroll 1
-      for (int i = t; i < m; i += kThreads)
-        atomicAdd(&part[(key_index(keys[i]) + row.off) / RowView<DT>::E >> a.tile], masses[i]);
-      // up to the last word that p keeps; words of the bins before it precede it
-      kept.end = kept_p ? keys[kept_p - 1] : ~0ull;
-      __syncthreads();
+    for (int i = t * per; i < (t + 1) * per && i < m; ++i) {
+      if (b <= place_at && place_at < b + masses[i])
+        pick = Pick{key_index(keys[i] >> 32), key_value(keys[i] << 32)};
+      b += masses[i];
     }
   } else if (list) {
     // too many to list: the cut by radix over the row
