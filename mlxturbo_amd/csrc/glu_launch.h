@@ -50,6 +50,10 @@ inline bool glu_wide_eligible(int64_t M, int64_t K) {
   return K % 64 == 0 && K * 2 * 256 < ((int64_t)1 << 31) && M <= ((int64_t)65535) * 64;
 }
 
+// Floats of a row of a split's plane: whole eights, so that planes are written and summed
+// four columns at a time whatever N is (N=9001, 45 rows: 5.2 us a sum before).
+__host__ __device__ inline int64_t glu_plane(int64_t N) { return (N + 7) / 8 * 8; }
+
 inline WidePlan glu_wide_plan(int64_t M, int64_t N, int64_t K, int bits, int cus, int max_splits) {
   return wide_plan(M, 2 * N, K, bits, cus, max_splits);
 }
@@ -63,7 +67,7 @@ inline bool glu_wide_route(int64_t M, int64_t N, int64_t K) {
 inline size_t glu_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int cus) {
   if (!glu_wide_route(M, N, K)) return 0;
   const WidePlan p = glu_wide_plan(M, N, K, bits, cus, 16);
-  return p.splits > 1 ? (size_t)p.splits * 2 * (size_t)M * (size_t)N * sizeof(float) : 0;
+  return p.splits > 1 ? (size_t)p.splits * 2 * (size_t)M * (size_t)glu_plane(N) * sizeof(float) : 0;
 }
 
 // ---- gradients past the weights ---------------------------------------------

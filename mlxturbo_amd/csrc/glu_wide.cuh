@@ -10,7 +10,7 @@ namespace mq {
 
 // Grid (ceil(N / 128), ceil(M / BM), splits), 256 threads; ranges as in dense.cuh.
 // part: split z's sums of its share of the k-steps (whole U) go to the float planes
-// part[2 z] (gate) and part[2 z + 1] (up), [M, N], for glu_reduce_kernel; else
+// part[2 z] (gate) and part[2 z + 1] (up), [M, glu_plane(N)], for glu_reduce_kernel; else
 // (splits == 1) out = act(gate) * up, and the sums to gf and uf where they are given.
 template <int DT, int BITS, int GS, int BM, int U>
 __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void glu_wide_kernel(
@@ -34,14 +34,14 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void glu_wide_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const auto xr = wide_rsrc(x + (int64_t)m0 * K, (int64_t)mrows * K * 2);
   auto xrow_off = [&](int r) { return (uint32_t)min(r, mrows - 1) * (uint32_t)K * 2u; };
-  const int64_t MN = (int64_t)M * N;
-  float* fg = part ? part + 2 * z * MN : gf;
-  float* fu = part ? part + (2 * z + 1) * MN : uf;
+  const int64_t ld = part ? glu_plane(N) : N;   // of the sums' rows
+  float* fg = part ? part + 2 * z * M * ld : gf;
+  float* fu = part ? part + (2 * z + 1) * M * ld : uf;
   const bool vec = N % 8 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)fg % 16 == 0 &&
                    (uintptr_t)fu % 16 == 0;
-  // four columns of both sums
+  // four columns of both sums (of planes: up to the padding)
   auto put_sums = [&](int64_t o, int c, const f32x4& g, const f32x4& u) {
-    if (vec) {
+    if (part || vec) {
       if (c < ncols) {
         *reinterpret_cast<f32x4*>(fg + o) = g;
         *reinterpret_cast<f32x4*>(fu + o) = u;
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void glu_wide_kernel(
       const int c = 32 * wave + 8 * q + 4 * h;
       const int64_t o = (int64_t)(m0 + r) * N + n0 + c;
       const f32x4 gq = quarter(g, q), uq = quarter(u, q);
-      if (fg) put_sums(o, c, gq, uq);
+      if (fg) put_sums((m0 + r) * ld + n0 + c, c, gq, uq);
       if (values) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -130,43 +130,46 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void glu_wide_kernel(
 }
 
 // out = act(sum of the gate planes) * (sum of the up planes), in split order; four
-// elements per thread, grid ceil(M * N / 1024), 256 threads.  VEC: M * N in whole
-// fours, out 8-byte and gf and uf 16-byte aligned.
+// elements of a row per thread, quads = M * glu_plane(N) / 4 of them, 256 threads.  VEC: N in
+// whole eights, out 8-byte and gf and uf 16-byte aligned.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void glu_reduce_kernel(const float* __restrict__ part,
                                                          uint16_t* __restrict__ out,
                                                          float* __restrict__ gf,
-                                                         float* __restrict__ uf, int64_t MN,
-                                                         int splits, int act) {
-  const int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if constexpr (VEC) {
-    if (i0 >= MN) return;
-    f32x4 g = *reinterpret_cast<const f32x4*>(part + i0);
-    f32x4 u = *reinterpret_cast<const f32x4*>(part + MN + i0);
-    for (int z = 1; z < splits; ++z) {
-      g += *reinterpret_cast<const f32x4*>(part + 2 * z * MN + i0);
-      u += *reinterpret_cast<const f32x4*>(part + (2 * z + 1) * MN + i0);
-    }
-    float v[4];
+                                                         float* __restrict__ uf, uint32_t quads,
+                                                         int N, int splits, int act) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= quads) return;
+  const f32x4* p = reinterpret_cast<const f32x4*>(part) + i;
+  const int64_t plane = quads;
+  f32x4 g = p[0], u = p[plane];
+  for (int z = 1; z < splits; ++z) {
+    g += p[2 * z * plane];
+    u += p[(2 * z + 1) * plane];
+  }
+  float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = glu_act(g[e], act) * u[e];
-    *reinterpret_cast<u32x2*>(out + i0) =
+  for (int e = 0; e < 4; ++e) v[e] = glu_act(g[e], act) * u[e];
+  if constexpr (VEC) {
+    const int64_t o = 4 * (int64_t)i;
+    *reinterpret_cast<u32x2*>(out + o) =
         (u32x2){T16<DT>::pack2(v[0], v[1]), T16<DT>::pack2(v[2], v[3])};
     if (gf) {
-      *reinterpret_cast<f32x4*>(gf + i0) = g;
-      *reinterpret_cast<f32x4*>(uf + i0) = u;
+      *reinterpret_cast<f32x4*>(gf + o) = g;
+      *reinterpret_cast<f32x4*>(uf + o) = u;
     }
   } else {
-    for (int64_t i = i0; i < i0 + 4 && i < MN; ++i) {
-      float g = part[i], u = part[MN + i];
-      for (int z = 1; z < splits; ++z) {
-        g += part[2 * z * MN + i];
-        u += part[(2 * z + 1) * MN + i];
-      }
-      out[i] = T16<DT>::round1(glu_act(g, act) * u);
-      if (gf) {
-        gf[i] = g;
-        uf[i] = u;
+    const uint32_t per = (uint32_t)glu_plane(N) / 4, r = i / per;
+    const int c = 4 * (int)(i - r * per);
+    const int64_t o = (int64_t)r * N + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (c + e < N) {
+        out[o + e] = T16<DT>::round1(v[e]);
+        if (gf) {
+          gf[o + e] = g[e];
+          uf[o + e] = u[e];
+        }
       }
     }
   }
@@ -200,12 +203,12 @@ int GluWideLaunch<DT, BITS, GS>::run(const GluArgs& a, const WidePlan& plan, voi
   }
   *nlaunch += 1;
   if (part) {
-    const int64_t MN = a.M * a.N;
-    const bool vec = MN % 4 == 0 && (uintptr_t)a.out % 8 == 0 &&
+    const uint32_t quads = (uint32_t)(a.M * glu_plane(a.N) / 4);
+    const bool vec = a.N % 8 == 0 && (uintptr_t)a.out % 8 == 0 &&
                      (((uintptr_t)a.gf | (uintptr_t)a.uf) & 15u) == 0;
     auto reduce = [&](auto kern) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)((MN + 1023) / 1024)), dim3(256), 0, st, part,
-                         (uint16_t*)a.out, a.gf, a.uf, MN, plan.splits, a.act);
+      hipLaunchKernelGGL(kern, dim3((quads + 255) / 256), dim3(256), 0, st, part,
+                         (uint16_t*)a.out, a.gf, a.uf, quads, (int)a.N, plan.splits, a.act);
     };
     if (vec) reduce(glu_reduce_kernel<DT, true>);
     else reduce(glu_reduce_kernel<DT, false>);
