@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -85,31 +86,26 @@ def _filtered(stderr: str) -> str:
 def build(verbose: bool = False) -> str:
     compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
     with tempfile.TemporaryDirectory(prefix="mq_build_") as tmpdir:
-        probe_cmd = [hipcc(), *HIPCC_FLAGS, "-o", PROBE_OUT + ".tmp", PROBE_SRC]
-        if verbose:
-            print(" ".join(probe_cmd), flush=True)
-        probe = subprocess.Popen(probe_cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE,
-                                 text=True)
-        procs = []
+        cmds = [[hipcc(), *HIPCC_FLAGS, "-o", PROBE_OUT + ".tmp", PROBE_SRC]]
+        objs = []
         for i, (src, defs) in enumerate(UNITS):
-            obj = os.path.join(tmpdir, f"unit{i}.o")
-            cmd = [hipcc(), *compile_flags, *defs, "-c", "-o", obj, os.path.join(CSRC, src)]
+            objs.append(os.path.join(tmpdir, f"unit{i}.o"))
+            cmds.append([hipcc(), *compile_flags, *defs, "-c", "-o", objs[-1],
+                         os.path.join(CSRC, src)])
+
+        def run(cmd):
             if verbose:
                 print(" ".join(cmd), flush=True)
-            procs.append((obj, cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE,
-                                                     stderr=subprocess.PIPE, text=True)))
-        objs = []
+            return subprocess.run(cmd, capture_output=True, text=True)
+
+        # one unit per CPU at a time (each holds a compiler's memory)
         failed = []
-        for obj, cmd, proc in procs:
-            _, err = proc.communicate()
-            if proc.returncode != 0:
-                failed.append(f"{' '.join(cmd)}\n{_filtered(err)}")
-            elif verbose and _filtered(err).strip():
-                print(_filtered(err), file=sys.stderr)
-            objs.append(obj)
-        _, err = probe.communicate()
-        if probe.returncode != 0:
-            failed.append(f"{' '.join(probe_cmd)}\n{_filtered(err)}")
+        with ThreadPoolExecutor(max(1, len(os.sched_getaffinity(0)))) as pool:
+            for cmd, res in zip(cmds, pool.map(run, cmds)):
+                if res.returncode != 0:
+                    failed.append(f"{' '.join(cmd)}\n{_filtered(res.stderr)}")
+                elif verbose and _filtered(res.stderr).strip():
+                    print(_filtered(res.stderr), file=sys.stderr)
         if failed:
             raise RuntimeError("hipcc failed:\n" + "\n\n".join(failed))
         os.replace(PROBE_OUT + ".tmp", PROBE_OUT)

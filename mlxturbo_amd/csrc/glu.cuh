@@ -188,8 +188,8 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
               const uint32_t s2 = v.s[2 * h + e], b2 = v.b[2 * h + e];
               o[2 * e] = (s2 & 0xffffu) | b2 << 16;
               o[2 * e + 1] = s2 >> 16 | (b2 & 0xffff0000u);
-              big |= needs_plain(T::to_f32((uint16_t)s2)) |
-                     needs_plain(T::to_f32((uint16_t)(s2 >> 16)));
+              big |= needs_plain(T::to_f32((uint16_t)s2));
+              big |= needs_plain(T::to_f32((uint16_t)(s2 >> 16)));
             }
             *reinterpret_cast<u32x4*>(d + 4 * h) = o;
           }

@@ -816,7 +816,7 @@ __device__ __forceinline__ u64 cut_of_list(const u64* keys, int n, u64* bins, co
     }
     __syncthreads();
     // the bits above the 11 are those of all that were asked about
-    prefix = (ones >> shift & ~(u64)(kBins - 1) | res[0]) << shift;
+    prefix = ((ones >> shift & ~(u64)(kBins - 1)) | res[0]) << shift;
     before = res[1];
     top = shift;
     __syncthreads();

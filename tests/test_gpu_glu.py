@@ -414,3 +414,85 @@ def test_streams_at_once():
                 got[i].append(mq.quantized_glu(x, gate, up))
     torch.cuda.synchronize()
     assert all(torch.equal(h, want[i]) for i in range(2) for h in got[i])
+
+
+# One row: waves of whole quads and of split ones (more quads than SIMDs, a leftover), K split
+# over 2 and 4 waves, rows that end inside a load and their scales' last chunk, scales past
+# the copy (then the kernel of 2 to 16 rows).  2 to 16 rows: scales of single entries and of
+# eights, more of either than the threads read ahead; x in slices.  Split sums of odd
+# widths.
+MORE = [
+    (1, 4099, 2048, 64, 4, BF, "silu"),
+    (1, 2057, 2048, 128, 8, HF, "silu"),
+    (1, 40, 20480, 32, 4, BF, "gelu_tanh"),
+    (1, 131, 544, 32, 4, HF, "silu"),
+    (1, 77, 800, 32, 8, BF, "silu"),
+    (1, 24, 131072, 32, 4, BF, "silu"),
+    (1, 3, 32, 32, 8, HF, "silu"),
+    (2, 17000, 4096, 32, 4, BF, "silu"),
+    (4, 17000, 960, 64, 4, BF, "silu"),
+    (6, 9, 1056, 32, 8, HF, "silu"),
+    (16, 2100, 10240, 128, 4, BF, "gelu_tanh"),
+    (45, 1001, 2560, 128, 8, HF, "silu"),
+    (64, 513, 4096, 64, 4, BF, "silu"),
+]
+
+
+@pytest.mark.parametrize("M,N,K,gs,bits,dtype,act", MORE)
+def test_more_forward(M, N, K, gs, bits, dtype, act):
+    _, x, gate, wg, up, wu = _case(M, N, K, gs, bits, dtype, seed=7)
+    h = mq.quantized_glu(x, gate, up, act, group_size=gs, bits=bits)
+    check(h, *glu_ref(x, wg, wu, act, dtype))
+    # the sums kept for the gradient leave the result as it is
+    x.requires_grad_()
+    assert torch.equal(mq.quantized_glu(x, gate, up, act, group_size=gs, bits=bits).detach(), h)
+
+
+@pytest.mark.parametrize("M,N,K,gs,bits,dtype,act", MORE)
+def test_more_gradient(M, N, K, gs, bits, dtype, act):
+    g, x, gate, wg, up, wu = _case(M, N, K, gs, bits, dtype, seed=8)
+    d = torch.randn((M, N), generator=g, device="cuda").to(dtype)
+    x.requires_grad_()
+    h = mq.quantized_glu(x, gate, up, act, group_size=gs, bits=bits)
+    dx, = torch.autograd.grad(h, x, d)
+    check(dx, *glu_grad_ref(x.detach(), d, wg, wu, act, dtype), "dx")
+
+
+@pytest.mark.parametrize("bits,dtype", [(4, BF), (8, HF)])
+def test_one_row_scales_at_any_address(bits, dtype):
+    """Scales and biases from two-byte addresses: every value of the same bits."""
+    _, x, gate, _, up, _ = _case(1, 515, 1056, 32, bits, dtype, seed=9)
+    kw = dict(group_size=32, bits=bits)
+    want = mq.quantized_glu(x, gate, up, **kw)
+    lib = mq._lib.lib()
+    moved = []
+    for m in (gate, up):
+        moved.append(m[0])
+        for t in m[1:]:
+            buf = torch.full((t.numel() + 8,), float("nan"), dtype=dtype, device="cuda")
+            buf[3:3 + t.numel()] = t.reshape(-1)
+            moved.append(buf[3:3 + t.numel()])
+    out = torch.full_like(want, float("nan"))
+    rc = lib.mq_quantized_glu(x.data_ptr(), *[t.data_ptr() for t in moved], out.data_ptr(), None,
+                              None, 1, 515, 1056, 32, bits, 0 if dtype == BF else 1, 0, None, 0,
+                              torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(out, want)
+
+
+def test_weights_replaced_or_changed():
+    """Like a saved tensor of the engine's: a weight changed in place since the forward pass
+    is refused, and a graph can be gone through twice if it is kept."""
+    _, x, gate, _, up, _ = _case(20, 240, 128, 64, 4, BF, seed=10)
+    x.requires_grad_()
+    h = mq.quantized_glu(x, gate, up)
+    y = mq.quantized_matmul(x, *gate)
+    first = [torch.autograd.grad(t.float().sum(), x, retain_graph=True)[0] for t in (h, y)]
+    again = [torch.autograd.grad(t.float().sum(), x, retain_graph=True)[0] for t in (h, y)]
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    up[2].add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        h.sum().backward(retain_graph=True)
+    y.sum().backward(retain_graph=True)
+    gate[0].copy_(gate[0].clone())
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()

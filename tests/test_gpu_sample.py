@@ -220,3 +220,21 @@ def test_head_then_sample():
     _check(logits, torch.rand((2, 5), generator=g, device="cuda"), top_k=64, top_p=0.95)
     tok, _ = mq.sample(logits, torch.zeros((2, 5), device="cuda"), temperature=0)
     assert torch.equal(tok.long(), logits.float().argmax(-1))
+
+
+@pytest.mark.parametrize("dtype,spread", [(F32, 0.012), (F32, 1e-5), (F32, 0.0), (BF, 0.012),
+                                          (HF, 0.3), (HF, 0.012)])
+@pytest.mark.parametrize("V", [2, 600, 3001, 4096, 4099])
+@pytest.mark.parametrize("kw", [dict(top_p=p, min_p=m) for p in (1e-6, 0.0377, 0.5137, 0.999)
+                                for m in (0.0, 0.993)], ids=str)
+def test_cut_of_p_inside_one_bin(V, dtype, spread, kw):
+    """The cut of p among thousands of words of nearly, or just, the same logit, some with
+    masked words and larger ones between them."""
+    g = _gen(V)
+    logits = 1 + torch.rand((3, V), generator=g, device="cuda") * spread
+    logits[1, ::3] = -INF
+    if V > 10:
+        logits[2, 5::7] += 2
+    # (these p times counts of equal words are no whole numbers; a row in three may lie at a
+    # border by u)
+    _check(logits.to(dtype), torch.rand(3, generator=g, device="cuda"), skip=1 / 3, **kw)
