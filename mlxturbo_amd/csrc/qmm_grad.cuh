@@ -11,9 +11,9 @@
 // (The transposing LDS reads, ds_read_b64_tr_b16, would take the other half too, but
 // the compiler has them wait for every load into LDS that is under way.)
 //
-// MFMA- and power-bound: both matrices of 17408 x 5120, 4 bits, 2048 rows 646 us, 1.13 PFLOP/s
-// (a library product d . W of that size 824), and 23 for the sum of 2 splits; 301 rows of 2 x
-// (8192 x 2048) 44.5 + 6.1, 77 rows of 65536 x 2048 at 8 bits 63.7 + 8.3.
+// MFMA- and power-bound: both matrices of 17408 x 5120, 4 bits, 2048 rows 660 us, 1.1 PFLOP/s
+// (a library product d . W of that size 824), and 24 for the sum of 3 splits; 301 rows of 2 x
+// (8192 x 2048) on 13 splits 44.7 + 6.0, 77 rows of 65536 x 2048 at 8 bits on 28 63.9 + 8.3.
 #pragma once
 #include "dense.cuh"
 #include "glu_launch.h"

@@ -20,8 +20,8 @@
 // row is spread over workgroups (chunks of its tiles, up to 1024 of 64 granules or
 // more), and the passes are launches for all rows whatever their settings.  (us of the
 // steps, 248320 bf16 words: one row with k and p 3.2, 7.1 and 10.9 for 3 and 4; 64 rows of
-// mixed settings 10.6, at 3 TB/s of logits, 22.8, of which 13 are the double arithmetic
-// of the masses, 18.3 and 16.2.)
+// mixed settings 10.3, at 3 TB/s of logits, 22.6, of which 13 by instruction count are the double
+// arithmetic of the masses, 18.7 and 16.4.)
 //   1 each tile's first word.  Where k tiles hold a word, the k-th largest of their
 //     first words is no larger than the k-th largest word: a bound (step 2 finds it)
 //     above which lie few more than k words;
