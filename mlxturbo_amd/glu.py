@@ -45,13 +45,15 @@ def _room(ws: Optional[torch.Tensor]):
     return (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
 
 
-def note_leaf(x: torch.Tensor) -> None:
+def note_leaf(x: torch.Tensor):
     """Refuses a capture that would end in an accumulator of another stream: a leaf's
     is made by the first graph of it that lives and keeps that graph's stream, and a
-    captured backward that reaches it from another stream ends the process."""
+    captured backward that reaches it from another stream ends the process.  Returns the
+    accumulator, which the caller holds until the graph does (else it and the note are gone)."""
     if not x.is_leaf:
-        return
-    meta = torch.autograd.graph.get_gradient_edge(x).node.metadata
+        return None
+    node = torch.autograd.graph.get_gradient_edge(x).node
+    meta = node.metadata
     stream = ops._stream_of(x.device)
     if torch.cuda.is_current_stream_capturing():
         if meta.get("mq_stream", stream) != stream:
@@ -59,6 +61,7 @@ def note_leaf(x: torch.Tensor) -> None:
                 "x is a leaf of a graph made on another stream that still lives, and its gradient "
                 "cannot be captured: drop that graph, or pass x.detach().requires_grad_()")
     meta.setdefault("mq_stream", stream)
+    return node
 
 
 def _glu_forward(x, flat, act: int, group_size: int, bits: int, save: bool):
@@ -196,10 +199,12 @@ def quantized_matmul_differentiable(x, w, scales, biases, group_size: int, bits:
     if any(t.requires_grad for t in (scales, biases)):
         raise NotImplementedError("quantized_matmul: scales and biases are constants here; "
                                   "gradients go to x")
-    note_leaf(x)
+    leaf = note_leaf(x)
     flat = [ops._aligned(t) for t in (w, scales, biases)]
-    y = _Matmul.apply(x.reshape(-1, x.shape[-1]), flat, group_size, bits)
-    return y.reshape(*x.shape[:-1], w.shape[0])
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    y = _Matmul.apply(x2, flat, group_size, bits)
+    del leaf
+    return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 
 def _activation(g: torch.Tensor, activation: str) -> torch.Tensor:
@@ -259,7 +264,9 @@ def quantized_glu(x: torch.Tensor, gate, up, activation: str = "silu",
     w = gate[0]
     if w.ndim != 2:
         raise NotImplementedError("batched w: only 2-D weights are on this path")
-    K = [ops._check_quant(*m, group_size, bits) for m in (gate, up)][0]
+    K = ops._check_quant(*gate, group_size, bits)
+    if up[2].shape != up[1].shape or up[2].dtype != up[1].dtype:
+        ops._check_quant(*up, group_size, bits)       # (the rest is the gate's: says what differs)
     if x.ndim < 1 or x.shape[-1] != K:
         raise ValueError(f"x {tuple(x.shape)} does not match the quantized weight K={K}")
     grad = wants_grad(x)
@@ -269,13 +276,14 @@ def quantized_glu(x: torch.Tensor, gate, up, activation: str = "silu",
     if K == 0 or not (bits in (4, 8) and ops._kernel_dtype(x.dtype, gate[1].dtype)):
         return _composed(x, gate, up, activation, group_size, bits, mode)
     N, lead = w.shape[0], tuple(x.shape[:-1])
-    x2 = x.reshape(math.prod(lead), K)
+    x2 = x if x.ndim == 2 else x.reshape(math.prod(lead), K)
     flat = [ops._aligned(t) for t in (*gate, *up)]
     if grad:
-        note_leaf(x)
+        leaf = note_leaf(x)
         y = _Glu.apply(ops._aligned(x2), flat, ACTIVATIONS[activation], group_size, bits)
-        return y.reshape(*lead, N)
+        del leaf
+        return y if x.ndim == 2 else y.reshape(*lead, N)
     r = _glu_forward(ops._aligned(x2), flat, ACTIVATIONS[activation], group_size, bits, False)
     if r is None:
         return _composed(x, gate, up, activation, group_size, bits, mode)
-    return r[0].reshape(*lead, N)
+    return r[0] if x.ndim == 2 else r[0].reshape(*lead, N)

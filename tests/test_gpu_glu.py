@@ -496,3 +496,21 @@ def test_weights_replaced_or_changed():
     gate[0].copy_(gate[0].clone())
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("shape", [(4, 128), (2, 2, 128)])
+@pytest.mark.parametrize("glu", [False, True])
+def test_every_call_notes_its_leaf(shape, glu):
+    """The refusal above of either operator alone, of rows and of more dimensions, by a
+    graph of the other one too."""
+    _, x, gate, _, up, _ = _case(4, 256, 128, 64, 4, BF, seed=15)
+    x = x.reshape(shape).requires_grad_()
+    calls = [lambda t: mq.quantized_matmul(t, *gate), lambda t: mq.quantized_glu(t, gate, up)]
+    for other in (False, True):
+        alive = calls[glu](x)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="still lives"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                calls[other](x)
+        torch.cuda.synchronize()
+        del alive
