@@ -140,8 +140,8 @@ def _versions(ts) -> list:
 
 def _constants(ctx, ts) -> None:
     """Keeps the weights for the backward pass.  They are constants, so they go past the
-    engine's saved tensors, whose packing and unpacking cost 2 us each a step; like those they
-    may not have changed by then."""
+    engine's saved tensors, whose packing and unpacking cost several us a step; like those
+    they may not have changed by then."""
     ctx.flat, ctx.versions = ts, _versions(ts)
 
 

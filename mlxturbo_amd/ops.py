@@ -17,6 +17,8 @@ MLX 0.32's operators as the reference calls them:
   (kernels/moe_combine.py:160-195)
 
 * ``qqmm`` - mx.qqmm: activations and weights both quantized
+* ``quantized_glu`` - a dense MLP's gate, up and activation (:mod:`mlxturbo_amd.glu`)
+* ``sample`` - a token from a head's logits (:mod:`mlxturbo_amd.sampling`)
 
 ``mode="mxfp4"`` (:mod:`mlxturbo_amd.mx`): block-scaled 4-bit floating point
 codes, without biases, in quantize, dequantize, quantized_matmul, gather_qmm and
