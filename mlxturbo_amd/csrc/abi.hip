@@ -224,7 +224,7 @@ int check_glu(const void* wg, const void* sg, const void* bg, const void* wu, co
     return fail(MQ_EUNSUPPORTED, "float32 activations are not implemented on this path");
   if (activation != MQ_ACT_SILU && activation != MQ_ACT_GELU_TANH)
     return fail(MQ_EINVAL, "unknown activation code %d", activation);
-  if (M < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX / 8)
+  if (M < 0 || M > INT32_MAX || N > INT32_MAX - 255 || K > INT32_MAX / 8)
     return fail(MQ_EINVAL, "invalid sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N,
                 (long long)K);
   if (workspace && !aligned16(workspace)) return fail(MQ_EINVAL, "workspace must be 16-byte aligned");
@@ -245,7 +245,7 @@ int grad_product(const void* d, const float* gate_sums, const float* up_sums, co
     return fail(MQ_EUNSUPPORTED, "float32 gradients are not implemented on this path");
   if (!d || !dx) return fail(MQ_EINVAL, "d and dx must be non-null");
   if (!aligned16(d)) return fail(MQ_EINVAL, "d must be 16-byte aligned");
-  if (M < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX / 8)
+  if (M < 0 || M > INT32_MAX || N > INT32_MAX - 255 || K > INT32_MAX / 8)
     return fail(MQ_EINVAL, "invalid sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N,
                 (long long)K);
   if (workspace && !aligned16(workspace)) return fail(MQ_EINVAL, "workspace must be 16-byte aligned");
