@@ -519,11 +519,11 @@ int QuadLaunch<DT, BITS, GS>::run(const void* x, const uint32_t* w, const void* 
   return 0;
 }
 
-// The gated launch: two waves per quad and K slice, so splits as of twice the quads.
+// The gated launch (x 16-byte aligned): two waves per quad and K slice, so splits as of
+// twice the quads.
 template <int DT, int BITS, int GS>
 int GluQuadLaunch<DT, BITS, GS>::run(const GluArgs& a, hipStream_t st) {
   auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  if (!a16(a.x)) return kStatusUnsupported;
   const int odd = !a16(a.sg) || !a16(a.bg) || !a16(a.su) || !a16(a.bu);
   const int64_t N = a.N, K = a.K;
   if (N * (K / GS) * 2 >= ((int64_t)1 << 31)) return kStatusUnsupported;

@@ -221,7 +221,7 @@ struct RowSpace {
   u64* mass;                                    // [kBins]
   u64* list;                                    // [kList] order keys
   uint32_t* count;                              // [kBins], the list's length, workgroups done
-  u64* row;                                     // Row
+  u64* row;                                     // first word's key; the bound's bits (-inf: none)
 };
 __device__ __forceinline__ RowSpace row_space(void* ws, int r) {
   unsigned char* p = static_cast<unsigned char*>(ws) + (size_t)r * kSampleRowBytes;
@@ -359,13 +359,6 @@ __device__ __forceinline__ float bound_of(const u64* tops, int tiles, int k) {
   }
   return key_value((u64)bound << 48);
 }
-
-// What step 2 leaves of that for the next ones: the first word, and the bound (-inf:
-// none).
-struct Row {
-  u64 first;
-  float low;
-};
 
 // ---- 1: each tile's first word; the row's histogram and list are emptied -----------
 template <int DT>
