@@ -14,13 +14,12 @@
 //    27.7 us (loads without the arithmetic; N=17408 K=5120, weights from memory).
 //  * A tile's K range is cut into units of one 128-byte line of each row; the units of
 //    all the workgroup's tiles, in order, are dealt to the waves in contiguous
-//    runs that differ by one unit at most.  A wave
-//    streams its run one unit ahead, without a stop at the tiles' ends: 16 waves
-//    hold 64 KB of loads in flight per CU; two, three and four units ahead took 0.9, 1.9 and
-//    2.9 us more of 28, as the scales then wait for behind the weights.  A run of at most
-//    one tile's units touches at most two tiles, whose sums meet the other waves' in LDS
-//    at the end, added in wave order: an order that depends on N, K and the CU count
-//    alone.
+//    runs that differ by one unit at most.  A wave streams its run one unit ahead,
+//    without a stop at the tiles' ends: 16 waves hold 64 KB of loads in flight per CU; two,
+//    three and four units ahead took 0.9, 1.9 and 2.9 us more of 28, as the scales then
+//    wait behind the weights.  A run of at most one tile's units touches at most two
+//    tiles, whose sums meet the other waves' in LDS at the end, added in wave order: an
+//    order that depends on the call's sizes and the CU count alone.
 //  * A load instruction reads one whole line of 8 rows of one matrix, non-temporal: lane
 //    (r = lane & 15, c = lane >> 4) the 16-byte chunk 2 c + (r >> 3) of row r & 7.  The
 //    operand wants rows 8 .. 15 to be the up matrix's: lanes r < 8 and r >= 8 of a
