@@ -19,7 +19,7 @@
 // One row of 248320 16-bit words is half a megabyte: latency bounds a few rows, so a
 // row is spread over workgroups (chunks of its tiles, up to 1024 of 64 granules or
 // more), and the passes are launches for all rows whatever their settings.  (us of the
-// steps, 248320 bf16 words: one row with k and p 3.2, 7.1 and 10.9 for 3 and 4; 64 rows of
+// steps, 248320 bf16 words: one row with k and p 3.2, 5.4 and 10.3 for 3 and 4; 64 rows of
 // mixed settings 10.3, at 3 TB/s of logits, 22.6, of which 13 by instruction count are the double
 // arithmetic of the masses, 18.7 and 16.4.)
 //   1 each tile's first word.  Where k tiles hold a word, the k-th largest of their
@@ -340,9 +340,9 @@ __device__ __forceinline__ Tops row_tops(const RowSet& set, const RowSpace& s, i
 }
 
 // Of the upper 16 bits of value keys, the largest that k of the tiles' first words reach,
-// as a logit.  One wave.
+// as a logit.  One wave, PER tiles a lane (485 tiles as 8 a lane 5.4 us of step 2, as 16 7.1).
+template <int PER>
 __device__ __forceinline__ float bound_of(const u64* tops, int tiles, int k) {
-  constexpr int PER = kSampleTiles / 64;
   const int lane = threadIdx.x & 63;
   uint32_t v[PER];
 #pragma unroll
@@ -410,7 +410,10 @@ __global__ __launch_bounds__(kThreads) void sample_mass_kernel(SampleArgs a, voi
     for (int i = t; i < kBins; i += kThreads) hm[i] = 0;
   const Tops tops = row_tops(set, s, n, tmp);   // (and the table is written)
   if (c == 0 && t < 64) {
-    const float low = tops.bound ? bound_of(s.tops, n, set.k) : kNone;
+    constexpr int PER = kSampleTiles / 64;
+    const float low = !tops.bound       ? kNone
+                      : n <= 32 * PER ? bound_of<PER / 2>(s.tops, n, set.k)
+                                      : bound_of<PER>(s.tops, n, set.k);
     if (t == 0) {
       s.row[0] = tops.first;
       s.row[1] = __float_as_uint(low);
