@@ -518,8 +518,8 @@ int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_sca
  * d[M, N] . deq(w), float sums, one rounding.  workspace of
  * mq_quantized_matmul_grad_workspace_size(M, N, K, group_size, bits) bytes, 16-byte
  * aligned; it may be NULL where N % 64 == 0 (then nothing splits N).  d and w
- * 16-byte aligned.  MQ_EUNSUPPORTED: no columns, codes of 2^31 bytes and more, rows
- * of d of 2^22 elements and more (padded to whole 64s), 2, 3, 5 and 6 bits, float32.
+ * 16-byte aligned.  MQ_EUNSUPPORTED: no columns, codes of 2^31 bytes and more and rows of
+ * d of 2^22 elements and more (N padded to whole 64s in both), 2, 3, 5 and 6 bits, float32.
  */
 size_t mq_quantized_matmul_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
                                                int bits);

@@ -102,10 +102,11 @@ struct GradLaunch {
   static int run(const GradArgs& a, const WidePlan& plan, void* ws, hipStream_t st, int* nlaunch);
 };
 
-// one tile's rows of d, and the matrices, must fit 31-bit buffer ranges
+// one tile's rows of d, and the matrices in whole steps of rows, must fit 31-bit buffer
+// ranges
 inline bool grad_eligible(int64_t M, int64_t N, int64_t K, int bits, int64_t ld) {
-  return N * (K * bits / 8) < ((int64_t)1 << 31) && ld * 2 * 256 < ((int64_t)1 << 31) &&
-         M <= (int64_t)65535 * 64;
+  return 64 * grad_steps(N) * (K * bits / 8) < ((int64_t)1 << 31) &&
+         ld * 2 * 256 < ((int64_t)1 << 31) && M <= (int64_t)65535 * 64;
 }
 
 // Tile height and split of the sum, the pair of least cost by a model fitted to 6600

@@ -61,6 +61,20 @@ constexpr int kGradWaveLds = kGradBlock + 2 * kGradScales;
 // the part that body step u reads: 0 (A0) or 1 (A2)
 constexpr int grad_part(int u) { return (u & 3) == 0 || (u & 3) == 3 ? 0 : 1; }
 
+// Scalar offset of a step's rows from `row` on in a matrix of `bytes` bytes and rows of
+// rowB.  A raw buffer load is in range where its lane's offset is below the buffer's size
+// less the scalar offset, so that one stays within the size: a block of the last step may
+// begin past the last row, and then reads zeros.
+__host__ __device__ inline uint32_t grad_rows_at(uint32_t row, uint32_t rowB, int64_t bytes) {
+  const uint32_t o = row * rowB;
+  return o < (uint32_t)bytes ? o : (uint32_t)bytes;
+}
+// The first of the two rows of a block (weight rows 8 s .. + 7 and 32 + 8 s .. + 7 of a step)
+// that a lane dequantizes, less 8 s.
+__host__ __device__ inline uint32_t grad_lane_row(int lane) {
+  return (uint32_t)(((lane & 7) >> 2) * 32 + 2 * (lane & 3));
+}
+
 // One tile: BM rows of d times 256 columns of the weights (64 per wave, as two
 // 32-column blocks) over steps kt0 .. kt0 + nk - 1 (nk >= 1) of 64 weight rows, nst
 // of them in each matrix.  As stream_tile.cuh's tile, d goes to LDS three steps
@@ -92,7 +106,7 @@ __device__ __forceinline__ void grad_tile(
   // block s of a step: weight rows 8 s .. + 7 and 32 + 8 s .. + 7; this lane's are rows
   // 2 np and 2 np + 1 of the 16, its columns 8 ko .. + 7 of the wave's 64
   const int np = lane & 7, ko = lane >> 3, wc = col0 + 64 * wave;
-  const uint32_t lrow = (uint32_t)((np >> 2) * 32 + 2 * (np & 3));
+  const uint32_t lrow = grad_lane_row(lane);
   const uint32_t wo = wc + 8 * ko < K ? lrow * rowB + (uint32_t)(wc + 8 * ko) * BITS / 8 : 0x80000000u;
   const uint32_t wo1 = wc + 8 * ko < K ? wo + rowB : 0x80000000u;
   // scales: lane l loads row l of the step
@@ -165,7 +179,7 @@ __device__ __forceinline__ void grad_tile(
   auto bload = [&](int kt, int s, auto cc) {
     constexpr int c = decltype(cc)::value & (RB - 1);
     bool second;
-    const uint32_t o = (place(kt, second) + 8 * s) * rowB;
+    const uint32_t o = grad_rows_at(place(kt, second) + 8 * s, rowB, wbytes);
     const auto rw = wide_rsrc(second ? w2 : w1, wbytes);
     if constexpr (WW == 1) {
       Wa[c][0] = __builtin_amdgcn_raw_buffer_load_b32(rw, wo, o, 0);
@@ -185,7 +199,7 @@ __device__ __forceinline__ void grad_tile(
   auto sload = [&](int kt, auto uc) {
     constexpr int u = decltype(uc)::value & 3;
     bool second;
-    const uint32_t o = place(kt, second) * rowS;
+    const uint32_t o = grad_rows_at(place(kt, second), rowS, sbytes);
     const auto rs = wide_rsrc(second ? s2 : s1, sbytes);
     const auto rb = wide_rsrc(second ? b2 : b1, sbytes);
 #pragma unroll
