@@ -530,8 +530,9 @@ int mq_quantized_matmul_grad(const void* d, const uint32_t* w, const void* scale
 
 /*
  * x's gradient through mq_quantized_glu: dx = dg . deq(gate) + du . deq(up) with dg =
- * T(d u act'(g)) and du = T(d act(g)) of the forward's float sums g and u.  The workspace
- * (mq_quantized_glu_grad_workspace_size bytes, 16-byte aligned) holds dg and du, so it
+ * d u act'(g) and du = d act(g) of the forward's float sums g and u, each multiplied as two
+ * numbers of the type (the value rounded, and the rest): float sums, one rounding.  The
+ * workspace (mq_quantized_glu_grad_workspace_size bytes, 16-byte aligned) holds them, so it
  * is needed; MQ_EUNSUPPORTED as above (rows of 2 N elements here).
  */
 size_t mq_quantized_glu_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,

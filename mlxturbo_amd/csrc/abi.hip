@@ -252,8 +252,8 @@ int grad_product(const void* d, const float* gate_sums, const float* up_sums, co
   if (M == 0) return MQ_OK;
   if (N == 0) return fail(MQ_EUNSUPPORTED, "%s of no columns is all zeros", what);
   const size_t rows = mq::grad_rows_bytes(M, N, banks);
-  const int64_t ld = rows ? banks * 64 * mq::grad_steps(N) : N;
-  if (!mq::grad_eligible(M, N, K, bits, ld))
+  const int64_t ld = rows ? mq::grad_row(N, banks) : N;
+  if (!mq::grad_eligible(M, N, K, bits, ld, banks))
     return fail(MQ_EUNSUPPORTED, "%s: the matrix or a tile's rows pass a 31-bit range", what);
   if (rows && (!workspace || workspace_bytes < rows))
     return fail(MQ_EINVAL, "%s needs a workspace of %zu bytes, 16-byte aligned", what, rows);

@@ -1,10 +1,13 @@
 // Between h's gradient and x's in the gated feed-forward block: from d = dL/dh and
-// the forward's float sums g and u, dL/dg = d u act'(g) and dL/du = d act(g), rounded
-// to T for the products past the weights (their one rounding: g and u are float).
+// the forward's float sums g and u, dL/dg = d u act'(g) and dL/du = d act(g), as operands of
+// the products past the weights.  One T number for each would add its rounding to x's
+// gradient, as large as that one's own (with both, 1.41 times the error of a float32 form), so
+// each is two: the value rounded to T, and the rest rounded to T, together within 2^-16 of
+// the value in bfloat16 and 2^-22 in float16.  The products then take twice the MFMAs.
 //
-// HBM-bound: 10 bytes read and 4 written per element, 2048 x 17408 in 103 us, 4.8 TB/s.  Eight columns per thread.  The two
-// halves lie side by side in a row, each padded with zeros to whole steps of 64
-// columns.
+// HBM-bound: 10 bytes read and 8 written per element.  Eight columns per thread.  dg and du
+// lie side by side in a row, each padded with zeros to whole steps of 64 columns, then
+// their rests.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,6 +27,19 @@ __device__ __forceinline__ void act_grad(float g, int act, float& a, float& da) 
   const float dz = act == kActSilu ? 1.0f : fminf(kGeluZ * (1.0f + 3.0f * gg), 0x1p60f);
   da = s + a * (1.0f - s) * dz;
 }
+
+// v rounded to T, and the rest; a value past T's range has no rest (inf - inf).
+template <int DT>
+struct Pair {
+  float hi, lo;
+  __device__ __forceinline__ explicit Pair(float v) {
+    // the rounding may pass T's largest number, of which the rest is then taken
+    hi = T16<DT>::to_f32(T16<DT>::round1(v));
+    if (__builtin_isinf(hi) && !__builtin_isinf(v)) hi = __builtin_copysignf(kMost, v);
+    lo = __builtin_isinf(hi) ? 0.f : v - hi;
+  }
+  static constexpr float kMost = DT == kBF16 ? 0x1.fep127f : 65504.f;
+};
 
 // Grid (ceil(P / 2048), min(M, 65535)), 256 threads; P = 64 ceil(N / 64).  VEC: N in
 // whole eights, all arrays 16-byte aligned.
@@ -62,23 +78,26 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const uint16_t* __restric
         u[e] = in ? uf[o + e] : 0.f;
       }
     }
-    u32x4 og, ou;
+    u32x4 out[4];                               // dg, du, and their rests
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      float x[2], y[2];
+      float v[4][2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float a, da;
         act_grad(g[2 * q + e], act, a, da);
-        x[e] = dv[2 * q + e] * u[2 * q + e] * da;
-        y[e] = dv[2 * q + e] * a;
+        const Pair<DT> x(dv[2 * q + e] * u[2 * q + e] * da), y(dv[2 * q + e] * a);
+        v[0][e] = x.hi;
+        v[1][e] = y.hi;
+        v[2][e] = x.lo;
+        v[3][e] = y.lo;
       }
-      og[q] = T::pack2(x[0], x[1]);
-      ou[q] = T::pack2(y[0], y[1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i][q] = T::pack2(v[i][0], v[i][1]);
     }
-    uint16_t* row = dgu + m * 2 * P + c;
-    *reinterpret_cast<u32x4*>(row) = og;
-    *reinterpret_cast<u32x4*>(row + P) = ou;
+    uint16_t* row = dgu + m * 4 * P + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(row + i * P) = out[i];
   }
 }
 

@@ -75,17 +75,17 @@ inline size_t glu_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int
 // Steps of 64 weight rows that N rows take.
 inline int64_t grad_steps(int64_t N) { return (N + 63) / 64; }
 
-// dgu[M, 2 * 64 * grad_steps(N)] (T): d * u * act'(g) in the first half, d * act(g)
-// in the second, zeros past N columns (glu_grad.hip).
+// dgu[M, 4 * P] (T), P = 64 * grad_steps(N): dg = d * u * act'(g), du = d * act(g), rounded
+// to T, then what the rounding left of each, rounded to T; zeros past N columns
+// (glu_grad.hip).
 int launch_glu_grad(const void* d, const float* gf, const float* uf, void* dgu, int64_t M,
                     int64_t N, int act, int dtype, hipStream_t st);
 
 // Rows of N elements of a 16-bit type to rows of 64 * grad_steps(N), zeros past N.
 int launch_pad_rows(const void* d, void* out, int64_t M, int64_t N, hipStream_t st);
 
-// out[M, K] = d[:, first half] . W1 + d[:, second half] . W2 (w2 NULL: d . W1) for
-// quantized W [N, K]; d's rows of ld elements, a half padded to whole steps of
-// 64 columns with zeros.
+// out[M, K] = d . W1, or with w2 dg . W1 + du . W2 of glu_grad.hip's rows, for quantized
+// W [N, K]; d's rows of ld elements, padded to whole steps of 64 columns with zeros.
 struct GradArgs {
   const void* d;
   int64_t ld;
@@ -102,11 +102,19 @@ struct GradLaunch {
   static int run(const GradArgs& a, const WidePlan& plan, void* ws, hipStream_t st, int* nlaunch);
 };
 
-// one tile's rows of d, and the matrices in whole steps of rows, must fit 31-bit buffer
-// ranges
-inline bool grad_eligible(int64_t M, int64_t N, int64_t K, int bits, int64_t ld) {
+// A tile's rows of out: with two matrices half its height, as each has two rows of d.
+constexpr int grad_tile_rows(int bm, bool pair) { return pair ? bm / 2 : bm; }
+
+// Elements of a row of d that the product reads: whole steps, of both matrices two numbers a
+// column.
+inline int64_t grad_row(int64_t N, int banks) { return (banks == 2 ? 4 : 1) * 64 * grad_steps(N); }
+
+// One tile's rows of d (ld elements each), and the matrices in whole steps of rows, must fit
+// 31-bit buffer ranges.
+inline bool grad_eligible(int64_t M, int64_t N, int64_t K, int bits, int64_t ld, int banks = 1) {
   return 64 * grad_steps(N) * (K * bits / 8) < ((int64_t)1 << 31) &&
-         ld * 2 * 256 < ((int64_t)1 << 31) && M <= (int64_t)65535 * 64;
+         ld * 2 * grad_tile_rows(256, banks == 2) < ((int64_t)1 << 31) &&
+         M <= (int64_t)65535 * grad_tile_rows(64, banks == 2);
 }
 
 // Tile height and split of the sum, the pair of least cost by a model fitted to 6600
@@ -128,8 +136,8 @@ inline WidePlan grad_plan(int64_t M, int64_t N, int64_t K, int bits, int banks, 
     const double steps = (double)((ns + sp - 1) / sp);
     if (sp > 1 && steps < 4) break;
     for (int i = 3; i >= 0; --i) {
-      const int bm = 64 * (i + 1);
-      const double tiles = (double)(cols * ((M + bm - 1) / bm) * sp);
+      const int bm = 64 * (i + 1), rows = grad_tile_rows(bm, banks == 2);
+      const double tiles = (double)(cols * ((M + rows - 1) / rows) * sp);
       const double rounds = (double)(int64_t)((tiles + cus - 1) / cus);
       const WideTileUs& u = us[w][i];
       double cost = bm == 64 ? u.c0 * (double)((int64_t)(rounds + 1) / 2) +
@@ -154,7 +162,7 @@ constexpr int kGradSplits = 48;
 // not whole steps (banks 2: dgu), then the split planes.
 inline size_t grad_rows_bytes(int64_t M, int64_t N, int banks) {
   if (banks == 1 && N % 64 == 0) return 0;
-  return ((size_t)M * banks * 64 * (size_t)grad_steps(N) * 2 + 255) & ~(size_t)255;
+  return ((size_t)M * (size_t)grad_row(N, banks) * 2 + 255) & ~(size_t)255;
 }
 inline size_t grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int banks, int cus) {
   return grad_rows_bytes(M, N, banks) +

@@ -83,8 +83,9 @@ __host__ __device__ inline uint32_t grad_lane_row(int lane) {
 // them, a step ahead), and are dequantized two substeps before their MFMAs.
 // Rows of W past N and columns past K read zeros (past the buffers' ranges).
 // col0: the tile's first column; xrow_off, put and put_block as there (a tile row's
-// weight rows are columns here).
-template <int DT, int BITS, int GS, int BM, class XRowOff, class Put, class PutBlock>
+// weight rows are columns here).  PAIR: a row's sums are those of tile rows r and r + BM / 2,
+// which put adds; put_block is given their sum (i < BM / 64).
+template <int DT, int BITS, int GS, int BM, bool PAIR, class XRowOff, class Put, class PutBlock>
 __device__ __forceinline__ void grad_tile(
     __amdgpu_buffer_rsrc_t xr, XRowOff xrow_off, const uint32_t* __restrict__ w1,
     const uint16_t* __restrict__ s1, const uint16_t* __restrict__ b1,
@@ -377,8 +378,8 @@ __device__ __forceinline__ void grad_tile(
     return;
   }
   // a scale of 2^100 or more: block by block, code by code from global memory
-  for (int i = 0; i < MB; ++i) {
-    const uint32_t xo = xrow_off(32 * i + lr) + 64u * h;
+  constexpr int PB = PAIR ? MB / 2 : MB;
+  for (int i = 0; i < PB; ++i) {
     for (int j = 0; j < 2; ++j) {
       f32x16 s;
 #pragma unroll
@@ -390,7 +391,6 @@ __device__ __forceinline__ void grad_tile(
         const auto rs = wide_rsrc(second ? s2 : s1, sbytes);
         const auto rb = wide_rsrc(second ? b2 : b1, sbytes);
         for (int q = 0; q < 4; ++q) {
-          const u32x4 xa = __builtin_amdgcn_raw_buffer_load_b128(xr, xo + 16u * q, k * 128, 0);
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -408,9 +408,11 @@ __device__ __forceinline__ void grad_tile(
             const uint32_t c = BITS == 8 ? code : (code >> (4 * (col & 1))) & 15u;
             v[e] = __builtin_fmaf((float)c, T::to_f32(s16), T::to_f32(b16));
           }
-          s = mfma32<DT>((u32x4){T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]),
-                                 T::pack2(v[6], v[7])},
-                         xa, s);
+          const u32x4 wv = {T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]),
+                            T::pack2(v[6], v[7])};
+          for (int r = 32 * i + lr; r < BM; r += 32 * PB)
+            s = mfma32<DT>(wv, __builtin_amdgcn_raw_buffer_load_b128(
+                                   xr, xrow_off(r) + 64u * h + 16u * q, k * 128, 0), s);
         }
       }
       put_block(i, j, s);
@@ -418,11 +420,15 @@ __device__ __forceinline__ void grad_tile(
   }
 }
 
-// Grid (ceil(K / 256), ceil(M / BM), splits), 256 threads.  d: rows of ld elements,
-// of which `banks` times 64 nst are read.  With part, split z sums its share of the
-// steps into the float plane part[z] ([M, K]) for wide_reduce_kernel; else
-// (splits == 1) the sums are rounded into out.
-template <int DT, int BITS, int GS, int BM>
+// Grid (ceil(K / 256), ceil(M / BM), splits), 256 threads.  d: rows of ld elements, of
+// which 64 nst are read.  With part, split z sums its share of the steps into the float
+// plane part[z] ([M, K]) for wide_reduce_kernel; else (splits == 1) the sums are rounded
+// into out.
+// PAIR: both matrices, and d as two T numbers whose sum is a value (glu_grad.hip): rows of
+// the first matrix's columns and the second's, 64 nst of each, then the second numbers in the
+// same order.  A tile is then BM / 2 rows, the first numbers in its upper half and the second
+// in its lower, whose sums are added in registers; grid.y = ceil(M / (BM / 2)).
+template <int DT, int BITS, int GS, int BM, bool PAIR>
 __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
     const uint16_t* __restrict__ d, int64_t ld, const uint32_t* __restrict__ w1,
     const uint16_t* __restrict__ s1, const uint16_t* __restrict__ b1,
@@ -433,14 +439,19 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
   __shared__ __align__(16) unsigned char A1[StreamLds<BM>::kStage];
   __shared__ __align__(16) unsigned char A2[StreamLds<BM>::kStage + 4 * kGradWaveLds];
   __shared__ __align__(16) unsigned char A3[StreamLds<BM>::kStage];
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * 256;
-  const int mrows = min(BM, M - m0), ncols = min(256, K - n0);
-  const int ns = nst * (w2 ? 2 : 1), z = blockIdx.z;
+  constexpr int R = grad_tile_rows(BM, PAIR);
+  const int m0 = blockIdx.y * R, n0 = blockIdx.x * 256;
+  const int mrows = min(R, M - m0), ncols = min(256, K - n0);
+  const int ns = nst * (PAIR ? 2 : 1), z = blockIdx.z;
   const int kt0 = (int)((int64_t)ns * z / splits), kt1 = (int)((int64_t)ns * (z + 1) / splits);
   const int lane = threadIdx.x & 63, lr = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const auto xr = wide_rsrc(d + (int64_t)m0 * ld, ((int64_t)(mrows - 1) * ld + 64 * ns) * 2);
-  auto xrow_off = [&](int r) { return (uint32_t)(min(r, mrows - 1) * ld) * 2u; };
+  const auto xr = wide_rsrc(d + (int64_t)m0 * ld,
+                            ((int64_t)(mrows - 1) * ld + 64 * (PAIR ? 2 * ns : ns)) * 2);
+  auto xrow_off = [&](int r) {
+    const int low = PAIR && r >= R;             // the value's second number
+    return (uint32_t)(min(r - (low ? R : 0), mrows - 1) * ld) * 2u + (low ? 128u * ns : 0u);
+  };
   const bool vec = (uintptr_t)out % 16 == 0;    // K is whole eights
   auto put_block = [&](int i, int j, const f32x16& acc) {
     const int r = 32 * i + lr;
@@ -464,13 +475,21 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
     auto pin = [&](f32x16& v) {
       if constexpr (BM >= 128) asm volatile("" : "+a"(v));
     };
+    auto sums = [&](int i, int j) {
+      pin(acc[i][j]);
+      if constexpr (PAIR) {
+        pin(acc[i + R / 32][j]);
+        return acc[i][j] + acc[i + R / 32][j];
+      } else {
+        return acc[i][j];
+      }
+    };
     if (part || !vec) {
 #pragma unroll
-      for (int i = 0; i < BM / 32; ++i)
+      for (int i = 0; i < R / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          pin(acc[i][j]);
-          put_block(i, j, acc[i][j]);
+          put_block(i, j, sums(i, j));
           __builtin_amdgcn_sched_barrier(0);
         }
       return;
@@ -479,46 +498,50 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
     // 128 contiguous bytes of 8 rows
     unsigned char* L = wave == 0 ? A0 : wave == 1 ? A1 : wave == 2 ? A2 : A3;
 #pragma unroll
-    for (int i = 0; i < BM / 32; ++i) {
+    for (int i = 0; i < R / 32; ++i) {
       const int r = 32 * i + lr;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        pin(acc[i][j]);
+        const f32x16 v = sums(i, j);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<u32x2*>(L + r * 128 + (((4 * j + q) ^ row_swz(r)) << 4) + 8 * h) =
-              (u32x2){T16<DT>::pack2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
-                      T16<DT>::pack2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+              (u32x2){T16<DT>::pack2(v[4 * q], v[4 * q + 1]),
+                      T16<DT>::pack2(v[4 * q + 2], v[4 * q + 3])};
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     const int c = 64 * wave + 8 * (lane & 7);
     uint16_t* ot = out + (int64_t)m0 * K + n0 + c;
 #pragma unroll 4
-    for (int i = 0; i < BM / 8; ++i) {
+    for (int i = 0; i < R / 8; ++i) {
       const int r = 8 * i + (lane >> 3);
       const u32x4 v =
           *reinterpret_cast<const u32x4*>(L + r * 128 + (((lane & 7) ^ row_swz(r)) << 4));
       if (r < mrows && c < ncols) *reinterpret_cast<u32x4*>(ot + (int64_t)r * K) = v;
     }
   };
-  grad_tile<DT, BITS, GS, BM>(xr, xrow_off, w1, s1, b1, w2, s2, b2, N, K, n0, nst, kt0, kt1 - kt0,
-                              put, put_block, A0, A1, A2, A3);
+  grad_tile<DT, BITS, GS, BM, PAIR>(xr, xrow_off, w1, s1, b1, w2, s2, b2, N, K, n0, nst, kt0,
+                                    kt1 - kt0, put, put_block, A0, A1, A2, A3);
 }
 
 template <int DT, int BITS, int GS>
 int GradLaunch<DT, BITS, GS>::run(const GradArgs& a, const WidePlan& plan, void* ws,
                                   hipStream_t st, int* nlaunch) {
   float* part = plan.splits > 1 ? static_cast<float*>(ws) : nullptr;
-  auto go = [&](auto bmc) {
-    constexpr int BM = decltype(bmc)::value;
-    const dim3 grid((unsigned)((a.K + 255) / 256), (unsigned)((a.M + BM - 1) / BM),
+  auto pair = [&](auto bmc, auto pairc) {
+    constexpr int BM = decltype(bmc)::value, R = grad_tile_rows(BM, decltype(pairc)::value);
+    const dim3 grid((unsigned)((a.K + 255) / 256), (unsigned)((a.M + R - 1) / R),
                     (unsigned)plan.splits);
-    hipLaunchKernelGGL((qmm_grad_kernel<DT, BITS, GS, BM>), grid, dim3(256), 0, st,
-                       (const uint16_t*)a.d, a.ld, a.w1, (const uint16_t*)a.s1,
+    hipLaunchKernelGGL((qmm_grad_kernel<DT, BITS, GS, BM, decltype(pairc)::value>), grid,
+                       dim3(256), 0, st, (const uint16_t*)a.d, a.ld, a.w1, (const uint16_t*)a.s1,
                        (const uint16_t*)a.b1, a.w2, (const uint16_t*)a.s2, (const uint16_t*)a.b2,
                        (uint16_t*)a.out, part, (int)a.M, (int)a.N, (int)a.K,
                        (int)grad_steps(a.N), plan.splits);
+  };
+  auto go = [&](auto bmc) {
+    if (a.w2) pair(bmc, std::true_type{});
+    else pair(bmc, std::false_type{});
   };
   switch (plan.bm) {
     case 64: go(std::integral_constant<int, 64>{}); break;

@@ -8,9 +8,9 @@
 
 The weights are constants: gradients go to x alone, as adapters below a quantized
 layer are trained.  Sums are float; in the gradient of the block, the gate and up
-products are kept in float between forward and backward (8 bytes per output), since
-rounding them to 16 bits would add two roundings to each of the summed terms, and the
-products' inputs ``d u act'(g)`` and ``d act(g)`` are rounded once.
+products are kept in float between forward and backward (8 bytes per output), and the
+products' inputs ``d u act'(g)`` and ``d act(g)`` are two 16-bit numbers each (the value
+rounded, and the rest), so that x's gradient is rounded once, as that of float32 products is.
 """
 
 from __future__ import annotations
@@ -127,9 +127,10 @@ def _glu_grad(d, g, u, flat, act: int, group_size: int, bits: int) -> torch.Tens
         with torch.enable_grad():
             gg, uu = g.detach().requires_grad_(), u.detach().requires_grad_()
             dg, du = torch.autograd.grad(_activation(gg, name) * uu, (gg, uu), d.float())
-        parts = [ops._composed_qmm(t.to(d.dtype), *flat[3 * i:3 * i + 3], False, group_size, bits)
-                 for i, t in enumerate((dg, du))]
-        return (parts[0].float() + parts[1].float()).to(d.dtype)
+        for i, t in enumerate((dg, du)):              # float products, as the kernels' sums are
+            w = ops.dequantize(*flat[3 * i:3 * i + 3], group_size, bits).float()
+            out = torch.addmm(out, t, w) if i else torch.mm(t, w)
+        return out.to(d.dtype)
     _lib.check(rc, "quantized_glu_grad")
     return dx
 

@@ -1,0 +1,138 @@
+"""The gated block's gradient against its definition in 64 bits: that it is rounded once, and
+that what lies between h's gradient and x's may be larger than the type holds."""
+
+import pytest
+import torch
+
+import mlxturbo_amd as mq
+from glu_helpers import activation, bank, check
+from mlxturbo_amd import glu
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _case(M, N, K, gs, bits, dtype, seed, scale=0.02):
+    g = _gen(seed)
+    gate, wg = bank(g, N, K, gs, bits, dtype, scale=scale)
+    up, wu = bank(g, N, K, gs, bits, dtype, scale=scale)
+    x = torch.randn((M, K), generator=g, device="cuda").to(dtype)
+    return g, x, gate, wg, up, wu
+
+
+def _grad(x, gate, up, act, gs, bits, d):
+    x = x.clone().requires_grad_()
+    return torch.autograd.grad(mq.quantized_glu(x, gate, up, act, group_size=gs, bits=bits), x, d)[0]
+
+
+def _between(x, d, wg, wu, act):
+    """dL/dg and dL/du in float64, and how far the float ones may be: of the sums over K
+    products, an addition 2^-23 of the sum of magnitudes (|act'| < 1.13, |act''| < 1.2), of the
+    activation's float steps (16, and an exponent's error times |g|), and of the two products."""
+    x, d = x.double(), d.double()
+    g, u = x @ wg.T, x @ wu.T
+    a, da = activation(g, act)
+    eg, eu = ((x.shape[1] + 16) * 2.0 ** -23 * (x.abs() @ w.abs().T) for w in (wg, wu))
+    rel = (18 + 4 * g.abs()) * 2.0 ** -23
+    dg, du = d * u * da, d * a
+    edg = d.abs() * ((u.abs() + eu) * (1.2 * eg + rel * 1.2) + eu * da.abs())
+    edu = d.abs() * (1.13 * eg + rel * a.abs() + 2.0 ** -126)
+    return dg, du, edg, edu
+
+
+def _half_step(y, dtype):
+    f = torch.finfo(dtype)
+    return (f.eps / 2) * y.abs() + f.smallest_normal * f.eps / 2
+
+
+def _pair(v, dtype):
+    """What two numbers of a type leave of a value: half a step of half a step."""
+    return (torch.finfo(dtype).eps / 2) ** 2 * v.abs() + _half_step(0 * v, dtype)
+
+
+ONE_COLUMN = [
+    (1, 40, 64, 64, 4, BF, "silu"),
+    (7, 9, 64, 32, 8, HF, "gelu_tanh"),
+    (33, 65, 96, 32, 4, BF, "gelu_tanh"),
+    (64, 128, 128, 128, 4, HF, "silu"),
+    (130, 300, 192, 64, 8, BF, "silu"),
+    (300, 77, 128, 64, 4, HF, "gelu_tanh"),
+]
+
+
+@pytest.mark.parametrize("M,N,K,gs,bits,dtype,act", ONE_COLUMN)
+def test_rounded_once(M, N, K, gs, bits, dtype, act):
+    """h's gradient in one column of each row: x's is two products, whose error is the last
+    rounding's and little else."""
+    g, x, gate, wg, up, wu = _case(M, N, K, gs, bits, dtype, 1)
+    d = torch.zeros((M, N), dtype=dtype, device="cuda")
+    rows = torch.arange(M, device="cuda")
+    d[rows, rows * 5 % N] = (1 + torch.rand(M, generator=g, device="cuda")).to(dtype)
+    dg, du, edg, edu = _between(x, d, wg, wu, act)
+    edg, edu = (e + _pair(v.abs() + e, dtype) for v, e in ((dg, edg), (du, edu)))
+    edg, edu = edg * (d != 0), edu * (d != 0)
+    # the sums: four products that are not 0, so a handful of roundings
+    off = edg @ wg.abs() + edu @ wu.abs()
+    off += 2.0 ** -20 * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    dx = dg @ wg + du @ wu
+    check(_grad(x, gate, up, act, gs, bits, d), dx, off + _half_step(dx.abs() + off, dtype))
+
+
+ALL_COLUMNS = [
+    (17, 1111, 512, 64, 4, BF, "silu"),
+    (45, 1001, 2560, 128, 8, HF, "silu"),
+    (129, 640, 1024, 64, 8, BF, "gelu_tanh"),
+    (301, 2048, 1024, 32, 4, HF, "gelu_tanh"),
+    (515, 2056, 640, 64, 4, BF, "silu"),
+]
+
+
+@pytest.mark.parametrize("M,N,K,gs,bits,dtype,act", ALL_COLUMNS)
+def test_error_is_that_of_one_rounding(M, N, K, gs, bits, dtype, act):
+    """Over all columns, the error's root mean square is that of rounding the exact gradient,
+    to a tenth.  A number rounded to half a step eps / 2 is off by about eps / 5 in the mean
+    square.  To it come, independent of it, the rests that pairs leave (eps^2 / 4 of each term at
+    most) and the float sums' roundings: of about sqrt(4 N) additions 2^-23 each, 2^-16 of the
+    result at N = 2056, where eps / 5 is 2^-9.3 (bfloat16) and 2^-12.3; so 1.01 at most.  One
+    more rounding of the terms to the type makes it 1.41."""
+    g, x, gate, wg, up, wu = _case(M, N, K, gs, bits, dtype, 2)
+    d = torch.randn((M, N), generator=g, device="cuda").to(dtype)
+    dg, du, _, _ = _between(x, d, wg, wu, act)
+    dx = dg @ wg + du @ wu
+    got = _grad(x, gate, up, act, gs, bits, d)
+    err, least = (got.double() - dx).norm(), (dx.to(dtype).double() - dx).norm()
+    assert float(err) < 1.1 * float(least), (float(err), float(least))
+    # and the same bits again
+    assert torch.equal(got, _grad(x, gate, up, act, gs, bits, d))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_sizes_without_a_kernel(dtype, monkeypatch):
+    """Sizes that the C entry refuses: float products over the dequantized weights."""
+    g, x, gate, wg, up, wu = _case(5, 200, 128, 64, 4, dtype, 3)
+    d = torch.randn((5, 200), generator=g, device="cuda").to(dtype)
+    want = _grad(x, gate, up, "silu", 64, 4, d)
+    lib = mq._lib.lib()
+
+    class Refusing:
+        def __getattr__(self, name):
+            return getattr(lib, name)
+
+        def mq_quantized_glu_grad(self, *args):
+            return glu.ops._EUNSUPPORTED
+
+    monkeypatch.setattr(glu._lib, "lib", Refusing)
+    got = _grad(x, gate, up, "silu", 64, 4, d)
+    dg, du, edg, edu = _between(x, d, wg, wu, "silu")
+    dx = dg @ wg + du @ wu
+    off = (edg + _pair(dg, dtype)) @ wg.abs() + (edu + _pair(du, dtype)) @ wu.abs()
+    off += 450 * 2.0 ** -23 * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    for v in (got, want):
+        check(v, dx, off + _half_step(dx.abs() + off, dtype))
