@@ -531,7 +531,8 @@ int mq_quantized_matmul_grad(const void* d, const uint32_t* w, const void* scale
 /*
  * x's gradient through mq_quantized_glu: dx = dg . deq(gate) + du . deq(up) with dg =
  * d u act'(g) and du = d act(g) of the forward's float sums g and u, each multiplied as two
- * numbers of the type (the value rounded, and the rest): float sums, one rounding.  The
+ * numbers of the type (the value rounded, and the rest; in float16 rows of them are scaled,
+ * so that they may pass its range): float sums, one rounding.  The
  * workspace (mq_quantized_glu_grad_workspace_size bytes, 16-byte aligned) holds them, so it
  * is needed; MQ_EUNSUPPORTED as above (rows of 2 N elements here).
  */

@@ -265,16 +265,19 @@ int grad_product(const void* d, const float* gate_sums, const float* up_sums, co
     plan = mq::grad_plan(M, N, K, bits, banks, cus, 1);
   int nl = 0;
   const void* dr = d;
+  float* undo = nullptr;
   if (banks == 2) {
-    rc = mq::launch_glu_grad(d, gate_sums, up_sums, workspace, M, N, activation, dtype, st);
-    dr = workspace;
+    undo = static_cast<float*>(workspace);
+    void* dgu = static_cast<char*>(workspace) + mq::grad_undo_bytes(M, banks);
+    rc = mq::launch_glu_grad(d, gate_sums, up_sums, dgu, undo, M, N, activation, dtype, st);
+    dr = dgu;
     ++nl;
   } else if (rows) {
     rc = mq::launch_pad_rows(d, workspace, M, N, st);
     dr = workspace;
     ++nl;
   }
-  const mq::GradArgs a{dr, ld, w1, s1, b1, w2, s2, b2, dx, M, N, K};
+  const mq::GradArgs a{dr, ld, w1, s1, b1, w2, s2, b2, undo, dx, M, N, K};
   if (!rc)
     rc = dispatch_16<mq::GradLaunch>(dtype, bits, group_size, a, plan,
                                      workspace ? static_cast<char*>(workspace) + rows : nullptr,

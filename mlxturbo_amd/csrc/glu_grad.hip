@@ -5,6 +5,11 @@
 // each is two: the value rounded to T, and the rest rounded to T, together within 2^-16 of
 // the value in bfloat16 and 2^-22 in float16.  The products then take twice the MFMAs.
 //
+// float16 holds no more than 65504, and d u act'(g) of a scaled loss may pass it where x's
+// gradient does not.  Its rows are multiplied by a power of two that brings their largest
+// value to 2^14 .. 2^15, which the product's sums are divided by: exact, and what falls below
+// float16's smallest number is then below 2^-39 of the row's largest.
+//
 // HBM-bound: 10 bytes read and 8 written per element.  Eight columns per thread.  dg and du
 // lie side by side in a row, each padded with zeros to whole steps of 64 columns, then
 // their rests.
@@ -41,63 +46,126 @@ struct Pair {
   static constexpr float kMost = DT == kBF16 ? 0x1.fep127f : 65504.f;
 };
 
-// Grid (ceil(P / 2048), min(M, 65535)), 256 threads; P = 64 ceil(N / 64).  VEC: N in
-// whole eights, all arrays 16-byte aligned.
+// dg and du of columns c .. c + 7 of row m, zeros past N.  VEC: N in whole eights, all
+// arrays 16-byte aligned.
 template <int DT, bool VEC>
+__device__ __forceinline__ void row_values(const uint16_t* __restrict__ d,
+                                           const float* __restrict__ gf,
+                                           const float* __restrict__ uf, int64_t m, int64_t c,
+                                           int64_t N, int act, float (&x)[8], float (&y)[8]) {
+  using T = T16<DT>;
+  const int64_t o = m * N + c;
+  float dv[8], g[8], u[8];
+  if (VEC && c < N) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(d + o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dv[e] = T::to_f32((uint16_t)(v[e / 2] >> (16 * (e & 1))));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(gf + o + 4 * q);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(uf + o + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[4 * q + e] = a[e];
+        u[4 * q + e] = b[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = c + e < N;
+      dv[e] = in ? T::to_f32(d[o + e]) : 0.f;
+      g[e] = in ? gf[o + e] : 0.f;
+      u[e] = in ? uf[o + e] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float a, da;
+    act_grad(g[e], act, a, da);
+    x[e] = dv[e] * u[e] * da;
+    y[e] = dv[e] * a;
+  }
+}
+
+// Their pairs to a row of dgu, from its column c on.
+template <int DT>
+__device__ __forceinline__ void put_pairs(uint16_t* row, int64_t P, const float (&x)[8],
+                                          const float (&y)[8]) {
+  u32x4 out[4];                                 // dg, du, and their rests
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const Pair<DT> x0(x[2 * q]), x1(x[2 * q + 1]), y0(y[2 * q]), y1(y[2 * q + 1]);
+    out[0][q] = T16<DT>::pack2(x0.hi, x1.hi);
+    out[1][q] = T16<DT>::pack2(y0.hi, y1.hi);
+    out[2][q] = T16<DT>::pack2(x0.lo, x1.lo);
+    out[3][q] = T16<DT>::pack2(y0.lo, y1.lo);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(row + i * P) = out[i];
+}
+
+// bfloat16.  Grid (ceil(P / 2048), min(M, 65535)), 256 threads; P = 64 ceil(N / 64).
+template <bool VEC>
 __global__ __launch_bounds__(256) void glu_grad_kernel(const uint16_t* __restrict__ d,
                                                        const float* __restrict__ gf,
                                                        const float* __restrict__ uf,
                                                        uint16_t* __restrict__ dgu, int64_t M,
                                                        int64_t N, int64_t P, int act) {
-  using T = T16<DT>;
   const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (c >= P) return;
   for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-    const int64_t o = m * N + c;
-    float dv[8], g[8], u[8];
-    if (VEC && c < N) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(d + o);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dv[e] = T::to_f32((uint16_t)(v[e / 2] >> (16 * (e & 1))));
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(gf + o + 4 * q);
-        const f32x4 b = *reinterpret_cast<const f32x4*>(uf + o + 4 * q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[4 * q + e] = a[e];
-          u[4 * q + e] = b[e];
-        }
-      }
-    } else {
+    float x[8], y[8];
+    row_values<kBF16, VEC>(d, gf, uf, m, c, N, act, x, y);
+    put_pairs<kBF16>(dgu + m * 4 * P + c, P, x, y);
+  }
+}
+
+constexpr int kRowThreads = 512;
+
+// float16: a row per workgroup, computed twice, for its largest value and for its pairs (the
+// second time from the L2 or the cache behind it).  undo[m]: the power of two that the sums
+// of row m are multiplied by.  Infinities and NaN stay, and the finite values set the factor.
+template <bool VEC>
+__global__ __launch_bounds__(kRowThreads) void glu_grad_scaled_kernel(
+    const uint16_t* __restrict__ d, const float* __restrict__ gf, const float* __restrict__ uf,
+    uint16_t* __restrict__ dgu, float* __restrict__ undo, int64_t M, int64_t N, int64_t P,
+    int act) {
+  __shared__ uint32_t tops[kRowThreads / 64];
+  const int t = threadIdx.x;
+  for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
+    float x[8], y[8];
+    uint32_t top = 0;                           // bits of the largest magnitude
+    for (int64_t c = 8 * t; c < N; c += 8 * kRowThreads) {
+      row_values<kF16, VEC>(d, gf, uf, m, c, N, act, x, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool in = c + e < N;
-        dv[e] = in ? T::to_f32(d[o + e]) : 0.f;
-        g[e] = in ? gf[o + e] : 0.f;
-        u[e] = in ? uf[o + e] : 0.f;
+        const uint32_t a = __float_as_uint(x[e]) & 0x7fffffffu;
+        const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
+        if (a < 0x7f800000u) top = max(top, a);
+        if (b < 0x7f800000u) top = max(top, b);
       }
     }
-    u32x4 out[4];                               // dg, du, and their rests
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float v[4][2];
+    for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    if ((t & 63) == 0) tops[t >> 6] = top;
+    __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float a, da;
-        act_grad(g[2 * q + e], act, a, da);
-        const Pair<DT> x(dv[2 * q + e] * u[2 * q + e] * da), y(dv[2 * q + e] * a);
-        v[0][e] = x.hi;
-        v[1][e] = y.hi;
-        v[2][e] = x.lo;
-        v[3][e] = y.lo;
+    for (int w = 0; w < kRowThreads / 64; ++w) top = max(top, tops[w]);
+    __syncthreads();
+    // largest in [2^e, 2^(e + 1)): times 2^(14 - e); both factors stay normal numbers
+    const int e = (int)(top >> 23) - 127, k = top ? min(14 - e, 126) : 0;
+    const float factor = __uint_as_float((uint32_t)(127 + k) << 23);
+    if (t == 0) undo[m] = __uint_as_float((uint32_t)(127 - k) << 23);
+    for (int64_t c = 8 * t; c < P; c += 8 * kRowThreads) {
+      row_values<kF16, VEC>(d, gf, uf, m, c, N, act, x, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= factor;
+        y[i] *= factor;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[i][q] = T::pack2(v[i][0], v[i][1]);
+      put_pairs<kF16>(dgu + m * 4 * P + c, P, x, y);
     }
-    uint16_t* row = dgu + m * 4 * P + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(row + i * P) = out[i];
   }
 }
 
@@ -115,18 +183,27 @@ inline unsigned grid_rows(int64_t M) { return (unsigned)(M < 65535 ? M : 65535);
 
 }  // namespace
 
-int launch_glu_grad(const void* d, const float* gf, const float* uf, void* dgu, int64_t M,
-                    int64_t N, int act, int dtype, hipStream_t st) {
+int launch_glu_grad(const void* d, const float* gf, const float* uf, void* dgu, float* undo,
+                    int64_t M, int64_t N, int act, int dtype, hipStream_t st) {
   const int64_t P = 64 * grad_steps(N);
-  const dim3 grid((unsigned)((P + 2047) / 2048), grid_rows(M));
   const bool vec = N % 8 == 0 && (((uintptr_t)d | (uintptr_t)gf | (uintptr_t)uf) & 15u) == 0;
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const uint16_t*)d, gf, uf, (uint16_t*)dgu, M,
-                       N, P, act);
-    return 0;
-  };
-  if (dtype == kBF16) return vec ? go(glu_grad_kernel<kBF16, true>) : go(glu_grad_kernel<kBF16, false>);
-  return vec ? go(glu_grad_kernel<kF16, true>) : go(glu_grad_kernel<kF16, false>);
+  if (dtype == kBF16) {
+    const dim3 grid((unsigned)((P + 2047) / 2048), grid_rows(M));
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const uint16_t*)d, gf, uf, (uint16_t*)dgu,
+                         M, N, P, act);
+    };
+    if (vec) go(glu_grad_kernel<true>);
+    else go(glu_grad_kernel<false>);
+  } else {
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3(grid_rows(M)), dim3(kRowThreads), 0, st, (const uint16_t*)d, gf,
+                         uf, (uint16_t*)dgu, undo, M, N, P, act);
+    };
+    if (vec) go(glu_grad_scaled_kernel<true>);
+    else go(glu_grad_scaled_kernel<false>);
+  }
+  return 0;
 }
 
 int launch_pad_rows(const void* d, void* out, int64_t M, int64_t N, hipStream_t st) {

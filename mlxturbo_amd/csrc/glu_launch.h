@@ -77,15 +77,16 @@ inline int64_t grad_steps(int64_t N) { return (N + 63) / 64; }
 
 // dgu[M, 4 * P] (T), P = 64 * grad_steps(N): dg = d * u * act'(g), du = d * act(g), rounded
 // to T, then what the rounding left of each, rounded to T; zeros past N columns
-// (glu_grad.hip).
-int launch_glu_grad(const void* d, const float* gf, const float* uf, void* dgu, int64_t M,
-                    int64_t N, int act, int dtype, hipStream_t st);
+// (glu_grad.hip).  float16: rows times a power of two, undo[M] its reciprocal.
+int launch_glu_grad(const void* d, const float* gf, const float* uf, void* dgu, float* undo,
+                    int64_t M, int64_t N, int act, int dtype, hipStream_t st);
 
 // Rows of N elements of a 16-bit type to rows of 64 * grad_steps(N), zeros past N.
 int launch_pad_rows(const void* d, void* out, int64_t M, int64_t N, hipStream_t st);
 
 // out[M, K] = d . W1, or with w2 dg . W1 + du . W2 of glu_grad.hip's rows, for quantized
-// W [N, K]; d's rows of ld elements, padded to whole steps of 64 columns with zeros.
+// W [N, K]; d's rows of ld elements, padded to whole steps of 64 columns with zeros.  undo:
+// glu_grad.hip's, with w2 and float16.
 struct GradArgs {
   const void* d;
   int64_t ld;
@@ -93,6 +94,7 @@ struct GradArgs {
   const void *s1, *b1;
   const uint32_t* w2;
   const void *s2, *b2;
+  const float* undo;
   void* out;
   int64_t M, N, K;
 };
@@ -159,10 +161,14 @@ inline WidePlan grad_plan(int64_t M, int64_t N, int64_t K, int bits, int banks, 
 constexpr int kGradSplits = 48;
 
 // Workspace of a product past one matrix (banks 1) or two: d's padded rows where N is
-// not whole steps (banks 2: dgu), then the split planes.
+// not whole steps (banks 2: undo, then dgu), then the split planes.
+inline size_t grad_undo_bytes(int64_t M, int banks) {
+  return banks == 2 ? ((size_t)M * 4 + 255) & ~(size_t)255 : 0;
+}
 inline size_t grad_rows_bytes(int64_t M, int64_t N, int banks) {
   if (banks == 1 && N % 64 == 0) return 0;
-  return ((size_t)M * (size_t)grad_row(N, banks) * 2 + 255) & ~(size_t)255;
+  return grad_undo_bytes(M, banks) +
+         (((size_t)M * (size_t)grad_row(N, banks) * 2 + 255) & ~(size_t)255);
 }
 inline size_t grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int banks, int cus) {
   return grad_rows_bytes(M, N, banks) +

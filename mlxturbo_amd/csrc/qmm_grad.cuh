@@ -427,14 +427,15 @@ __device__ __forceinline__ void grad_tile(
 // PAIR: both matrices, and d as two T numbers whose sum is a value (glu_grad.hip): rows of
 // the first matrix's columns and the second's, 64 nst of each, then the second numbers in the
 // same order.  A tile is then BM / 2 rows, the first numbers in its upper half and the second
-// in its lower, whose sums are added in registers; grid.y = ceil(M / (BM / 2)).
+// in its lower, whose sums are added in registers; grid.y = ceil(M / (BM / 2)).  In float16
+// row m's sums are multiplied by undo[m].
 template <int DT, int BITS, int GS, int BM, bool PAIR>
 __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
     const uint16_t* __restrict__ d, int64_t ld, const uint32_t* __restrict__ w1,
     const uint16_t* __restrict__ s1, const uint16_t* __restrict__ b1,
     const uint32_t* __restrict__ w2, const uint16_t* __restrict__ s2,
-    const uint16_t* __restrict__ b2, uint16_t* __restrict__ out, float* __restrict__ part, int M,
-    int N, int K, int nst, int splits) {
+    const uint16_t* __restrict__ b2, const float* __restrict__ undo, uint16_t* __restrict__ out,
+    float* __restrict__ part, int M, int N, int K, int nst, int splits) {
   __shared__ __align__(16) unsigned char A0[StreamLds<BM>::kStage + 4 * kGradWaveLds];
   __shared__ __align__(16) unsigned char A1[StreamLds<BM>::kStage];
   __shared__ __align__(16) unsigned char A2[StreamLds<BM>::kStage + 4 * kGradWaveLds];
@@ -453,9 +454,15 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
     return (uint32_t)(min(r - (low ? R : 0), mrows - 1) * ld) * 2u + (low ? 128u * ns : 0u);
   };
   const bool vec = (uintptr_t)out % 16 == 0;    // K is whole eights
-  auto put_block = [&](int i, int j, const f32x16& acc) {
+  // the sums of tile row r (the last of the tile past M)
+  auto scaled = [&](int r, const f32x16& v) {
+    if constexpr (PAIR && DT == kF16) return v * undo[m0 + min(r, mrows - 1)];
+    else return v;
+  };
+  auto put_block = [&](int i, int j, const f32x16& sums) {
     const int r = 32 * i + lr;
     if (r >= mrows) return;
+    const f32x16 acc = scaled(r, sums);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int c = 64 * wave + 32 * j + 8 * q + 4 * h;
@@ -502,7 +509,7 @@ __global__ __launch_bounds__(256, BM <= 64 ? 2 : 1) void qmm_grad_kernel(
       const int r = 32 * i + lr;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const f32x16 v = sums(i, j);
+        const f32x16 v = scaled(r, sums(i, j));
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<u32x2*>(L + r * 128 + (((4 * j + q) ^ row_swz(r)) << 4) + 8 * h) =
@@ -536,7 +543,7 @@ int GradLaunch<DT, BITS, GS>::run(const GradArgs& a, const WidePlan& plan, void*
     hipLaunchKernelGGL((qmm_grad_kernel<DT, BITS, GS, BM, decltype(pairc)::value>), grid,
                        dim3(256), 0, st, (const uint16_t*)a.d, a.ld, a.w1, (const uint16_t*)a.s1,
                        (const uint16_t*)a.b1, a.w2, (const uint16_t*)a.s2, (const uint16_t*)a.b2,
-                       (uint16_t*)a.out, part, (int)a.M, (int)a.N, (int)a.K,
+                       a.undo, (uint16_t*)a.out, part, (int)a.M, (int)a.N, (int)a.K,
                        (int)grad_steps(a.N), plan.splits);
   };
   auto go = [&](auto bmc) {

@@ -10,7 +10,8 @@ The weights are constants: gradients go to x alone, as adapters below a quantize
 layer are trained.  Sums are float; in the gradient of the block, the gate and up
 products are kept in float between forward and backward (8 bytes per output), and the
 products' inputs ``d u act'(g)`` and ``d act(g)`` are two 16-bit numbers each (the value
-rounded, and the rest), so that x's gradient is rounded once, as that of float32 products is.
+rounded, and the rest), in float16 scaled by rows, so that x's gradient is rounded once and in
+range as that of float32 products is.
 """
 
 from __future__ import annotations

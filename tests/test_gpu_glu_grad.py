@@ -136,3 +136,48 @@ def test_sizes_without_a_kernel(dtype, monkeypatch):
     off += 450 * 2.0 ** -23 * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
     for v in (got, want):
         check(v, dx, off + _half_step(dx.abs() + off, dtype))
+
+
+@pytest.mark.parametrize("M,bits", [(1, 4), (6, 8), (40, 4), (300, 4)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_range_between(M, bits, dtype):
+    """A scaled loss' gradient and an activation far out: dL/dg and dL/du pass float16's
+    range, and x's gradient does not.  Other rows are ordinary, tiny, or of zeros."""
+    N, K = 200, 128
+    g, x, gate, wg, up, wu = _case(M, N, K, 64, bits, dtype, 4)
+    d = torch.randn((M, N), generator=g, device="cuda").to(dtype)
+    x[0] = (x[0].float() * 400).to(dtype)
+    gv, uv = (x[0].double() @ w.T for w in (wg, wu))
+    av, dav = activation(gv, "silu")
+    d[0] = 0
+    d[0, (dav * uv).abs().argmax()], d[0, av.argmax()] = 600, -400
+    if M > 4:
+        d[1] = 0
+        d[2] = (d[2].float() * 2.0 ** -12).to(dtype)
+        x[3] = 0
+    dg, du, edg, edu = _between(x, d, wg, wu, "silu")
+    dx = dg @ wg + du @ wu
+    assert float(dg.abs().max()) > 65504 and float(du.abs().max()) > 65504
+    assert float(dx.abs().max()) < 60000
+    got = _grad(x, gate, up, "silu", 64, bits, d)
+    # a pair's last place: 2^-25 of float16 on rows whose largest is 2^14 at least
+    last = 2.0 ** -39 * torch.maximum(dg.abs().amax(-1), du.abs().amax(-1))[:, None]
+    rel = (torch.finfo(dtype).eps / 2) ** 2
+    off = (edg + rel * dg.abs() + last) @ wg.abs() + (edu + rel * du.abs() + last) @ wu.abs()
+    off += (2 * N + 20) * 2.0 ** -23 * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    check(got, dx, off + _half_step(dx.abs() + off, dtype))
+    if M > 4:
+        assert not got[1].any()
+
+
+def test_rows_with_infinities():
+    """In float16 a row's factor is of its finite values, and rows that hold an infinity or
+    a NaN stay apart from the others."""
+    g, x, gate, wg, up, wu = _case(9, 72, 128, 64, 4, HF, 5)
+    d = torch.randn((9, 72), generator=g, device="cuda").to(HF)
+    want = _grad(x, gate, up, "silu", 64, 4, d)
+    d[2, 5], d[4, 7], d[4, 8] = float("inf"), float("nan"), 3.0
+    got = _grad(x, gate, up, "silu", 64, 4, d)
+    rest = [r for r in range(9) if r not in (2, 4)]
+    assert torch.equal(got[rest], want[rest])
+    assert not got[2].isfinite().any() and got[4].isnan().all()
