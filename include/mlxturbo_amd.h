@@ -518,8 +518,9 @@ int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_sca
  * d[M, N] . deq(w), float sums, one rounding.  workspace of
  * mq_quantized_matmul_grad_workspace_size(M, N, K, group_size, bits) bytes, 16-byte
  * aligned; it may be NULL where N % 64 == 0 (then nothing splits N).  d and w
- * 16-byte aligned.  MQ_EUNSUPPORTED: no columns, codes of 2^31 bytes and more and rows of
- * d of 2^22 elements and more (N padded to whole 64s in both), 2, 3, 5 and 6 bits, float32.
+ * 16-byte aligned, dx as its type.  MQ_EUNSUPPORTED: no columns, codes of 2^31 bytes and
+ * more and rows of d of 2^22 elements and more (N padded to whole 64s in both), 2, 3, 5 and 6
+ * bits, float32.
  */
 size_t mq_quantized_matmul_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
                                                int bits);
@@ -532,9 +533,9 @@ int mq_quantized_matmul_grad(const void* d, const uint32_t* w, const void* scale
  * x's gradient through mq_quantized_glu: dx = dg . deq(gate) + du . deq(up) with dg =
  * d u act'(g) and du = d act(g) of the forward's float sums g and u, each multiplied as two
  * numbers of the type (the value rounded, and the rest; in float16 rows of them are scaled,
- * so that they may pass its range): float sums, one rounding.  The
- * workspace (mq_quantized_glu_grad_workspace_size bytes, 16-byte aligned) holds them, so it
- * is needed; MQ_EUNSUPPORTED as above (rows of 2 N elements here).
+ * so that they may pass its range): float sums, one rounding.  The workspace
+ * (mq_quantized_glu_grad_workspace_size bytes, 16-byte aligned) holds them, so it is needed;
+ * MQ_EUNSUPPORTED as above (rows of 2 N elements here).
  */
 size_t mq_quantized_glu_grad_workspace_size(int64_t M, int64_t N, int64_t K, int group_size,
                                             int bits);

@@ -559,8 +559,10 @@ int GradLaunch<DT, BITS, GS>::run(const GradArgs& a, const WidePlan& plan, void*
   *nlaunch += 1;
   if (part) {
     const int64_t MK = a.M * a.K;
-    hipLaunchKernelGGL((wide_reduce_kernel<DT, true>), dim3((unsigned)((MK + 1023) / 1024)),
-                       dim3(256), 0, st, part, (uint16_t*)a.out, MK, plan.splits);
+    const auto kern = (uintptr_t)a.out % 8 == 0 ? wide_reduce_kernel<DT, true>
+                                                : wide_reduce_kernel<DT, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((MK + 1023) / 1024)), dim3(256), 0, st, part,
+                       (uint16_t*)a.out, MK, plan.splits);
     *nlaunch += 1;
   }
   return 0;

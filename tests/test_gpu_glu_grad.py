@@ -181,3 +181,33 @@ def test_rows_with_infinities():
     rest = [r for r in range(9) if r not in (2, 4)]
     assert torch.equal(got[rest], want[rest])
     assert not got[2].isfinite().any() and got[4].isnan().all()
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("M,N,K", [(40, 1500, 256), (2100, 64, 8192)])
+def test_gradient_at_any_address(M, N, K, both):
+    """The C entries with x's gradient at two-byte addresses, its sums split and whole: the
+    same bits, and nothing written beside them."""
+    lib = mq._lib.lib()
+    g, x, gate, _, up, _ = _case(M, N, K, 64, 4, BF, 6)
+    d = torch.randn((M, N), generator=g, device="cuda").to(BF)
+    sums = [torch.randn((M, N), generator=g, device="cuda") for _ in range(2)]
+    size = lib.mq_quantized_glu_grad_workspace_size if both else lib.mq_quantized_matmul_grad_workspace_size
+    ws = torch.empty(size(M, N, K, 64, 4), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    got = []
+    for off in (0, 1, 2, 4):
+        buf = torch.full((M * K + 16,), 7.0, dtype=BF, device="cuda")
+        dx = buf[off:].data_ptr()
+        if both:
+            rc = lib.mq_quantized_glu_grad(
+                d.data_ptr(), *[t.data_ptr() for t in (*sums, *gate, *up)], dx, M, N, K, 64, 4, 0,
+                0, ws.data_ptr(), ws.numel(), stream)
+        else:
+            rc = lib.mq_quantized_matmul_grad(
+                d.data_ptr(), *[t.data_ptr() for t in gate], dx, M, N, K, 64, 4, 0, ws.data_ptr(),
+                ws.numel(), stream)
+        assert rc == 0
+        assert (buf[:off] == 7).all() and (buf[off + M * K:] == 7).all()
+        got.append(buf[off:off + M * K])
+    assert got[0].isfinite().all() and all(torch.equal(t, got[0]) for t in got)
