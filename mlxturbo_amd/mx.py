@@ -14,6 +14,9 @@ every group is not pinned by any test here.
   type, what :func:`ops.dequantize` gives, rounded once to T.  In float16 a
   scale beyond 2**13 overflows as its dequantized values do.  qqmm multiplies
   codes and scales as they are, with no rounding to T before the sums.
+* gradients: quantized_matmul has x's, ``d @ dequantize(w)`` as a GPU GEMM over the
+  dequantized weights, which are constants.  qqmm quantizes x, which has none: its backward
+  pass raises.
 
 The operators of :mod:`mlxturbo_amd.ops` call these for the mode; arguments and
 errors are theirs.
@@ -27,7 +30,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib, ops
+from . import _lib, glu, ops
 
 GROUP_SIZE = 32
 BITS = 4
@@ -162,6 +165,33 @@ def _product(call, size, x, w, s, out, M: int, N: int, K: int) -> int:
                    size(M, N, K) if M > 16 else 0)   # up to 16 rows use none
 
 
+class _Matmul(torch.autograd.Function):
+    """quantized_matmul by its kernels, with x's gradient."""
+
+    @staticmethod
+    def forward(ctx, x, w, scales):
+        glu._constants(ctx, (w, scales))
+        return quantized_matmul(x, w, scales, None, True)
+
+    @staticmethod
+    @glu._first_order
+    def backward(ctx, d):
+        deq = dequantize(*glu._same_constants(ctx), dtype=d.dtype)
+        return (d.reshape(-1, deq.shape[0]) @ deq).reshape(*d.shape[:-1], deq.shape[1]), None, None
+
+
+class _QQMatmul(torch.autograd.Function):
+    """qqmm, as part of a graph that cannot be gone through."""
+
+    @staticmethod
+    def forward(ctx, x, w, scales):
+        return qqmm(x, w, scales)
+
+    @staticmethod
+    def backward(ctx, d):
+        raise NotImplementedError("qqmm: x is quantized, which has no gradient")
+
+
 def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
     _no_biases(biases)
     dev = ops._require_gpu(x, w, scales)
@@ -181,6 +211,11 @@ def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
             f"x last dimension {x.shape[-1]} does not match the quantized weight K={K}")
     if not transpose or x.dtype == torch.float32:
         return _composed(x, w, scales, transpose)
+    if glu.wants_grad(x):
+        leaf = glu.note_leaf(x)
+        out = _Matmul.apply(x, w, scales)
+        del leaf
+        return out
     lead = tuple(x.shape[:-1])
     M = math.prod(lead)
     out = torch.empty((*lead, N), dtype=x.dtype, device=dev)
@@ -209,6 +244,8 @@ def qqmm(x, w, scales) -> torch.Tensor:
     _float_type(x.dtype)
     if x.ndim < 1 or x.shape[-1] != K:
         raise ValueError(f"x {tuple(x.shape)} does not match the quantized weight K={K}")
+    if glu.wants_grad(x):
+        return _QQMatmul.apply(x, w, scales)
     N = w.shape[0]
     lead = tuple(x.shape[:-1])
     M = math.prod(lead)

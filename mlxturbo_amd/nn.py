@@ -197,7 +197,8 @@ class QuantizedMLP(torch.nn.Module):
     """mlx-lm's dense ``MLP``: ``down_proj(act(gate_proj(x)) * up_proj(x))``, the first
     half as :func:`ops.quantized_glu` where gate and up are affine layers of one
     format without bias, else as the two layers and the activation in float.
-    Where x requires grad, the backward pass gives its gradient."""
+    Where x requires grad, the backward pass gives its gradient (a :class:`QQLinear`,
+    which quantizes its activations, refuses it there)."""
 
     def __init__(self, gate_proj: QuantizedLinear, up_proj: QuantizedLinear,
                  down_proj: QuantizedLinear, activation: str = "silu"):

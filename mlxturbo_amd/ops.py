@@ -281,8 +281,8 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     dequantize plus one GPU GEMM (:func:`_composed_qmm`).  ``mode="mxfp4"``
     (uint8 scales, no biases) takes the same x and gives x's dtype.
 
-    Where ``x`` requires grad, so does the affine result: the backward pass gives x's
-    gradient ``d @ dequantize(w)`` (mq_quantized_matmul_grad where the forward ran on
+    Where ``x`` requires grad, so does the result: the backward pass gives x's
+    gradient ``d @ dequantize(w)`` (mq_quantized_matmul_grad where an affine forward ran on
     the kernels); the weights are constants.
     """
     group_size, bits = _format(group_size, bits, mode)
@@ -329,7 +329,8 @@ def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
          mode: str = "mxfp4") -> torch.Tensor:
     """``mx.qqmm``: ``x`` is quantized along its last axis in the weight's
     format and multiplied there, ``dequantize(quantize(x)) @ dequantize(w).T``
-    with float sums over the exact values, rounded once to x's dtype.  ``w``
+    with float sums over the exact values, rounded once to x's dtype.  Quantizing x has
+    no gradient: a backward pass that reaches it raises.  ``w``
     ``[N, K/8]`` and ``scales`` ``[N, K/32]`` are :func:`quantize`'s.  Both
     operands enter the MFMAs as codes with their scales; the mode is mxfp4."""
     _format(group_size, bits, mode)
