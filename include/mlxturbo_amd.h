@@ -61,10 +61,11 @@ uint64_t mq_launch_count(void);
  * tolerance of all of them, not bit-identical to the same row computed in
  * a call of another width.  With on != 0, calls of 1 to 32 rows all run the
  * 2..32-row kernel family, so a row's result does not depend on which of
- * these row counts the call has (decode vs. speculative verify).  The
- * reference keeps this property with its opt-in small-M route: rows of an
- * M = 2..8 call bit-identical to the M = 1 call
- * (kernels/qmv_small_m.py:289-307, dispatch.py:337-347).
+ * these row counts the call has (decode vs. speculative verify); so do
+ * mq_quantized_glu's, on its kernel of 2..16 rows.  The reference keeps this
+ * property with its opt-in small-M route: rows of an M = 2..8 call
+ * bit-identical to the M = 1 call (kernels/qmv_small_m.py:289-307,
+ * dispatch.py:337-347).
  * Returns the previous setting.  Not for calls running concurrently with a
  * change of the setting; workspaces are to be sized under the setting that
  * the call runs under.

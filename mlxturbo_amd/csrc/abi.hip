@@ -967,7 +967,8 @@ int mq_mxfp4_gather_qmm(const void* x, const uint32_t* w, const uint8_t* scales,
 
 size_t mq_quantized_glu_workspace_size(int64_t M, int64_t N, int64_t K, int group_size, int bits) {
   if (M <= 0 || N <= 0 || K <= 0 || (bits != 4 && bits != 8) || group_size <= 0) return 0;
-  return mq::glu_workspace_bytes(M, N, K, bits, mq::device_cu_count());
+  return mq::glu_workspace_bytes(M, N, K, bits, mq::device_cu_count(),
+                                 g_row_identity.load(std::memory_order_relaxed) != 0);
 }
 
 int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_scales,
@@ -986,15 +987,18 @@ int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_sca
   const mq::GluArgs a{x,  gate_w, gate_scales, gate_biases, up_w, up_scales, up_biases, out, gate_sums,
                       up_sums, M, N, K, activation};
   int nl = 0;
-  if (mq::glu_wide_route(M, N, K)) {
+  const bool row_identity = g_row_identity.load(std::memory_order_relaxed) != 0;
+  if (mq::glu_wide_route(M, K, row_identity)) {
     const int cus = mq::device_cu_count();
     mq::WidePlan plan = mq::glu_wide_plan(M, N, K, bits, cus, 16);
-    if (plan.splits > 1 && (!workspace || workspace_bytes < mq::glu_workspace_bytes(M, N, K, bits, cus)))
+    if (plan.splits > 1 &&
+        (!workspace ||
+         workspace_bytes < mq::glu_workspace_bytes(M, N, K, bits, cus, row_identity)))
       plan = mq::glu_wide_plan(M, N, K, bits, cus, 1);
     rc = dispatch_16<mq::GluWideLaunch>(dtype, bits, group_size, a, plan, workspace, st, &nl);
   } else {
     int64_t m0 = 0;
-    if (M == 1) {
+    if (M == 1 && !row_identity) {
       rc = dispatch_16<mq::GluQuadLaunch>(dtype, bits, group_size, a, st);
       if (rc == mq::kStatusUnsupported) {
         rc = MQ_OK;
@@ -1005,7 +1009,8 @@ int mq_quantized_glu(const void* x, const uint32_t* gate_w, const void* gate_sca
     }
     for (; m0 < M && !rc; m0 += mq::kGluSkinnyRows) {
       const int64_t m = M - m0 < mq::kGluSkinnyRows ? M - m0 : mq::kGluSkinnyRows;
-      rc = dispatch_16<mq::GluSkinnyLaunch>(dtype, bits, group_size, a, m0, m, st);
+      rc = dispatch_16<mq::GluSkinnyLaunch>(dtype, bits, group_size, a, m0, m,
+                                            row_identity ? (int64_t)mq::kGluSkinnyRows : m, st);
       ++nl;
     }
   }

@@ -337,7 +337,8 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
 constexpr int kGluLdsMax = 160 * 1024 - 1024;
 
 template <int DT, int BITS, int GS>
-int GluSkinnyLaunch<DT, BITS, GS>::run(const GluArgs& a, int64_t m0, int64_t M, hipStream_t st) {
+int GluSkinnyLaunch<DT, BITS, GS>::run(const GluArgs& a, int64_t m0, int64_t M, int64_t rows,
+                                       hipStream_t st) {
   constexpr int UC = GluGeom<BITS>::UC;
   const int64_t tiles = (a.N + kGluCols - 1) / kGluCols, S = (a.K + UC - 1) / UC;
   const int cus = device_cu_count();
@@ -350,7 +351,7 @@ int GluSkinnyLaunch<DT, BITS, GS>::run(const GluArgs& a, int64_t m0, int64_t M, 
   size_t lds = 0;
   for (int64_t n = 1;; ++n) {
     slice = (S + n - 1) / n;
-    lds = glu_slice_bytes<BITS, GS>(M, most, (int)slice) + (slice < S ? kGluSum : 0);
+    lds = glu_slice_bytes<BITS, GS>(rows, most, (int)slice) + (slice < S ? kGluSum : 0);
     if (lds <= (size_t)kGluLdsMax) break;
   }
   const auto kern = &glu_skinny_kernel<DT, BITS, GS>;

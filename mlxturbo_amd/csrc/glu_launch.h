@@ -25,11 +25,12 @@ struct GluArgs {
   int act;
 };
 
-// Rows m0 .. m0 + M - 1 (M <= kGluSkinnyRows), one launch.
+// Rows m0 .. m0 + M - 1 (M <= kGluSkinnyRows), one launch, with K in the slices that a
+// launch of `rows` rows (M or more) needs: its sums' order.
 constexpr int kGluSkinnyRows = 16;
 template <int DT, int BITS, int GS>
 struct GluSkinnyLaunch {
-  static int run(const GluArgs& a, int64_t m0, int64_t M, hipStream_t st);
+  static int run(const GluArgs& a, int64_t m0, int64_t M, int64_t rows, hipStream_t st);
 };
 
 // One row, in waves of 4 rows of either matrix (qmv_quad.cuh), one launch;
@@ -58,14 +59,15 @@ inline WidePlan glu_wide_plan(int64_t M, int64_t N, int64_t K, int bits, int cus
   return wide_plan(M, 2 * N, K, bits, cus, max_splits);
 }
 
-// Rows from which the MFMA tile runs.
-inline bool glu_wide_route(int64_t M, int64_t N, int64_t K) {
-  (void)N;
-  return M > kGluSkinnyRows && glu_wide_eligible(M, K);
+// Whether the MFMA tile runs.  row_identity (mq_set_row_identity): calls of up to 32 rows all
+// run launches of the few-row kernel in the slices of its 16.
+inline bool glu_wide_route(int64_t M, int64_t K, bool row_identity) {
+  return M > (row_identity ? 32 : kGluSkinnyRows) && glu_wide_eligible(M, K);
 }
 
-inline size_t glu_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int cus) {
-  if (!glu_wide_route(M, N, K)) return 0;
+inline size_t glu_workspace_bytes(int64_t M, int64_t N, int64_t K, int bits, int cus,
+                                  bool row_identity) {
+  if (!glu_wide_route(M, K, row_identity)) return 0;
   const WidePlan p = glu_wide_plan(M, N, K, bits, cus, 16);
   return p.splits > 1 ? (size_t)p.splits * 2 * (size_t)M * (size_t)glu_plane(N) * sizeof(float) : 0;
 }

@@ -1302,8 +1302,8 @@ def launch_count() -> int:
 
 
 def set_row_identity(on: bool) -> bool:
-    """Run every ``quantized_matmul`` call of 1 to 32 rows on the 2..32-row
-    kernel family, so every output row is bit-identical whatever the number of
+    """Run every ``quantized_matmul`` and ``quantized_glu`` call of 1 to 32 rows on
+    their kernels of 2 rows and more, so every output row is bit-identical whatever the number of
     rows in the call (a decode step and a speculative verify of the same token
     agree bit for bit).  Off by default: one-row calls then take their own
     faster kernel, and calls of 17-32 rows the wide tile where that is the
