@@ -193,10 +193,25 @@ class QQLinear(QuantizedLinear):
         return super().from_linear(weight, bias, group_size, bits, mode)
 
 
+_OWN_CALL = (QuantizedLinear.forward, QuantizedLinear.quantized_forward)
+
+
+def _is_its_product(m) -> bool:
+    """Whether calling ``m`` is :class:`QuantizedLinear`'s own product and no more: no
+    subclass's or instance's forward, no routing (:mod:`dispatch`), no hooks."""
+    return (isinstance(m, QuantizedLinear)
+            and (type(m).forward, type(m).quantized_forward) == _OWN_CALL
+            and not {"forward", "quantized_forward"} & m.__dict__.keys()
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
+                     or m._backward_pre_hooks)
+            and not torch.nn.modules.module._has_any_global_hook())
+
+
 class QuantizedMLP(torch.nn.Module):
     """mlx-lm's dense ``MLP``: ``down_proj(act(gate_proj(x)) * up_proj(x))``, the first
-    half as :func:`ops.quantized_glu` where gate and up are affine layers of one
-    format without bias, else as the two layers and the activation in float.
+    half as :func:`ops.quantized_glu` where gate and up are plain affine layers of one
+    format without bias, else (other formats, adapters around a layer, hooks, routed
+    layers) as the two modules called and the activation in float.
     Where x requires grad, the backward pass gives its gradient (a :class:`QQLinear`,
     which quantizes its activations, refuses it there)."""
 
@@ -213,7 +228,8 @@ class QuantizedMLP(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         g, u = self.gate_proj, self.up_proj
-        if (g.mode == "affine" and g.bias is None and u.bias is None
+        if (_is_its_product(g) and _is_its_product(u)
+                and g.mode == "affine" and g.bias is None and u.bias is None
                 and g.weight.shape == u.weight.shape and g.scales.dtype == u.scales.dtype
                 and (g.group_size, g.bits, g.mode) == (u.group_size, u.bits, u.mode)):
             h = ops.quantized_glu(x, (g.weight, g.scales, g.biases),

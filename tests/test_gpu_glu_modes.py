@@ -57,3 +57,100 @@ def test_row_identity_of_an_mlp():
         one = torch.cat([mlp(x[m:m + 1]) for m in range(32)])
         for M in (2, 8, 16, 20, 32):
             assert torch.equal(mlp(x[:M]), one[:M])
+
+
+def _layers(seed, **kw):
+    g = _gen(seed)
+    return [QuantizedLinear.from_linear((torch.randn((n, k), generator=g, device="cuda") * 0.05).to(BF),
+                                        **kw) for n, k in ((192, 128), (192, 128), (128, 192))]
+
+
+def _stepwise(mlp, x):
+    gv, uv = mlp.gate_proj(x), mlp.up_proj(x)
+    return mlp.down_proj((torch.nn.functional.silu(gv.float()) * uv.float()).to(gv.dtype))
+
+
+class Adapted(torch.nn.Module):
+    """A frozen layer and a low-rank adapter."""
+
+    def __init__(self, base, rank=4):
+        super().__init__()
+        g = _gen(7)
+        self.base = base
+        self.a = torch.nn.Parameter(torch.randn((rank, base.input_dims), generator=g, device="cuda")
+                                    .to(BF) * 0.1)
+        self.b = torch.nn.Parameter(torch.randn((base.output_dims, rank), generator=g, device="cuda")
+                                    .to(BF) * 0.1)
+
+    def forward(self, x):
+        return self.base(x) + x @ self.a.T @ self.b.T
+
+
+class Doubled(QuantizedLinear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class DoubledProduct(QuantizedLinear):
+    def quantized_forward(self, x):
+        return 2 * super().quantized_forward(x)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("kind", ["adapter", "subclass", "product", "instance", "pre_hook", "hook",
+                                  "global_hook", "routed"])
+def test_mlp_calls_layers_that_are_not_plain(kind, which):
+    """Gate or up wrapped, subclassed, hooked or routed: the MLP's result is of its call."""
+    layers = _layers(3)
+    x = torch.randn((40, 128), generator=_gen(4), device="cuda").to(BF)
+    plain = QuantizedMLP(*layers)(x)
+    layer, calls, handle = layers[which], [], None
+    if kind == "adapter":
+        layers[which] = Adapted(layer)
+    elif kind in ("subclass", "product"):
+        layer.__class__ = Doubled if kind == "subclass" else DoubledProduct
+    elif kind == "instance":
+        layer.forward = lambda v: 2 * QuantizedLinear.forward(layer, v)
+    elif kind == "pre_hook":
+        layer.register_forward_pre_hook(lambda m, a: (2 * a[0],))
+    elif kind == "hook":
+        layer.register_forward_hook(lambda m, a, y: 2 * y)
+    elif kind == "global_hook":
+        handle = torch.nn.modules.module.register_module_forward_hook(
+            lambda m, a, y: 2 * y if m is layer else None)
+    elif kind == "routed":
+        mq.dispatch.enable(layer)
+        seen = mq.dispatch.quantized_matmul
+        mq.dispatch.quantized_matmul = lambda *a, **k: calls.append(1) or seen(*a, **k)
+    try:
+        mlp = QuantizedMLP(*layers)
+        y = mlp(x)
+        assert torch.equal(y, _stepwise(mlp, x))
+        if kind == "routed":
+            assert calls
+        else:
+            assert not torch.allclose(y.float(), plain.float(), rtol=0.05)
+        if kind == "adapter":
+            y.float().sum().backward()
+            assert mlp.get_submodule(("gate_proj", "up_proj")[which]).b.grad.any()
+    finally:
+        if handle is not None:
+            handle.remove()
+        if kind == "routed":
+            mq.dispatch.quantized_matmul = seen
+    if kind in ("instance", "routed"):
+        layer.__dict__.pop("forward", None)
+        mq.dispatch.disable(layer)
+        assert torch.equal(mlp(x), plain)
+
+
+def test_mlp_under_the_class_patch():
+    mlp = QuantizedMLP(*_layers(5))
+    x = torch.randn((3, 128), generator=_gen(6), device="cuda").to(BF)
+    plain = mlp(x)
+    mq.dispatch.enable_class()
+    try:
+        assert torch.equal(mlp(x), _stepwise(mlp, x))
+    finally:
+        mq.dispatch.disable_class()
+    assert torch.equal(mlp(x), plain)
