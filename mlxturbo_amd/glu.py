@@ -20,6 +20,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -34,6 +35,12 @@ def elsewhere(dev: torch.device) -> bool:
 
 def wants_grad(x: torch.Tensor) -> bool:
     return x.requires_grad and torch.is_grad_enabled()
+
+
+def differentiated(x: torch.Tensor) -> bool:
+    """Whether a call on x is part of a graph, or x has a forward-mode tangent."""
+    return (x.requires_grad and torch.is_grad_enabled()
+            or forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None)
 
 
 def _workspace(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
@@ -51,7 +58,7 @@ def note_leaf(x: torch.Tensor):
     is made by the first graph of it that lives and keeps that graph's stream, and a
     captured backward that reaches it from another stream ends the process.  Returns the
     accumulator, which the caller holds until the graph does (else it and the note are gone)."""
-    if not x.is_leaf:
+    if not (x.is_leaf and x.requires_grad):
         return None
     node = torch.autograd.graph.get_gradient_edge(x).node
     meta = node.metadata
@@ -124,10 +131,9 @@ def _glu_grad(d, g, u, flat, act: int, group_size: int, bits: int) -> torch.Tens
                                    group_size, bits, ops._DTYPE_CODE[d.dtype], act, *_room(ws),
                                    ops._stream_ptr(dx))
     if rc == ops._EUNSUPPORTED:                       # beyond the kernel's address ranges
-        name = next(k for k, v in ACTIVATIONS.items() if v == act)
         with torch.enable_grad():
             gg, uu = g.detach().requires_grad_(), u.detach().requires_grad_()
-            dg, du = torch.autograd.grad(_activation(gg, name) * uu, (gg, uu), d.float())
+            dg, du = torch.autograd.grad(_activation(gg, _name(act)) * uu, (gg, uu), d.float())
         for i, t in enumerate((dg, du)):              # float products, as the kernels' sums are
             w = ops.dequantize(*flat[3 * i:3 * i + 3], group_size, bits).float()
             out = torch.addmm(out, t, w) if i else torch.mm(t, w)
@@ -170,8 +176,21 @@ class _Glu(torch.autograd.Function):
         out, g, u = r
         ctx.args = act, group_size, bits
         ctx.save_for_backward(g, u)
+        ctx.sums = (g, u) if forward_ad._current_level >= 0 else None
         _constants(ctx, flat)
         return out
+
+    @staticmethod
+    def jvp(ctx, t, *_):
+        """h's tangent; those of the two products are rounded to their type."""
+        (g, u), ctx.sums = ctx.sums, None
+        act, *form = ctx.args
+        tg, tu = (ops.quantized_matmul(t, *ctx.flat[i:i + 3], True, *form).float() for i in (0, 3))
+        with torch.enable_grad():
+            leaf = g.detach().requires_grad_()
+            a = _activation(leaf, _name(act))
+            da, = torch.autograd.grad(a, leaf, torch.ones_like(a))
+        return (da * tg * u + a.detach() * tu).to(t.dtype)
 
     @staticmethod
     @_first_order
@@ -190,15 +209,19 @@ class _Matmul(torch.autograd.Function):
         return ops.quantized_matmul(x, *flat, True, group_size, bits)
 
     @staticmethod
+    def jvp(ctx, t, *_):
+        return ops.quantized_matmul(t, *ctx.flat, True, *ctx.args)
+
+    @staticmethod
     @_first_order
     def backward(ctx, d):
         return matmul_grad(d, *_same_constants(ctx), *ctx.args), None, None, None
 
 
 def quantized_matmul_differentiable(x, w, scales, biases, group_size: int, bits: int):
-    """:func:`ops.quantized_matmul` of checked kernel-path arguments whose x wants a
-    gradient."""
-    if any(t.requires_grad for t in (scales, biases)):
+    """:func:`ops.quantized_matmul` of checked kernel-path arguments whose x is
+    differentiated."""
+    if wants_grad(x) and any(t.requires_grad for t in (scales, biases)):
         raise NotImplementedError("quantized_matmul: scales and biases are constants here; "
                                   "gradients go to x")
     leaf = note_leaf(x)
@@ -207,6 +230,10 @@ def quantized_matmul_differentiable(x, w, scales, biases, group_size: int, bits:
     y = _Matmul.apply(x2, flat, group_size, bits)
     del leaf
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
+
+
+def _name(act: int) -> str:
+    return next(k for k, v in ACTIVATIONS.items() if v == act)
 
 
 def _activation(g: torch.Tensor, activation: str) -> torch.Tensor:
@@ -240,7 +267,8 @@ def quantized_glu(x: torch.Tensor, gate, up, activation: str = "silu",
     the biases).
 
     Where ``x`` requires grad, so does the result: the backward pass gives x's
-    gradient (``gate`` and ``up`` are constants; mxfp4 has none)."""
+    gradient (``gate`` and ``up`` are constants; mxfp4 has none).  A forward-mode
+    tangent of x gives the result's."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
     group_size, bits = ops._format(group_size, bits, mode)
@@ -271,8 +299,8 @@ def quantized_glu(x: torch.Tensor, gate, up, activation: str = "silu",
         ops._check_quant(*up, group_size, bits)       # (the rest is the gate's: says what differs)
     if x.ndim < 1 or x.shape[-1] != K:
         raise ValueError(f"x {tuple(x.shape)} does not match the quantized weight K={K}")
-    grad = wants_grad(x)
-    if grad and any(t.requires_grad for t in (*gate[1:], *up[1:])):
+    grad = differentiated(x)
+    if wants_grad(x) and any(t.requires_grad for t in (*gate[1:], *up[1:])):
         raise NotImplementedError("quantized_glu: scales and biases are constants here; "
                                   "gradients go to x")
     if K == 0 or not (bits in (4, 8) and ops._kernel_dtype(x.dtype, gate[1].dtype)):

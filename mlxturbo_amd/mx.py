@@ -174,6 +174,10 @@ class _Matmul(torch.autograd.Function):
         return quantized_matmul(x, w, scales, None, True)
 
     @staticmethod
+    def jvp(ctx, t, *_):
+        return quantized_matmul(t, *ctx.flat, None, True)
+
+    @staticmethod
     @glu._first_order
     def backward(ctx, d):
         deq = dequantize(*glu._same_constants(ctx), dtype=d.dtype)
@@ -189,6 +193,10 @@ class _QQMatmul(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d):
+        raise NotImplementedError("qqmm: x is quantized, which has no gradient")
+
+    @staticmethod
+    def jvp(ctx, t, *_):
         raise NotImplementedError("qqmm: x is quantized, which has no gradient")
 
 
@@ -211,7 +219,7 @@ def quantized_matmul(x, w, scales, biases, transpose: bool) -> torch.Tensor:
             f"x last dimension {x.shape[-1]} does not match the quantized weight K={K}")
     if not transpose or x.dtype == torch.float32:
         return _composed(x, w, scales, transpose)
-    if glu.wants_grad(x):
+    if glu.differentiated(x):
         leaf = glu.note_leaf(x)
         out = _Matmul.apply(x, w, scales)
         del leaf
@@ -244,7 +252,7 @@ def qqmm(x, w, scales) -> torch.Tensor:
     _float_type(x.dtype)
     if x.ndim < 1 or x.shape[-1] != K:
         raise ValueError(f"x {tuple(x.shape)} does not match the quantized weight K={K}")
-    if glu.wants_grad(x):
+    if glu.differentiated(x):
         return _QQMatmul.apply(x, w, scales)
     N = w.shape[0]
     lead = tuple(x.shape[:-1])

@@ -283,7 +283,8 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
 
     Where ``x`` requires grad, so does the result: the backward pass gives x's
     gradient ``d @ dequantize(w)`` (mq_quantized_matmul_grad where an affine forward ran on
-    the kernels); the weights are constants.
+    the kernels); the weights are constants.  A forward-mode tangent of ``x`` gives the
+    result's.
     """
     group_size, bits = _format(group_size, bits, mode)
     if mode == "mxfp4":
@@ -301,7 +302,7 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
             f"x last dimension {x.shape[-1]} does not match the quantized weight K={K}")
     if not (transpose and bits in (4, 8) and _kernel_dtype(x.dtype, scales.dtype)):
         return _composed_qmm(x, w, scales, biases, transpose, group_size, bits)
-    if x.requires_grad and torch.is_grad_enabled():
+    if _glu.differentiated(x):
         return _glu.quantized_matmul_differentiable(x, w, scales, biases, group_size, bits)
     code = _DTYPE_CODE[x.dtype]
     lead = tuple(x.shape[:-1])
@@ -383,7 +384,7 @@ def quantized_matmul_prepared(x: torch.Tensor, p: PreparedWeights) -> torch.Tens
     shape = x.shape
     N, K = p.N, p.K
     if (p.code is None or x.dtype != p.dtype or x.get_device() != p.index or not shape
-            or shape[-1] != K or x.requires_grad and torch.is_grad_enabled()):
+            or shape[-1] != K or _glu.differentiated(x)):
         return quantized_matmul(x, p.w, p.s, p.b, group_size=p.group_size, bits=p.bits)
     M = x.numel() // K
     out = torch.empty((*shape[:-1], N), dtype=p.dtype, device=p.dev)
