@@ -67,6 +67,19 @@ __host__ __device__ inline size_t glu_slice_bytes(int64_t M, int tiles, int unit
   return ((n > (size_t)kGluPart ? n : (size_t)kGluPart) + 15) & ~(size_t)15;
 }
 
+// A lane's weight row in a tile whose first is row n0 (the last one, past N), and its byte of
+// unit s in a row of rowB: chunks past the row read its last one.
+__host__ __device__ inline int glu_lane_row(int lane, int64_t n0, int N) {
+  const int last = (int)(N - 1 - n0), r = lane & 7;
+  return r < last ? r : last;
+}
+__host__ __device__ inline uint32_t glu_lane_byte(int lane, int s, uint32_t rowB) {
+  const uint32_t o = 128u * (uint32_t)s + 16u * (2 * (lane >> 4) + ((lane & 15) >> 3));
+  return o < rowB - 16u ? o : rowB - 16u;
+}
+// Its piece of P groups from group g on of a row's G: past them, the last (and zeros count).
+__host__ __device__ inline int glu_piece_at(int g, int G, int P) { return g < G - P ? g : G - P; }
+
 // Lanes 8 .. 15 of every 16 of a from lanes 0 .. 7 of b (HIGH), or the reverse.
 template <bool HIGH>
 __device__ __forceinline__ uint32_t swap_halves(uint32_t a, uint32_t b) {
@@ -101,7 +114,6 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
       lds + glu_slice_bytes<BITS, GS>(M, (tiles + (int)gridDim.x - 1) / (int)gridDim.x, slice));
 
   u32x4 W[R][2];                                // a line of the gate's rows, and of the up's
-  const uint32_t lo = 16u * (2 * c + (r >> 3));
   const unsigned char *pg = nullptr, *pu = nullptr;
   uint32_t ro = 0;
   // tile j's first row in both matrices, and this lane's row (the last, past N)
@@ -109,12 +121,12 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
     const int64_t n0 = (int64_t)(t0 + j) * kGluCols;
     pg = reinterpret_cast<const unsigned char*>(wg) + n0 * rowB;
     pu = reinterpret_cast<const unsigned char*>(wu) + n0 * rowB;
-    ro = (uint32_t)min(r & 7, (int)(N - 1 - n0)) * rowB;
+    ro = (uint32_t)glu_lane_row(lane, n0, N) * rowB;
   };
-  // unit s of that tile into slot b; chunks past the row read its last one
+  // unit s of that tile into slot b
   auto load = [&](auto bc, int s) {
     constexpr int b = decltype(bc)::value;
-    const uint32_t o = ro + min(128u * (uint32_t)s + lo, rowB - 16u);
+    const uint32_t o = ro + glu_lane_byte(lane, s, rowB);
     W[b][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(pg + o));
     W[b][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(pu + o));
   };
@@ -165,7 +177,7 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
         const int q = i / per, g = g0 + (i - q * per) * P;
         const bool up = q >= rows;
         const int64_t o =
-            (int64_t)min(t0 * kGluCols + (up ? q - rows : q), N - 1) * G + min(g, G - P);
+            (int64_t)min(t0 * kGluCols + (up ? q - rows : q), N - 1) * G + glu_piece_at(g, G, P);
         Piece v;
         v.s = *reinterpret_cast<const V*>((up ? su : sg) + o);
         v.b = *reinterpret_cast<const V*>((up ? bu : bg) + o);
@@ -336,34 +348,40 @@ __global__ __launch_bounds__(64 * kGluWaves) void glu_skinny_kernel(
 // Most LDS of a workgroup.
 constexpr int kGluLdsMax = 160 * 1024 - 1024;
 
+// Workgroups of a launch: one per CU, more where that would be over 16 tiles each; and x and
+// scales in equal slices of whole units, as the LDS of `rows` rows needs.
+struct GluSlices {
+  int64_t wgs, units;
+  size_t lds;
+};
+template <int BITS, int GS>
+inline GluSlices glu_slices(int64_t rows, int64_t tiles, int64_t S, int cus) {
+  const int64_t per = (tiles + (int64_t)cus * kGluTiles - 1) / ((int64_t)cus * kGluTiles);
+  GluSlices p{tiles < cus * per ? tiles : cus * per, S, 0};
+  const int most = (int)((tiles + p.wgs - 1) / p.wgs);
+  for (int64_t n = 1;; ++n) {
+    p.units = (S + n - 1) / n;
+    p.lds = glu_slice_bytes<BITS, GS>(rows, most, (int)p.units) + (p.units < S ? kGluSum : 0);
+    if (p.lds <= (size_t)kGluLdsMax) return p;
+  }
+}
+
 template <int DT, int BITS, int GS>
 int GluSkinnyLaunch<DT, BITS, GS>::run(const GluArgs& a, int64_t m0, int64_t M, int64_t rows,
                                        hipStream_t st) {
   constexpr int UC = GluGeom<BITS>::UC;
   const int64_t tiles = (a.N + kGluCols - 1) / kGluCols, S = (a.K + UC - 1) / UC;
-  const int cus = device_cu_count();
-  // one workgroup per CU, more where that would be over 16 tiles each
-  const int64_t per = (tiles + (int64_t)cus * kGluTiles - 1) / ((int64_t)cus * kGluTiles);
-  const int64_t wgs = tiles < cus * per ? tiles : cus * per;
-  // x and scales in equal slices of whole units
-  const int most = (int)((tiles + wgs - 1) / wgs);
-  int64_t slice = S;
-  size_t lds = 0;
-  for (int64_t n = 1;; ++n) {
-    slice = (S + n - 1) / n;
-    lds = glu_slice_bytes<BITS, GS>(rows, most, (int)slice) + (slice < S ? kGluSum : 0);
-    if (lds <= (size_t)kGluLdsMax) break;
-  }
+  const GluSlices p = glu_slices<BITS, GS>(rows, tiles, S, device_cu_count());
   const auto kern = &glu_skinny_kernel<DT, BITS, GS>;
   static std::atomic<uint64_t> lds_set{0};
   if (hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(kern), kGluLdsMax, lds_set))
     return (int)e;
   const int64_t o = m0 * a.N;
-  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * kGluWaves), lds, st,
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.wgs), dim3(64 * kGluWaves), p.lds, st,
                      (const uint16_t*)a.x + m0 * a.K, a.wg, (const uint16_t*)a.sg,
                      (const uint16_t*)a.bg, a.wu, (const uint16_t*)a.su, (const uint16_t*)a.bu,
                      (uint16_t*)a.out + o, a.gf ? a.gf + o : nullptr, a.uf ? a.uf + o : nullptr,
-                     (int)M, (int)a.N, (int)a.K, a.act, (int)tiles, (int)slice);
+                     (int)M, (int)a.N, (int)a.K, a.act, (int)tiles, (int)p.units);
   return 0;
 }
 
