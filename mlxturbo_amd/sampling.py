@@ -63,7 +63,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     -inf.  Masses are held in integers, so a row's result depends on the row alone.
     In tensors, which are not looked at on the host, a temperature below 0 or NaN is 0,
     top_k below 0 is 0, top_p outside (0, 1) is 1 or, at most 0, the first word alone,
-    and u is moved into [0, 1)."""
+    min_p below 0 is 0 and above 1 or NaN leaves the first word alone, and u is moved into
+    [0, 1)."""
     dev = ops._require_gpu(logits, u)
     if glu.elsewhere(dev):
         with torch.cuda.device(dev):

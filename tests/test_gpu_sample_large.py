@@ -53,6 +53,20 @@ def test_many_tiles_at_odd_places(V, dtype):
         assert tok[2] == V - 1 and lp[2] == 0
 
 
+def test_min_p_outside_its_range():
+    """In a tensor: below 0 all, above 1 and NaN the first word alone, whatever else is set."""
+    g = _gen(3)
+    logits = (torch.randn((4, 5003), generator=g, device="cuda") * 2).to(BF)
+    u = torch.full((4,), 0.97, device="cuda")
+    m = torch.tensor([-0.5, 1.5, float("nan"), 0.0], device="cuda")
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9)):
+        tok, lp = mq.sample(logits, u, min_p=m, **kw)
+        want, wlp = mq.sample(logits, u, **kw)
+        top = logits.float().argmax(-1)
+        assert tok.tolist() == [want[0], top[1], top[2], want[3]]
+        assert lp[0] == wlp[0] and lp[1] == 0 and lp[2] == 0 and lp[3] == wlp[3]
+
+
 OVERFLOWS = [
     dict(top_k=3), dict(top_k=60), dict(top_k=500), dict(top_k=11000), dict(top_k=33333),
     dict(top_p=0.31), dict(top_p=0.9137), dict(top_p=0.99999),
