@@ -25,7 +25,7 @@
 //    operand wants rows 8 .. 15 to be the up matrix's: lanes r < 8 and r >= 8 of a
 //    gate and an up register change places by one DPP move each, after which both hold
 //    chunk 2 c, or 2 c + 1, of 16 rows.
-// Bound by the exact dequantization (20 VALU per 8 codes; v_fma_mix, v_cvt_pk and DPP moves
+// Bound by the exact dequantization (VALU issue 73% of the CUs' busy time; 20 VALU per 8 codes; v_fma_mix, v_cvt_pk and DPP moves
 // issue every 4.9 cycles, and and shift every 2.8) over the 15 us after the scales, whose
 // read and barrier take 5.5, and by the last workgroups' 9 tiles against 8.5 on average:
 // N=17408 K=5120, 4 bits, 25.9, 26.6 and 34.3 us for 2, 8 and 16 rows (100 MB: 20 us at the

@@ -10,7 +10,9 @@
 // value to 2^14 .. 2^15, which the product's sums are divided by: exact, and what falls below
 // float16's smallest number is then below 2^-39 of the row's largest.
 //
-// HBM-bound: 10 bytes read and 8 written per element.  Eight columns per thread.  dg and du
+// HBM-bound: 10 bytes read and 8 written per element, 2048 x 17408 in 119 us, 5.4 TB/s; float16,
+// 301 x 8192, 20 us, of which the second computation and the wait between are half (9.3
+// unscaled).  Eight columns per thread.  dg and du
 // lie side by side in a row, each padded with zeros to whole steps of 64 columns, then
 // their rests.
 #include <hip/hip_runtime.h>

@@ -2,10 +2,12 @@
 // wave's two 32-row blocks on the gate and the up matrix, so that a lane holds
 // both sums of its outputs and each x tile is read once for both.
 //
-// MFMA- and power-bound, as the plain product's tile (dense.cuh): M=2048 N=17408 K=5120
-// 630 us, 1.16 PFLOP/s (a library product of that size 650, over weights already
-// dequantized).  Few rows are bound by the latency of a tile's steps and the sum of the
-// splits: N=9001 K=2560, 8 bits, 45 rows on 3 splits 19.7 + 4.2 us.
+// Many rows: MFMAs, at a clock that power holds near 1.8 GHz, as the plain product's tile
+// (dense.cuh): M=2048 N=17408 K=5120 640 - 680 us, 1.07 - 1.14 PFLOP/s (a library product of that
+// size 650, over weights already dequantized); the MFMA pipes are busy for 71% of the tiles'
+// time, and 1088 tiles take 5 rounds of 256 CUs, the last a quarter full.  Few rows are bound
+// by the latency of a tile's steps (MFMAs 19%, VALU 28%) and the sum of the splits: N=9001
+// K=2560, 8 bits, 45 rows on 3 splits 19.9 + 4.0 us.
 #pragma once
 #include "glu.cuh"
 

@@ -11,9 +11,12 @@
 // (The transposing LDS reads, ds_read_b64_tr_b16, would take the other half too, but
 // the compiler has them wait for every load into LDS that is under way.)
 //
-// MFMA- and power-bound: both matrices of 17408 x 5120, 4 bits, 2048 rows 660 us, 1.1 PFLOP/s
-// (a library product d . W of that size 824), and 24 for the sum of 3 splits; 301 rows of 2 x
-// (8192 x 2048) on 13 splits 44.7 + 6.0, 77 rows of 65536 x 2048 at 8 bits on 28 63.9 + 8.3.
+// Many rows: MFMAs, at a clock that power holds near 1.8 GHz.  Both matrices of 17408 x 5120,
+// 4 bits, 2048 rows of pairs 1400 - 1430 us, 1.04 PFLOP/s of MFMAs, whose pipes are busy for 63%
+// of the tiles' time, and 17 for the sum of 2 splits.  One matrix of 5120 x 17408, 1024 rows
+// 232 - 268 us (51%, 408 tiles on 256 CUs).  Fewer rows: the latency of a step's chain at
+// one wave per SIMD (30 - 36%): 301 rows of pairs of 2 x (8192 x 2048) on 6 splits 65 + 4, 77 rows
+// of 65536 x 2048 at 8 bits on 28 62 + 8.
 #pragma once
 #include "dense.cuh"
 #include "glu_launch.h"

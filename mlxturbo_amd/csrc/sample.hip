@@ -19,9 +19,11 @@
 // One row of 248320 16-bit words is half a megabyte: latency bounds a few rows, so a
 // row is spread over workgroups (chunks of its tiles, up to 1024 of 64 granules or
 // more), and the passes are launches for all rows whatever their settings.  (us of the
-// steps, 248320 bf16 words: one row with k and p 3.2, 5.4 and 10.3 for 3 and 4; 64 rows of
-// mixed settings 10.3, at 3 TB/s of logits, 22.6, of which 13 by instruction count are the double
-// arithmetic of the masses, 18.7 and 16.4.)
+// steps, 248320 bf16 words: one row with k and p 3.3, 5.3 and 10.5 for 3 and 4; 64 rows of
+// mixed settings 10.3, at 3 TB/s of logits, 22.7, 18.7 and 16.4.  Of the 22.7, the double
+// arithmetic of the 22 rows that need masses is about 8 by instruction count; CUs are busy for
+// 60% of the launch, as the other rows' workgroups end at once.  In the last step 64 CUs have
+// a row each.)
 //   1 each tile's first word.  Where k tiles hold a word, the k-th largest of their
 //     first words is no larger than the k-th largest word: a bound (step 2 finds it)
 //     above which lie few more than k words;

@@ -261,8 +261,9 @@ def quantized_glu(x: torch.Tensor, gate, up, activation: str = "silu",
     once (the three calls it replaces round three times).
 
     4- and 8-bit codes with bf16/fp16 activations in the scales' dtype run on the
-    block's kernels: up to 16 rows one that streams both matrices once, more on
-    the MFMA tile.  Other configurations run as two :func:`ops.quantized_matmul`
+    block's kernels: up to 16 rows (32 under :func:`ops.row_identity`) one that streams
+    both matrices once, more on the MFMA tile; K in odd multiples of 32, which the tile does
+    not take, in launches of 16 rows.  Other configurations run as two :func:`ops.quantized_matmul`
     and the activation, as does ``mode="mxfp4"`` (``(w, scales)``, or with None for
     the biases).
 
