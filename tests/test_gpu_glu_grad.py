@@ -211,3 +211,42 @@ def test_gradient_at_any_address(M, N, K, both):
         assert (buf[:off] == 7).all() and (buf[off + M * K:] == 7).all()
         got.append(buf[off:off + M * K])
     assert got[0].isfinite().all() and all(torch.equal(t, got[0]) for t in got)
+
+
+def test_streams_at_once_and_graphs():
+    """float16 steps, whose rows' factors lie in the call's workspace: on two streams at once,
+    and captured, both graphs replayed on streams of their own between eager steps."""
+    cases = [_case(m, 512, 256, 64, 4, HF, 30 + m) for m in (40, 200)]
+    ds = [torch.randn((x.shape[0], 512), generator=g, device="cuda").to(HF) for g, x, *_ in cases]
+
+    def step(i):
+        _, x, gate, _, up, _ = cases[i]
+        leaf = x.detach().requires_grad_()
+        return torch.autograd.grad(mq.quantized_glu(leaf, gate, up), leaf, ds[i])[0]
+
+    want = [step(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want[i]) for i in range(2) for v in got[i])
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(step(i))
+    for n in range(4):
+        for i in range(2):
+            ds[i].mul_(-2.0 if n % 2 else 0.5)
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], step(i))
+        torch.cuda.synchronize()
